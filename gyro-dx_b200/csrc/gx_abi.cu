@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "../../include/gyro_moe.h"
+#include "gx_checks.h"
 #include "gx_comm.h"
 #include "gx_internal.h"
 #include "gx_tile.h"
@@ -60,6 +61,13 @@ struct Layer {
     uint64_t hc_bytes = 0;
     gx::SharedMat hc_down{}, hc_up{}, hc_inject{};
     float *hc_norm = nullptr;
+    // norms, gate and residual scale of the layer as a block of a plain residual stream
+    // (gx_upload_norms), in an arena of its own; a nullptr weight is 1
+    float *nm_arena = nullptr;
+    uint64_t nm_bytes = 0;
+    const float *nm_pre = nullptr, *nm_post = nullptr, *nm_gate = nullptr;
+    bool nm_post_norm = false;
+    float nm_eps = 0.f, nm_res_scale = 1.f, nm_block_scale = 1.f;
 };
 
 // Copies of hot experts one expert-parallel rank can hold per layer, beside its own shard.
@@ -68,6 +76,7 @@ constexpr uint32_t kMaxReplicas = 32;
 struct Matrix {
     uint32_t type = 0, rows = 0, cols = 0;
     uint8_t *tiles = nullptr;
+    uint64_t bytes = 0;
 };
 
 using GraphKey = std::tuple<uint32_t, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t>;
@@ -119,6 +128,7 @@ struct gx_context {
         __half *Ylo = nullptr, *gate = nullptr;
         int *ints = nullptr;  // tile_expert | tile_rows | n_mtiles
     } hc;
+    float *norm_gate = nullptr;      // [max_tokens] gate logits of gx_norm_block (first gx_upload_norms)
     uint32_t *ids = nullptr;
     int *err = nullptr;
     void *x_stage = nullptr, *y_stage = nullptr;     // device staging (graphs, host calls)
@@ -317,6 +327,7 @@ void release_all(gx_context *c) {
         if (l.arena) cudaFree(l.arena);
         if (l.sh_arena) cudaFree(l.sh_arena);
         if (l.hc_arena) cudaFree(l.hc_arena);
+        if (l.nm_arena) cudaFree(l.nm_arena);
     }
     void *sh[] = {c->sh.logit, c->sh.act, c->sh.y, c->sh.A, c->sh.A2, c->sh.pact, c->sh.Ysh, c->sh.ints,
                   c->hc.xn, c->hc.lo, c->hc.inj, c->hc.cur, c->hc.y, c->hc.A, c->hc.A2, c->hc.Ylo, c->hc.gate,
@@ -326,7 +337,8 @@ void release_all(gx_context *c) {
     for (void *p : pf) if (p) cudaFree(p);
     for (auto &m : c->mats) if (m.tiles) cudaFree(m.tiles);
     void *dev[] = {c->codebook, c->codebook_image, c->router_done, c->logits, c->weights, c->xscale, c->ss, c->ids,
-                   c->act, c->xbuf[0], c->xbuf[1], c->x_stage, c->y_stage, c->err, c->stack_table, c->stack_sync};
+                   c->act, c->xbuf[0], c->xbuf[1], c->x_stage, c->y_stage, c->err, c->stack_table, c->stack_sync,
+                   c->norm_gate};
     for (void *p : dev) if (p) cudaFree(p);
     if (c->h_in) cudaFreeHost(c->h_in);
     if (c->h_out) cudaFreeHost(c->h_out);
@@ -351,7 +363,7 @@ void release_all(gx_context *c) {
     if (c->stream) cudaStreamDestroy(c->stream);
 }
 
-size_t dtype_size(uint32_t dt) { return dt == GX_BF16 ? 2 : 4; }
+using gx::dtype_size;
 
 // Phase event: a plain record on the stream, or an event-record node (external record) while
 // the stream is being captured into a graph (a plain record there only orders graph nodes).
@@ -1704,8 +1716,8 @@ GX_API gx_result gx_get_caps(gx_context *c, gx_caps *caps) {
     caps->hbm_bytes = total_b;
     caps->free_bytes = free_b;
     caps->l2_bytes = (uint64_t)prop.l2CacheSize;
-    for (auto &l : c->layers) caps->arena_bytes += l.bytes + l.sh_bytes + l.hc_bytes;
-    for (auto &m : c->mats) caps->arena_bytes += (uint64_t)m.rows / 8 * (m.cols / 128) * gx::tile_bytes(m.type);
+    for (auto &l : c->layers) caps->arena_bytes += l.bytes + l.sh_bytes + l.hc_bytes + l.nm_bytes;
+    for (auto &m : c->mats) caps->arena_bytes += m.bytes;
     std::strncpy(caps->device_name, prop.name, sizeof(caps->device_name) - 1);
     caps->ep_exchange = c->ep.peer_state == 1 ? GX_EP_PEER : c->ep.peer_state == -1 ? GX_EP_NCCL : GX_EP_NONE;
     caps->ep_peer_layers = c->ep.peer_layers;
@@ -1746,6 +1758,7 @@ GX_API gx_result gx_upload_layer(gx_context *c, uint32_t layer, const gx_layer_d
         cudaFree(L.arena);
         if (L.sh_arena) cudaFree(L.sh_arena);
         if (L.hc_arena) cudaFree(L.hc_arena);
+        if (L.nm_arena) cudaFree(L.nm_arena);
         L = Layer{};
     }
     const uint64_t NEl = NE / c->world, first = c->rank * NEl;
@@ -2333,21 +2346,28 @@ GX_API gx_result gx_decode_blocks(gx_context *c, uint32_t type_id, const void *p
 
 GX_API gx_result gx_upload_matrix(gx_context *c, uint32_t type_id, uint32_t rows, uint32_t cols, const void *packed,
                                   uint64_t packed_bytes, uint32_t *out_handle, uint32_t timeout_ms) {
-    if (!c || !packed || !out_handle || !known_type(type_id) || rows == 0 || rows % 8 || cols == 0 || cols % 128 ||
-        cols > 2048)
+    if (!c || !packed || !out_handle || rows == 0 || cols == 0) return GX_E_INVALIDARG;
+    const bool q4 = type_id == GX_Q4_0 || type_id == GX_Q4_1;
+    if (q4) {
+        if (cols % 32 || cols > gx::kQ4MaxCols || rows > gx::kQ4MaxRows) return GX_E_INVALIDARG;
+    } else if (!known_type(type_id) || rows % 8 || cols % 128 || cols > 2048) {
         return GX_E_INVALIDARG;
-    const uint64_t row_bytes = (uint64_t)cols / 128 * gx::type_block_bytes(type_id);
+    }
+    const uint64_t row_bytes = q4 ? gx::q4_row_bytes(type_id, cols) : (uint64_t)cols / 128 * gx::type_block_bytes(type_id);
     if (packed_bytes != row_bytes * rows) return GX_E_INVALIDARG;
     if (c->broken) return GX_E_DEVICE;
     GX_CUDA(cudaSetDevice(c->device));
     // the GEMV takes rows 16 at a time: an odd count of 8-row groups gets a zero group after it
-    const uint64_t pad = rows % 16 ? (uint64_t)gx::tile_bytes(type_id) * (cols / 128) : 0;
+    const uint64_t pad = !q4 && rows % 16 ? (uint64_t)gx::tile_bytes(type_id) * (cols / 128) : 0;
+    const uint64_t bytes = q4 ? gx::q4_bytes(type_id, rows, cols) : packed_bytes + pad;
     uint8_t *raw = nullptr, *tiles = nullptr;
-    GX_CUDA(cudaMalloc(&tiles, packed_bytes + pad));
+    GX_CUDA(cudaMalloc(&tiles, bytes));
     cudaError_t e = cudaMalloc(&raw, packed_bytes);
     if (e == cudaSuccess && pad) e = cudaMemsetAsync(tiles + packed_bytes, 0, pad, c->stream);
     if (e == cudaSuccess) e = cudaMemcpyAsync(raw, packed, packed_bytes, cudaMemcpyHostToDevice, c->stream);
-    if (e == cudaSuccess) e = gx::launch_repack(type_id, raw, row_bytes, rows, cols, tiles, c->stream);
+    if (e == cudaSuccess)
+        e = q4 ? gx::launch_q4_repack(type_id, raw, rows, cols, tiles, c->stream)
+               : gx::launch_repack(type_id, raw, row_bytes, rows, cols, tiles, c->stream);
     gx_result r = e == cudaSuccess ? sync_all(c, timeout_ms) : fail_cuda(c, e);
     if (r != GX_E_TIMEOUT) cudaFree(raw);
     if (r != GX_OK) {
@@ -2359,10 +2379,34 @@ GX_API gx_result gx_upload_matrix(gx_context *c, uint32_t type_id, uint32_t rows
     m.rows = rows;
     m.cols = cols;
     m.tiles = tiles;
+    m.bytes = q4 ? bytes : packed_bytes;
     c->mats.push_back(m);
     *out_handle = (uint32_t)(c->mats.size() - 1);
     return GX_OK;
 }
+
+namespace {
+
+// Enqueues y = W x for a 4-bit matrix.
+gx_result enqueue_q4(gx_context *c, const Matrix &m, const void *x, uint32_t x_dtype, uint64_t ldx, uint32_t n_tok,
+                     void *y, uint32_t y_dtype, uint64_t ldy) {
+    gx::Q4Args a{};
+    a.type = m.type;
+    a.w = m.tiles;
+    a.x = x;
+    a.x_bf16 = x_dtype == GX_BF16;
+    a.ldx = (long long)ldx;
+    a.y = y;
+    a.y_bf16 = y_dtype == GX_BF16;
+    a.ldy = (long long)ldy;
+    a.rows = (int)m.rows;
+    a.cols = (int)m.cols;
+    a.n_tok = (int)n_tok;
+    GX_CUDA(gx::launch_q4_linear(a, c->sm_count, c->stream));
+    return GX_OK;
+}
+
+}  // namespace
 
 GX_API gx_result gx_matvec(gx_context *c, uint32_t handle, const float *x, uint32_t n_tok, float *y,
                            uint64_t *out_ticket) {
@@ -2372,6 +2416,11 @@ GX_API gx_result gx_matvec(gx_context *c, uint32_t handle, const float *x, uint3
     GX_CUDA(cudaSetDevice(c->device));
     if (n_tok) {
         const Matrix &m = c->mats[handle];
+        if (m.type == GX_Q4_0 || m.type == GX_Q4_1) {
+            gx_result r = enqueue_q4(c, m, x, GX_F32, m.cols, n_tok, y, GX_F32, m.rows);
+            if (r != GX_OK) return r;
+            return record_ticket(c, out_ticket);
+        }
         gx::MatvecArgs a{};
         a.type = m.type;
         a.tiles = m.tiles;
@@ -2383,6 +2432,230 @@ GX_API gx_result gx_matvec(gx_context *c, uint32_t handle, const float *x, uint3
         a.n_tok = (int)n_tok;
         a.err = c->err;
         GX_CUDA(gx::launch_matvec(a, c->sm_count, c->stream));
+    }
+    return record_ticket(c, out_ticket);
+}
+
+// ---- operators around the layer --------------------------------------------------------------
+namespace {
+
+// Calls that may be captured from the context's stream: whether it is being captured now. A
+// captured call has no ticket (its event would belong to the graph).
+gx_result check_capture(gx_context *c, const uint64_t *out_ticket, bool *capturing) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    GX_CUDA(cudaStreamIsCapturing(c->stream, &st));
+    *capturing = st != cudaStreamCaptureStatusNone;
+    return *capturing && out_ticket ? GX_E_STATE : GX_OK;
+}
+gx_result finish_call(gx_context *c, bool capturing, uint64_t *out_ticket) {
+    return capturing ? (gx_result)GX_OK : record_ticket(c, out_ticket);
+}
+
+}  // namespace
+
+GX_API gx_result gx_linear(gx_context *c, uint32_t handle, const void *x, uint32_t x_dtype, uint64_t x_stride,
+                           uint32_t n_tok, void *y, uint32_t y_dtype, uint64_t y_stride, uint64_t *out_ticket) {
+    if (!c || handle >= c->mats.size()) return GX_E_INVALIDARG;
+    const Matrix &m = c->mats[handle];
+    if (m.type != GX_Q4_0 && m.type != GX_Q4_1) return GX_E_UNSUPPORTED;
+    if (!gx::linear_args_ok(m.rows, m.cols, x, x_dtype, x_stride, n_tok, y, y_dtype, y_stride)) return GX_E_INVALIDARG;
+    if (c->broken) return GX_E_DEVICE;
+    GX_CUDA(cudaSetDevice(c->device));
+    bool capturing = false;
+    gx_result r = check_capture(c, out_ticket, &capturing);
+    if (r != GX_OK) return r;
+    if (n_tok) {
+        r = enqueue_q4(c, m, x, x_dtype, x_stride, n_tok, y, y_dtype, y_stride);
+        if (r != GX_OK) return r;
+    }
+    return finish_call(c, capturing, out_ticket);
+}
+
+GX_API gx_result gx_norm(gx_context *c, const gx_norm_desc *d, uint32_t n_tok, uint64_t *out_ticket) {
+    if (!c || !d || !gx::norm_args_ok(*d, n_tok)) return GX_E_INVALIDARG;
+    if (c->broken) return GX_E_DEVICE;
+    GX_CUDA(cudaSetDevice(c->device));
+    bool capturing = false;
+    gx_result r = check_capture(c, out_ticket, &capturing);
+    if (r != GX_OK) return r;
+    gx::NormArgs a{};
+    a.x = d->x;
+    a.x_bf16 = d->x_dtype == GX_BF16;
+    a.ldx = (long long)d->x_stride;
+    a.w = d->weight;
+    a.y = d->y;
+    a.y_bf16 = d->y_dtype == GX_BF16;
+    a.ldy = (long long)d->y_stride;
+    a.gate_w = d->gate_weight;
+    a.gate = d->gate;
+    a.n_tok = (int)n_tok;
+    a.E = (int)d->n_embd;
+    a.eps = d->eps;
+    GX_CUDA(gx::launch_norm(a, c->stream));
+    return finish_call(c, capturing, out_ticket);
+}
+
+GX_API gx_result gx_norm_residual(gx_context *c, const gx_residual_desc *d, uint32_t n_tok, uint64_t *out_ticket) {
+    if (!c || !d || !gx::residual_args_ok(*d, n_tok)) return GX_E_INVALIDARG;
+    if (c->broken) return GX_E_DEVICE;
+    GX_CUDA(cudaSetDevice(c->device));
+    bool capturing = false;
+    gx_result r = check_capture(c, out_ticket, &capturing);
+    if (r != GX_OK) return r;
+    gx::ResidualArgs a{};
+    a.y = d->y;
+    a.y_bf16 = d->y_dtype == GX_BF16;
+    a.ldy = (long long)d->y_stride;
+    a.res = d->res;
+    a.res_bf16 = d->res_dtype == GX_BF16;
+    a.ldr = (long long)d->res_stride;
+    a.res_out = d->res_out;
+    a.ldro = (long long)d->res_out_stride;
+    a.post_norm = (d->flags & GX_RES_POST_NORM) != 0;
+    a.post = d->post;
+    a.gate_kind = (int)d->gate_kind;
+    a.gate = d->gate;
+    a.gate_bf16 = d->gate_dtype == GX_BF16;
+    a.ldg = (long long)d->gate_stride;
+    a.out = d->out;
+    a.out_bf16 = d->out_dtype == GX_BF16;
+    a.ldo = (long long)d->out_stride;
+    a.next = d->next;
+    a.next_gate_w = d->next_gate_weight;
+    a.next_gate = d->next_gate;
+    a.n_tok = (int)n_tok;
+    a.E = (int)d->n_embd;
+    a.eps = a.next_eps = d->eps;
+    a.res_scale = d->res_scale;
+    a.block_scale = d->block_scale;
+    GX_CUDA(gx::launch_norm_residual(a, c->stream));
+    return finish_call(c, capturing, out_ticket);
+}
+
+GX_API gx_result gx_logprobs(gx_context *c, const gx_logprobs_desc *d, uint32_t n_rows, uint64_t *out_ticket) {
+    if (!c || !d || !gx::logprobs_args_ok(*d, n_rows)) return GX_E_INVALIDARG;
+    if (c->broken) return GX_E_DEVICE;
+    GX_CUDA(cudaSetDevice(c->device));
+    bool capturing = false;
+    gx_result r = check_capture(c, out_ticket, &capturing);
+    if (r != GX_OK) return r;
+    gx::LogprobsArgs a{};
+    a.logits = d->logits;
+    a.bf16 = d->dtype == GX_BF16;
+    a.stride = (long long)d->stride;
+    a.tokens = d->tokens;
+    a.logprob = d->logprob;
+    a.rank = d->rank;
+    a.entropy = d->entropy;
+    a.top_ids = d->top_ids;
+    a.top_logprobs = d->top_logprobs;
+    a.n_rows = (int)n_rows;
+    a.n_vocab = (int)d->n_vocab;
+    a.n_top = (d->top_ids || d->top_logprobs) ? (int)d->n_top : 0;
+    a.scale = d->scale;
+    a.err = c->err;
+    GX_CUDA(gx::launch_logprobs(a, c->sm_count, c->stream));
+    return finish_call(c, capturing, out_ticket);
+}
+
+GX_API gx_result gx_upload_norms(gx_context *c, uint32_t layer, const gx_norms_desc *d, uint32_t timeout_ms) {
+    if (!c) return GX_E_INVALIDARG;
+    if (c->broken) return GX_E_DEVICE;
+    if (layer >= c->layers.size() || !c->layers[layer].ready) return GX_E_STATE;
+    Layer &L = c->layers[layer];
+    const uint64_t E = L.E;
+    if (d && !gx::norms_args_ok(*d)) return GX_E_INVALIDARG;
+    GX_CUDA(cudaSetDevice(c->device));
+    if (L.nm_arena) {
+        gx_result r = sync_all(c, timeout_ms);  // queued blocks may still read the old weights
+        if (r != GX_OK) return r;
+        cudaFree(L.nm_arena);
+    }
+    L.nm_arena = nullptr;
+    L.nm_bytes = 0;
+    L.nm_pre = L.nm_post = L.nm_gate = nullptr;
+    if (!d) return GX_OK;
+    if (!c->norm_gate) GX_CUDA(cudaMalloc(&c->norm_gate, (size_t)c->max_tokens * sizeof(float)));
+    float *arena = nullptr;
+    GX_CUDA(cudaMalloc(&arena, 3 * E * sizeof(float)));
+    const float *src[3] = {d->pre, d->post, d->gate};
+    cudaError_t e = cudaSuccess;
+    for (int i = 0; i < 3 && e == cudaSuccess; ++i)
+        if (src[i]) e = cudaMemcpy(arena + i * E, src[i], E * sizeof(float), cudaMemcpyHostToDevice);
+    if (e != cudaSuccess) {
+        cudaFree(arena);
+        return fail_cuda(c, e);
+    }
+    L.nm_arena = arena;
+    L.nm_bytes = 3 * E * sizeof(float);
+    L.nm_pre = d->pre ? arena : nullptr;
+    L.nm_post = d->post ? arena + E : nullptr;
+    L.nm_gate = d->gate ? arena + 2 * E : nullptr;
+    L.nm_post_norm = d->post_norm != 0;
+    L.nm_eps = d->eps;
+    L.nm_res_scale = d->res_scale;
+    L.nm_block_scale = d->block_scale;
+    return GX_OK;
+}
+
+GX_API gx_result gx_norm_block(gx_context *c, uint32_t first, uint32_t n_layers, float *res, uint32_t n_tok,
+                               uint64_t *out_ticket) {
+    if (!c || n_layers == 0 || (uint64_t)first + n_layers > c->layers.size()) return GX_E_INVALIDARG;
+    for (uint32_t i = 0; i < n_layers; ++i) {
+        gx_result r = check_forward(c, first + i, GX_F32, n_tok, GX_F32);
+        if (r != GX_OK) return r;
+        if (!c->layers[first + i].nm_arena) return GX_E_STATE;
+        if (c->layers[first + i].E != c->layers[first].E) return GX_E_INVALIDARG;
+    }
+    if (n_tok > 0 && (!res || ((uintptr_t)res & 15))) return GX_E_INVALIDARG;
+    GX_CUDA(cudaSetDevice(c->device));
+    if (c->world > 1) {  // every rank takes part in the layers' exchange, also with no tokens
+        gx_result r = ep_sync_ntok(c, n_tok);
+        if (r != GX_OK) return r;
+    } else if (n_tok == 0) {
+        return record_ticket(c, out_ticket);
+    }
+    const long long E = c->layers[first].E;
+    float *h = c->xbuf[0], *y = c->xbuf[1];
+    {
+        const Layer &L = c->layers[first];
+        gx::NormArgs a{};
+        a.x = res;
+        a.ldx = a.ldy = E;
+        a.w = L.nm_pre;
+        a.y = h;
+        a.gate_w = L.nm_gate;
+        a.gate = L.nm_gate ? c->norm_gate : nullptr;
+        a.n_tok = (int)n_tok;
+        a.E = (int)E;
+        a.eps = L.nm_eps;
+        GX_CUDA(gx::launch_norm(a, c->stream));
+    }
+    for (uint32_t i = 0; i < n_layers; ++i) {
+        const Layer &L = c->layers[first + i];
+        const Layer *N = i + 1 < n_layers ? &c->layers[first + i + 1] : nullptr;
+        gx_result r = enqueue_layer(c, L, h, GX_F32, n_tok, nullptr, GX_F32, y, GX_F32, -1, 0.f, false);
+        if (r != GX_OK) return r;
+        gx::ResidualArgs a{};
+        a.y = y;
+        a.res = res;
+        a.res_out = res;
+        a.ldy = a.ldr = a.ldro = a.ldo = E;
+        a.post_norm = L.nm_post_norm;
+        a.post = L.nm_post;
+        a.gate_kind = L.nm_gate ? GX_GATE_TOKEN : GX_GATE_NONE;
+        a.gate = L.nm_gate ? c->norm_gate : nullptr;
+        a.out = N ? h : nullptr;
+        a.next = N ? N->nm_pre : nullptr;
+        a.next_gate_w = N ? N->nm_gate : nullptr;
+        a.next_gate = N && N->nm_gate ? c->norm_gate : nullptr;
+        a.n_tok = (int)n_tok;
+        a.E = (int)E;
+        a.eps = L.nm_eps;
+        a.next_eps = N ? N->nm_eps : 0.f;
+        a.res_scale = L.nm_res_scale;
+        a.block_scale = L.nm_block_scale;
+        GX_CUDA(gx::launch_norm_residual(a, c->stream));
     }
     return record_ticket(c, out_ticket);
 }

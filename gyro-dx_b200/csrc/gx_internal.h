@@ -396,6 +396,83 @@ struct MatvecArgs {
     int *err;
 };
 
+// ---- operators around the layer: 4-bit matrices, norms, log probabilities --------------------
+// A 4-bit matrix with group scales (GGUF type ids 2 and 3) on the device.
+struct Q4Args {
+    uint32_t type;           // GX_Q4_0 or GX_Q4_1
+    const uint8_t *w;        // q4_bytes(...) as launch_q4_repack lays them out
+    const void *x;           // [n_tok][cols] at stride ldx
+    int x_bf16;
+    long long ldx;
+    void *y;                 // [n_tok][rows] at stride ldy
+    int y_bf16;
+    long long ldy;
+    int rows, cols, n_tok;
+};
+uint64_t q4_row_bytes(uint32_t type, uint64_t cols);               // of the model file's layout
+uint64_t q4_bytes(uint32_t type, uint64_t rows, uint64_t cols);    // of the device layout
+cudaError_t launch_q4_repack(uint32_t type, const uint8_t *raw, uint32_t rows, uint32_t cols, uint8_t *w,
+                             cudaStream_t s);
+cudaError_t launch_q4_linear(const Q4Args &a, int sm_count, cudaStream_t s);
+
+struct NormArgs {
+    const void *x;
+    int x_bf16;
+    long long ldx;
+    const float *w;          // [E] or nullptr
+    void *y;
+    int y_bf16;
+    long long ldy;
+    const float *gate_w;     // [E] or nullptr
+    float *gate;             // [n_tok] gate_w . y
+    int n_tok, E;
+    float eps;
+};
+cudaError_t launch_norm(const NormArgs &a, cudaStream_t s);
+
+struct ResidualArgs {
+    const void *y;           // the block's output
+    int y_bf16;
+    long long ldy;
+    const void *res;
+    int res_bf16;            // of res and res_out
+    long long ldr;
+    void *res_out;
+    long long ldro;
+    int post_norm;
+    const float *post;       // [E] or nullptr
+    int gate_kind;           // GX_GATE_*
+    const void *gate;
+    int gate_bf16;
+    long long ldg;
+    void *out;               // the next norm's output, or nullptr
+    int out_bf16;
+    long long ldo;
+    const float *next;       // [E] or nullptr
+    const float *next_gate_w;
+    float *next_gate;
+    int n_tok, E;
+    float eps, next_eps, res_scale, block_scale;
+};
+cudaError_t launch_norm_residual(const ResidualArgs &a, cudaStream_t s);
+
+constexpr int kMaxTop = 32;
+struct LogprobsArgs {
+    const void *logits;
+    int bf16;
+    long long stride;
+    const uint32_t *tokens;  // [n_rows] or nullptr
+    float *logprob;
+    uint32_t *rank;
+    float *entropy;
+    uint32_t *top_ids;
+    float *top_logprobs;
+    int n_rows, n_vocab, n_top;
+    float scale;
+    int *err;                // KERR_BOUNDS for a token id past n_vocab
+};
+cudaError_t launch_logprobs(const LogprobsArgs &a, int sm_count, cudaStream_t s);
+
 // pdl: launch with programmatic stream serialization (overlap with the previous kernel).
 // with_topk: also launch the per-token selection kernel (when gate_up does not fuse it).
 cudaError_t launch_router(const RouterArgs &a, cudaStream_t s, bool pdl, bool with_topk);

@@ -21,6 +21,10 @@ ERRORS = {-1: "GX_E_INVALIDARG", -2: "GX_E_OUTOFMEMORY", -3: "GX_E_TIMEOUT", -4:
           -5: "GX_E_UNSUPPORTED", -6: "GX_E_STATE", -7: "GX_E_MISMATCH", -8: "GX_E_COMM", -9: "GX_E_KERNEL",
           -10: "GX_E_RANGE"}
 GX_F32, GX_Q8_0, GX_BF16 = 0, 8, 30
+GX_Q4_0, GX_Q4_1 = 2, 3                           # 4-bit matrices with group scales (upload_matrix)
+GX_RES_POST_NORM = 1
+GX_GATE_NONE, GX_GATE_TOKEN, GX_GATE_ELEMENT = 0, 1, 2
+GX_NO_TOKEN, GX_MAX_TOP = 0xFFFFFFFF, 32
 GX_FLAG_PROFILE = 1
 GX_EP_NONE, GX_EP_NCCL, GX_EP_PEER = 0, 1, 2     # gx_caps.ep_exchange
 
@@ -78,6 +82,37 @@ class GgufLayerInfo(ctypes.Structure):
 GX_SHARED_NONE = 0xFFFFFFFF
 
 
+class NormDesc(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("weight", ctypes.c_void_p),
+                ("gate_weight", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("x_stride", ctypes.c_uint64),
+                ("y_stride", ctypes.c_uint64), ("x_dtype", ctypes.c_uint32), ("y_dtype", ctypes.c_uint32),
+                ("n_embd", ctypes.c_uint32), ("eps", ctypes.c_float)]
+
+
+class ResidualDesc(ctypes.Structure):
+    _fields_ = [("y", ctypes.c_void_p), ("res", ctypes.c_void_p), ("res_out", ctypes.c_void_p),
+                ("gate", ctypes.c_void_p), ("post", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("next", ctypes.c_void_p), ("next_gate_weight", ctypes.c_void_p), ("next_gate", ctypes.c_void_p),
+                ("y_stride", ctypes.c_uint64), ("res_stride", ctypes.c_uint64), ("res_out_stride", ctypes.c_uint64),
+                ("gate_stride", ctypes.c_uint64), ("out_stride", ctypes.c_uint64), ("y_dtype", ctypes.c_uint32),
+                ("res_dtype", ctypes.c_uint32), ("gate_dtype", ctypes.c_uint32), ("out_dtype", ctypes.c_uint32),
+                ("n_embd", ctypes.c_uint32), ("flags", ctypes.c_uint32), ("gate_kind", ctypes.c_uint32),
+                ("eps", ctypes.c_float), ("res_scale", ctypes.c_float), ("block_scale", ctypes.c_float)]
+
+
+class LogprobsDesc(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("tokens", ctypes.c_void_p), ("logprob", ctypes.c_void_p),
+                ("rank", ctypes.c_void_p), ("entropy", ctypes.c_void_p), ("top_ids", ctypes.c_void_p),
+                ("top_logprobs", ctypes.c_void_p), ("stride", ctypes.c_uint64), ("dtype", ctypes.c_uint32),
+                ("n_vocab", ctypes.c_uint32), ("n_top", ctypes.c_uint32), ("scale", ctypes.c_float)]
+
+
+class NormsDesc(ctypes.Structure):
+    _fields_ = [("pre", ctypes.c_void_p), ("post", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+                ("post_norm", ctypes.c_uint32), ("eps", ctypes.c_float), ("res_scale", ctypes.c_float),
+                ("block_scale", ctypes.c_float)]
+
+
 class Timings(ctypes.Structure):
     _fields_ = [("router_ns", ctypes.c_uint64), ("gate_up_ns", ctypes.c_uint64), ("down_ns", ctypes.c_uint64),
                 ("experts_ns", ctypes.c_uint64), ("total_ns", ctypes.c_uint64), ("layers", ctypes.c_uint64)]
@@ -85,6 +120,9 @@ class Timings(ctypes.Structure):
 
 assert ctypes.sizeof(Options) == 168 and ctypes.sizeof(Caps) == 192 and ctypes.sizeof(LayerDesc) == 112
 assert ctypes.sizeof(SharedDesc) == 64 and ctypes.sizeof(GgufLayerInfo) == 40 and ctypes.sizeof(HcDesc) == 72
+
+assert ctypes.sizeof(NormDesc) == 72 and ctypes.sizeof(ResidualDesc) == 152
+assert ctypes.sizeof(LogprobsDesc) == 80 and ctypes.sizeof(NormsDesc) == 40
 
 # (name, argtypes) of every exported entry point; include/gyro_moe.h declares exactly these.
 _P, _U32, _U64, _F = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_float
@@ -108,6 +146,12 @@ SIGNATURES = {
     "gx_decode_blocks": [_P, _U32, _P, _U64, _P, _U32, _P, ctypes.POINTER(_F), _U32],
     "gx_upload_matrix": [_P, _U32, _U32, _U32, _P, _U64, ctypes.POINTER(_U32), _U32],
     "gx_matvec": [_P, _U32, _P, _U32, _P, ctypes.POINTER(_U64)],
+    "gx_linear": [_P, _U32, _P, _U32, _U64, _U32, _P, _U32, _U64, ctypes.POINTER(_U64)],
+    "gx_norm": [_P, ctypes.POINTER(NormDesc), _U32, ctypes.POINTER(_U64)],
+    "gx_norm_residual": [_P, ctypes.POINTER(ResidualDesc), _U32, ctypes.POINTER(_U64)],
+    "gx_logprobs": [_P, ctypes.POINTER(LogprobsDesc), _U32, ctypes.POINTER(_U64)],
+    "gx_upload_norms": [_P, _U32, ctypes.POINTER(NormsDesc), _U32],
+    "gx_norm_block": [_P, _U32, _U32, _P, _U32, ctypes.POINTER(_U64)],
     "gx_read_timings": [_P, ctypes.POINTER(Timings)],
     "gx_read_expert_counts": [_P, _U32, _P, _U32, _U32],
     "gx_replicate_experts": [_P, _U32, _P, _U32, _U32],
@@ -179,6 +223,33 @@ def unique_id() -> bytes:
     return buf.raw
 
 
+def _rows(a, width: int | None = None) -> tuple[int, int, int]:
+    """(pointer, row stride in elements, dtype code) of a device tensor of rows (1-D: one row)."""
+    if a.ndim not in (1, 2) or a.stride(-1) != 1 and a.shape[-1] > 1:
+        raise ValueError("rows must be contiguous, in a tensor of one or two dimensions")
+    w = a.shape[-1]
+    if width is not None and w != width:
+        raise ValueError(f"rows of {w} values where {width} are needed")
+    n = a.shape[0] if a.ndim == 2 else 1
+    return a.data_ptr(), (a.stride(0) if n > 1 else w), _dtype_code(a)
+
+
+def _n_rows(a) -> int:
+    return a.shape[0] if a.ndim == 2 else 1
+
+
+def _words(a, n: int, what: str, dtypes=("float32",)) -> int | None:
+    """Pointer of a contiguous device vector of n 32-bit words, or None."""
+    if a is None:
+        return None
+    if a.numel() != n or not a.is_contiguous() or str(a.dtype).removeprefix("torch.") not in dtypes:
+        raise ValueError(f"{what}: {n} contiguous values of type {' or '.join(dtypes)} are needed")
+    return a.data_ptr()
+
+
+_IDS = ("int32", "uint32")
+
+
 class Context:
     """One device context (gx_create ... gx_destroy)."""
 
@@ -196,6 +267,7 @@ class Context:
         self.handle = h
         self.max_tokens = max_tokens
         self.layers: dict[int, dict] = {}
+        self.matrices: dict[int, tuple[int, int]] = {}   # (rows, cols) by handle
 
     # --- lifecycle -----------------------------------------------------------------------
     def close(self, timeout_ms: int = 60000) -> None:
@@ -371,9 +443,102 @@ class Context:
         h = ctypes.c_uint32()
         _check(self.lib.gx_upload_matrix(self.handle, type_id, rows, cols, p.ctypes.data, p.nbytes, ctypes.byref(h),
                                          timeout_ms), "gx_upload_matrix")
+        self.matrices[h.value] = (rows, cols)
         return h.value
 
     def matvec(self, handle: int, x, y) -> int:
         t = ctypes.c_uint64()
         _check(self.lib.gx_matvec(self.handle, handle, _ptr(x), x.shape[0], _ptr(y), ctypes.byref(t)), "gx_matvec")
+        return t.value
+
+    # --- operators around the layer ----------------------------------------------------------
+    # Device tensors of this context's device, rows in the last dimension; the work is enqueued on the
+    # context's stream. Each returns the ticket, or 0 with ticket=False (calls captured into a graph).
+    def _call(self, name: str, *args, ticket: bool = True) -> int:
+        t = ctypes.c_uint64() if ticket else None
+        rc = getattr(self.lib, name)(self.handle, *args, ctypes.byref(t) if ticket else None)
+        if rc != GX_OK:
+            raise GxError(rc, name)
+        return t.value if ticket else 0
+
+    def linear(self, handle: int, x, y, ticket: bool = True) -> int:
+        """gx_linear: y = W x for a 4-bit matrix, x [n, cols] and y [n, rows] in f32 or bf16, n <= 64."""
+        xp, xs, xd = _rows(x)
+        yp, ys, yd = _rows(y)
+        n = _n_rows(x)
+        rows, cols = self.matrices[handle]
+        if _n_rows(y) != n or x.shape[-1] != cols or y.shape[-1] != rows:
+            raise ValueError("gx_linear: x [n, cols] and y [n, rows] are needed")
+        return self._call("gx_linear", handle, xp, xd, xs, n, yp, yd, ys, ticket=ticket)
+
+    def norm(self, x, y, weight=None, eps: float = 1e-6, gate_weight=None, gate=None, ticket: bool = True) -> int:
+        """gx_norm: y = norm(x) * weight, and gate = gate_weight . y for each row."""
+        n, w = _n_rows(x), x.shape[-1]
+        xp, xs, xd = _rows(x)
+        yp, ys, yd = _rows(y, w)
+        if _n_rows(y) != n:
+            raise ValueError("gx_norm: as many rows in y as in x are needed")
+        d = NormDesc(xp, yp, _words(weight, w, "weight"), _words(gate_weight, w, "gate_weight"), _words(gate, n, "gate"),
+                     xs, ys, xd, yd, w, eps)
+        return self._call("gx_norm", ctypes.byref(d), n, ticket=ticket)
+
+    def norm_residual(self, y, res, res_out=None, post=None, post_norm: bool = True, eps: float = 1e-6,
+                      res_scale: float = 1.0, block_scale: float = 1.0, gate=None, out=None, next_weight=None,
+                      next_gate_weight=None, next_gate=None, ticket: bool = True) -> int:
+        """gx_norm_residual: res_out = res_scale * res + block_scale * gate * norm(y; post) (y itself
+        without post_norm), out = norm(res_out; next_weight). res_out None: res in place. gate: one f32
+        logit per row (1-D) or one logit per element (2-D)."""
+        n, w = _n_rows(y), y.shape[-1]
+        yp, ys, yd = _rows(y)
+        rp, rs, rd = _rows(res, w)
+        op, os_, od = _rows(res_out, w) if res_out is not None else (rp, rs, rd)
+        gp, gs, gd, kind = None, 0, GX_F32, GX_GATE_NONE
+        if gate is not None and gate.ndim == 1:
+            gp, kind = _words(gate, n, "gate"), GX_GATE_TOKEN
+        elif gate is not None:
+            (gp, gs, gd), kind = _rows(gate, w), GX_GATE_ELEMENT
+        hp, hs, hd = _rows(out, w) if out is not None else (None, 0, GX_F32)
+        if od != rd or any(_n_rows(a) != n for a in (res, res_out, out, gate if kind == GX_GATE_ELEMENT else None)
+                           if a is not None):
+            raise ValueError("gx_norm_residual: equal numbers of rows, and res_out in the type of res, are needed")
+        d = ResidualDesc(yp, rp, op, gp, _words(post, w, "post"), hp, _words(next_weight, w, "next_weight"),
+                         _words(next_gate_weight, w, "next_gate_weight"), _words(next_gate, n, "next_gate"),
+                         ys, rs, os_, gs, hs, yd, rd, gd, hd, w, GX_RES_POST_NORM if post_norm else 0, kind,
+                         eps, res_scale, block_scale)
+        return self._call("gx_norm_residual", ctypes.byref(d), n, ticket=ticket)
+
+    def logprobs(self, logits, tokens=None, n_top: int = 0, scale: float = 1.0, logprob=None, rank=None, entropy=None,
+                 top_ids=None, top_logprobs=None, ticket: bool = True) -> int:
+        """gx_logprobs over rows of logits [n, vocab]; tokens, rank and top_ids are 32-bit integers."""
+        n, v = _n_rows(logits), logits.shape[-1]
+        p, s, dt = _rows(logits)
+        d = LogprobsDesc(p, _words(tokens, n, "tokens", _IDS), _words(logprob, n, "logprob"),
+                         _words(rank, n, "rank", _IDS), _words(entropy, n, "entropy"),
+                         _words(top_ids, n * n_top, "top_ids", _IDS) if n_top or top_ids is not None and top_ids.numel() else None,
+                         _words(top_logprobs, n * n_top, "top_logprobs")
+                         if n_top or top_logprobs is not None and top_logprobs.numel() else None,
+                         s, dt, v, n_top, scale)
+        return self._call("gx_logprobs", ctypes.byref(d), n, ticket=ticket)
+
+    def upload_norms(self, index: int, norms: dict | None, timeout_ms: int = 600000) -> None:
+        """gx_upload_norms: pre, post and gate weights ([n_embd] f32 or None), post_norm, eps, res_scale and
+        block_scale of a layer as a block of a residual stream, or None to drop them."""
+        if norms is None:
+            _check(self.lib.gx_upload_norms(self.handle, index, None, timeout_ms), "gx_upload_norms")
+            return
+        w = {}
+        for k in ("pre", "post", "gate"):
+            a = norms.get(k)
+            w[k] = None if a is None else np.ascontiguousarray(a, dtype=np.float32)
+            if a is not None and w[k].shape != (self.layers[index]["n_embd"],):
+                raise ValueError(f"{k}: one weight per hidden channel is needed")
+        d = NormsDesc(_ptr(w["pre"]), _ptr(w["post"]), _ptr(w["gate"]), int(norms.get("post_norm", True)),
+                      norms.get("eps", 1e-6), norms.get("res_scale", 1.0), norms.get("block_scale", 1.0))
+        _check(self.lib.gx_upload_norms(self.handle, index, ctypes.byref(d), timeout_ms), "gx_upload_norms")
+
+    def norm_block(self, first: int, n_layers: int, res) -> int:
+        """gx_norm_block on a device f32 tensor res [n, n_embd], updated in place. Returns the ticket."""
+        t = ctypes.c_uint64()
+        _check(self.lib.gx_norm_block(self.handle, first, n_layers, _ptr(res), res.shape[0], ctypes.byref(t)),
+               "gx_norm_block")
         return t.value

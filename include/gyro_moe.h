@@ -61,6 +61,12 @@ enum {
  * src/kernels.zig:7-10). */
 enum { GX_F32 = 0, GX_Q8_0 = 8, GX_BF16 = 30 };
 
+/* 4-bit weights with group scales (GGUF type ids), for gx_upload_matrix: rows of groups of 32
+ * weights, each group an fp16 scale d (GX_Q4_1: then an fp16 minimum m) and 16 bytes of codes,
+ * weight j in the low half of byte j, weight j + 16 in its high half (j < 16).
+ *   GX_Q4_0: w = d * (q - 8), 18 bytes a group;   GX_Q4_1: w = d * q + m, 20 bytes a group. */
+enum { GX_Q4_0 = 2, GX_Q4_1 = 3 };
+
 /* Options: mirrors the role of gd_options (native/include/gyro_native.h:25-31). */
 enum {
     GX_FLAG_PROFILE = 1u      /* record per-phase device times (gx_read_timings) */
@@ -312,12 +318,125 @@ GX_API gx_result gx_decode_blocks(gx_context *context, uint32_t type_id, const v
  * (shaders/engine/moe.hlsl:108-211) and Engine.mv for Gyro weights:
  *   y[t][r] = sum_c W[r][c] * x[t][c],  W [rows][cols] packed (reference layout, host),
  * x [n_tok][cols] f32 device, y [n_tok][rows] f32 device, n_tok <= 64. gx_upload_matrix returns
- * a handle (index) owned by the context. */
+ * a handle (index) owned by the context. Gyro types (144..151): rows a multiple of 8, cols a
+ * multiple of 128 up to 2048. GX_Q4_0 and GX_Q4_1: any rows from 1 to 2^24, cols a multiple of
+ * 32 up to 65536. */
 GX_API gx_result gx_upload_matrix(gx_context *context, uint32_t type_id, uint32_t rows, uint32_t cols,
                                   const void *packed, uint64_t packed_bytes, uint32_t *out_handle,
                                   uint32_t timeout_ms);
 GX_API gx_result gx_matvec(gx_context *context, uint32_t handle, const float *x, uint32_t n_tok,
                            float *y, uint64_t *out_ticket);
+
+/* ---- operators around the routed layer ------------------------------------------------------
+ * What a host computes directly next to the layer: its dense projections and output head in 4 bits,
+ * the norms and residual adds around a block, and the log probabilities of the head's answer. All
+ * pointers are device pointers, all work is enqueued on the context's stream and completes with the
+ * ticket (out_ticket may be NULL). gx_linear, gx_norm, gx_norm_residual and gx_logprobs allocate no
+ * memory and do not wait, so they can be captured into a graph from that stream (with a NULL ticket:
+ * a captured call has none, and one that asks for it gets GX_E_STATE). Row strides are in elements, at least
+ * the row's width, and pointers need only the alignment of their element type. An output may not
+ * overlap an input or another output except where that is said; such calls are refused. Sums,
+ * norms and softmax statistics are f32 or wider, each output is rounded once. */
+
+/* gx_matvec for GX_Q4_0 / GX_Q4_1 matrices with activations and results in either encoding:
+ * x [n_tok][cols] at row stride x_stride, y [n_tok][rows] at row stride y_stride, n_tok <= 64. The
+ * products are those of the exact weights (no weight is rounded); an f32 activation keeps 22 bits
+ * relative to the largest of its token. A token with an Inf or NaN gets NaN in all its results.
+ * A Gyro matrix gives GX_E_UNSUPPORTED. */
+GX_API gx_result gx_linear(gx_context *context, uint32_t handle, const void *x, uint32_t x_dtype, uint64_t x_stride,
+                           uint32_t n_tok, void *y, uint32_t y_dtype, uint64_t y_stride, uint64_t *out_ticket);
+
+/* Norm before a block: y[t] = x[t] / sqrt(mean(x[t]^2) + eps) * weight (src/kernels.zig:281-291),
+ * and, with gate_weight, the block's gate logit gate[t] = sum_i gate_weight[i] * y[t][i] (from the
+ * unrounded y). Rows of n_embd values, 1..65536, at any number of tokens. */
+typedef struct gx_norm_desc {
+    const void *x;                /* [n_tok][n_embd] */
+    void *y;                      /* [n_tok][n_embd]; may be x itself (same pointer, stride and encoding) */
+    const float *weight;          /* [n_embd], or NULL for 1 */
+    const float *gate_weight;     /* [n_embd], or NULL */
+    float *gate;                  /* [n_tok], with gate_weight; else NULL */
+    uint64_t x_stride, y_stride;
+    uint32_t x_dtype, y_dtype;    /* GX_F32 or GX_BF16 */
+    uint32_t n_embd;
+    float eps;                    /* >= 0, finite */
+} gx_norm_desc;                   /* 72 bytes */
+GX_API gx_result gx_norm(gx_context *context, const gx_norm_desc *desc, uint32_t n_tok, uint64_t *out_ticket);
+
+/* Norm after a block fused with its gate, its residual add and the norm before the next block:
+ *   v = y[t], or y[t] / sqrt(mean(y[t]^2) + eps) * post          (GX_RES_POST_NORM)
+ *   r = res_scale * res[t] + block_scale * gate * v,  gate = 1, sigmoid(g[t]) or sigmoid(g[t][i])
+ *   res_out[t] = r;   out[t] = r / sqrt(mean(r^2) + eps) * next;  next_gate[t] = next_gate_weight . out[t]
+ * The next norm sees r before it is rounded to res_out's encoding. */
+enum { GX_RES_POST_NORM = 1u };
+enum { GX_GATE_NONE = 0, GX_GATE_TOKEN = 1, GX_GATE_ELEMENT = 2 };
+typedef struct gx_residual_desc {
+    const void *y;                /* [n_tok][n_embd] the block's output */
+    const void *res;              /* [n_tok][n_embd] the residual stream */
+    void *res_out;                /* [n_tok][n_embd] in res_dtype; may be res itself (same pointer and stride) */
+    const void *gate;             /* GX_GATE_TOKEN: [n_tok] f32; GX_GATE_ELEMENT: [n_tok][n_embd]; else NULL */
+    const float *post;            /* [n_embd] with GX_RES_POST_NORM (NULL for 1) */
+    void *out;                    /* [n_tok][n_embd] the next block's input, or NULL for no next norm */
+    const float *next;            /* [n_embd] with out (NULL for 1) */
+    const float *next_gate_weight;/* [n_embd] with out, or NULL */
+    float *next_gate;             /* [n_tok], with next_gate_weight; else NULL */
+    uint64_t y_stride, res_stride, res_out_stride, gate_stride, out_stride;
+    uint32_t y_dtype, res_dtype, gate_dtype, out_dtype;
+    uint32_t n_embd;              /* 1..65536 */
+    uint32_t flags;               /* GX_RES_* */
+    uint32_t gate_kind;           /* GX_GATE_* */
+    float eps, res_scale, block_scale;
+} gx_residual_desc;               /* 152 bytes */
+GX_API gx_result gx_norm_residual(gx_context *context, const gx_residual_desc *desc, uint32_t n_tok,
+                                  uint64_t *out_ticket);
+
+/* Log probabilities of rows of logits, in one pass over them: z = scale * logits[r],
+ *   logprob[r] = log softmax(z)[tokens[r]],  rank[r] = 1 + the number of logits above the given token's,
+ *   entropy[r] = -sum p ln p,  and the n_top likeliest tokens with their log probabilities, by falling
+ * logit, equal ones by rising id (the selection rule of the router, src/engine.zig:671-686; -0 and 0
+ * are equal). A logit of -Inf is a masked token of probability 0; a row with every token masked counts
+ * as a row of equal logits (entropy ln n_vocab, log probability -ln n_vocab for every token). A row
+ * with a NaN or +Inf has NaN in its log probabilities and entropy; NaN orders below -Inf for the rank
+ * and the top ids.
+ * A tokens entry of GX_NO_TOKEN gives logprob 0 and rank 0 (padded rows); another id past n_vocab
+ * gives NaN and rank 0, and gx_wait returns GX_E_KERNEL. */
+#define GX_NO_TOKEN 0xffffffffu
+#define GX_MAX_TOP 32u
+typedef struct gx_logprobs_desc {
+    const void *logits;           /* [n_rows][n_vocab] */
+    const uint32_t *tokens;       /* [n_rows] given tokens, or NULL (then logprob and rank are NULL) */
+    float *logprob;               /* [n_rows] or NULL */
+    uint32_t *rank;               /* [n_rows] or NULL */
+    float *entropy;               /* [n_rows] or NULL */
+    uint32_t *top_ids;            /* [n_rows][n_top] or NULL */
+    float *top_logprobs;          /* [n_rows][n_top] or NULL */
+    uint64_t stride;              /* elements between rows of logits, >= n_vocab */
+    uint32_t dtype;               /* GX_F32 or GX_BF16 */
+    uint32_t n_vocab;             /* 1..524288 */
+    uint32_t n_top;               /* 0..GX_MAX_TOP, at most n_vocab */
+    float scale;                  /* > 0, finite: 1 / temperature */
+} gx_logprobs_desc;               /* 80 bytes */
+GX_API gx_result gx_logprobs(gx_context *context, const gx_logprobs_desc *desc, uint32_t n_rows,
+                             uint64_t *out_ticket);
+
+/* The norms, gate and residual scale of an uploaded layer used as the FFN block of a plain residual
+ * stream (desc NULL removes them; gx_upload_layer of the same index does too). Blocking. */
+typedef struct gx_norms_desc {
+    const float *pre;             /* [n_embd] weights of the norm before the layer, host memory, NULL for 1 */
+    const float *post;            /* [n_embd] weights of the norm after it, with post_norm (NULL for 1) */
+    const float *gate;            /* [n_embd] gate weights: sigmoid(gate . h) scales the layer's output; NULL: no gate */
+    uint32_t post_norm;           /* 1: normalise the layer's output, 0: add it as it is */
+    float eps, res_scale, block_scale;
+} gx_norms_desc;                  /* 40 bytes */
+GX_API gx_result gx_upload_norms(gx_context *context, uint32_t layer, const gx_norms_desc *desc, uint32_t timeout_ms);
+
+/* n_layers consecutive layers as FFN blocks of one residual stream, each with its gx_upload_norms:
+ *   h = norm(res; pre),  y = the layer on h (as gx_moe_forward),
+ *   res = res_scale * res + block_scale * sigmoid(gate . h) * norm(y; post)
+ * gx_norm before the first layer, then after each layer one gx_norm_residual that also makes the next
+ * layer's input. res: [n_tok][n_embd] f32 device, 16-byte aligned, updated in place. With world > 1
+ * it is a collective like gx_moe_forward. */
+GX_API gx_result gx_norm_block(gx_context *context, uint32_t first_layer, uint32_t n_layers, float *res, uint32_t n_tok,
+                               uint64_t *out_ticket);
 
 GX_API gx_result gx_read_timings(gx_context *context, gx_timings *out_timings);
 
