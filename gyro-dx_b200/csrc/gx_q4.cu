@@ -1,9 +1,20 @@
 // gx_q4.cu — matrix-vector products with 4-bit weights and group scales (GGUF Q4_0 and Q4_1):
 //
-//   y[t][r] = sum over groups of 32 columns of  d * sum_c (q - 8) x[t][c]        (Q4_0)
-//                                               d * sum_c q x[t][c] + m * sum_c x[t][c]   (Q4_1)
+//   y[t][r] = sum over groups of 32 columns of  d * (sum_c q x[t][c] - 8 sum_c x[t][c])       (Q4_0)
+//                                               d *  sum_c q x[t][c] + m sum_c x[t][c]        (Q4_1)
 //
 // with fp16 d and m per group and 4-bit q.
+//
+// The sums over a group run on the tensor cores (mma.sync m16n8k16, f32 accumulation) with the codes
+// as they are stored: a 4-bit code in the low bits of an f16 is the subnormal q 2^-24, in the next
+// four bits q 2^-20, both exact, so two ands and one shift turn a word of 8 codes into its four
+// A registers, and no weight is ever rounded. The activations of the codes that land at 2^-20 carry a
+// factor 1/16. The scale d meets the group's sum in f32, where the offset -8 sum x already waits as
+// the product's initial accumulator (Q4_1: m sum x is added beside it).
+//
+// Activations become f16 fragments in shared memory once per CTA: each unit of 128 columns of a token
+// is scaled by a power of two that brings its largest value to 2^14..2^15; an f32 value is split into
+// two f16 (22 bits, two columns of the product), a bf16 value fits one.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -19,50 +30,444 @@ using namespace dense;
 
 namespace {
 
-constexpr int kQ4Warps = 4;
-constexpr int kQ4Tok = 8;
+// ---- device layout ---------------------------------------------------------------------------
+// Units of 16 rows x 128 columns (4 groups), ordered [row tile][unit]; rows and columns past the
+// matrix have zero scales. Lane l = 4 g + q of a warp owns rows g and g + 8 and, in each group, the
+// columns 8 q .. 8 q + 7, the k-slices its A registers hold:
+//   [32 lanes][4 groups] words of row g     code of column 8 q + i in bits 4 i .. 4 i + 3
+//   [32 lanes][4 groups] words of row g + 8
+//   [8 g][row g: 4 groups, row g + 8: 4 groups] fp16 d
+//   [8 g][the same] fp16 m                  (Q4_1)
+constexpr int kUnitCols = 128, kTileRows = 16;
+__host__ __device__ constexpr int unit_bytes(uint32_t type) { return type == GX_Q4_0 ? 1152 : 1280; }
 
 __device__ __forceinline__ void store_act(void *p, int bf16, size_t i, float v) {
     if (bf16) reinterpret_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
     else reinterpret_cast<float *>(p)[i] = v;
 }
 
-// One warp per row, a lane per group of 32 columns, up to 8 tokens at a time, f32 sums.
-__global__ void __launch_bounds__(kQ4Warps * 32) q4_rows_kernel(Q4Args a) {
-    const int r = blockIdx.x * kQ4Warps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (r >= a.rows) return;
-    const int NG = a.cols / 32, gb = a.type == GX_Q4_0 ? 18 : 20;
-    const uint8_t *row = a.w + (size_t)r * NG * gb;
-    for (int t0 = 0; t0 < a.n_tok; t0 += kQ4Tok) {
-        const int nt = min(kQ4Tok, a.n_tok - t0);
-        float acc[kQ4Tok];
-#pragma unroll
-        for (int t = 0; t < kQ4Tok; ++t) acc[t] = 0.f;
-        for (int g = lane; g < NG; g += 32) {
-            const uint8_t *b = row + (size_t)g * gb;
-            const float d = __half2float(*reinterpret_cast<const __half *>(b));
-            const float m = a.type == GX_Q4_0 ? -8.f * d : __half2float(*reinterpret_cast<const __half *>(b + 2));
-            const uint8_t *q = b + gb - 16;
-#pragma unroll
-            for (int t = 0; t < kQ4Tok; ++t) {
-                if (t >= nt) break;
-                const size_t base = (size_t)(t0 + t) * a.ldx + (size_t)g * 32;
-                float qx = 0.f, sx = 0.f;
-                for (int j = 0; j < 16; ++j) {
-                    const float x0 = load_act(a.x, a.x_bf16, base + j), x1 = load_act(a.x, a.x_bf16, base + j + 16);
-                    qx = fmaf((float)(q[j] & 15), x0, fmaf((float)(q[j] >> 4), x1, qx));
-                    sx += x0 + x1;
-                }
-                acc[t] = fmaf(d, qx, fmaf(m, sx, acc[t])) + (sx - sx);  // Inf and NaN activations: NaN
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < kQ4Tok; ++t) {
-            if (t >= nt) break;
-            const float s = warp_sum(acc[t]);
-            if (lane == 0) store_act(a.y, a.y_bf16, (size_t)(t0 + t) * a.ldy + r, s);
+// One thread per (row of the padded matrix, group): 4 words and the scales of a group.
+__global__ void __launch_bounds__(256) q4_repack_kernel(uint32_t type, const uint8_t *raw, int rows, int cols,
+                                                        uint8_t *w, long long n) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int NG = (cols + kUnitCols - 1) / kUnitCols * 4;
+    const long long row = i / NG;
+    const int grp = (int)(i % NG), g = (int)(row & 7), hi = (int)(row >> 3) & 1, j = grp & 3;
+    uint8_t *u = w + ((row / kTileRows) * (NG / 4) + grp / 4) * unit_bytes(type);
+    uint32_t words[4] = {0u, 0u, 0u, 0u};
+    uint16_t d = 0, m = 0;
+    if (row < rows && grp < cols / 32) {
+        const int gb = type == GX_Q4_0 ? 18 : 20;
+        const uint16_t *b = reinterpret_cast<const uint16_t *>(raw + (row * (cols / 32) + grp) * gb);
+        d = b[0];
+        if (type == GX_Q4_1) m = b[1];
+        b += gb / 2 - 8;
+        for (int k = 0; k < 8; ++k) {  // bytes 2k, 2k+1: columns 2k, 2k+1 (low halves) and 2k+16, 2k+17
+            const uint32_t v = b[k];
+            const int q = k >> 2, s = 8 * (k & 3);
+            words[q] |= ((v & 15u) | ((v >> 4) & 0xf0u)) << s;
+            words[q + 2] |= (((v >> 4) & 15u) | ((v >> 8) & 0xf0u)) << s;
         }
     }
+    uint32_t *codes = reinterpret_cast<uint32_t *>(u + 512 * hi);
+    for (int q = 0; q < 4; ++q) codes[(4 * g + q) * 4 + j] = words[q];
+    reinterpret_cast<uint16_t *>(u + 1024)[g * 8 + hi * 4 + j] = d;
+    if (type == GX_Q4_1) reinterpret_cast<uint16_t *>(u + 1152)[g * 8 + hi * 4 + j] = m;
+}
+
+// ---- few tokens: a GEMV on mma.sync ------------------------------------------------------------
+struct Unit {
+    uint4 c0, c1, d, m;
+};
+template <uint32_t TYPE>
+__device__ __forceinline__ void load_unit(Unit &u, const uint8_t *p, int lane) {
+    u.c0 = __ldcs(reinterpret_cast<const uint4 *>(p) + lane);
+    u.c1 = __ldcs(reinterpret_cast<const uint4 *>(p + 512) + lane);
+    u.d = __ldcs(reinterpret_cast<const uint4 *>(p + 1024) + (lane >> 2));
+    if constexpr (TYPE == GX_Q4_1) u.m = __ldcs(reinterpret_cast<const uint4 *>(p + 1152) + (lane >> 2));
+}
+
+// Activations of one CTA's units in shared memory, for NT tiles of 8 product columns: a column is a
+// token in bf16, or the upper or lower part of a token in f32.
+//   frag [group][8 NT columns][4 q] 16 B    x of columns (0,4) (2,6) (1,5)/16 (3,7)/16 of 8 q ..
+//   sum  [group][8 NT columns / parts]      Q4_0: -8 2^-24 sum x, Q4_1: 2^-24 sum x (scaled x)
+//   inv  [unit][tokens]                     1 / scale
+template <bool XB, int NT>
+struct XLayout {
+    static constexpr int COLS = 8 * NT, TOK = XB ? 8 * NT : 4 * NT;
+    static constexpr int GROUP_BYTES = COLS * 64, UNIT_BYTES = 4 * GROUP_BYTES + 4 * TOK * 4 + TOK * 4;
+};
+
+template <uint32_t TYPE, bool XB, int NT>
+__device__ __forceinline__ void stage_x(const Q4Args &a, int t0, int nt, int u0, int nu, uint8_t *frag, float *sum,
+                                        float *inv, bool vec, int tid, int nthreads) {
+    using L = XLayout<XB, NT>;
+    const int cells = nu * 16, total = nt * cells;
+    for (int base = 0; base < total; base += nthreads) {
+        const int i = base + tid;
+        const bool on = i < total;
+        const int t = on ? i / cells : 0, cell = on ? i % cells : 0, col = u0 * kUnitCols + cell * 8;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = 0.f;
+        if (on && col < a.cols) {  // cols is a multiple of 32: a cell is inside or outside
+            const size_t at = (size_t)(t0 + t) * a.ldx + col;
+            if (vec) load_x8(a.x, XB, at, v);
+            else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = load_act(a.x, XB, at + k);
+            }
+        }
+        // the unit's largest magnitude, by its bits (an Inf or NaN has the largest exponent)
+        uint32_t big = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) big = max(big, __float_as_uint(v[k]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+        const uint32_t e = big >> 23, se = min(268u - e, 247u);
+        const float s = __uint_as_float(se << 23);
+        float ss = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            v[k] = e == 255u ? __uint_as_float(0x7fffffffu) : v[k] * s;
+            ss += v[k];
+        }
+        ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+        ss += __shfl_xor_sync(0xffffffffu, ss, 2);
+        if (!on) continue;
+        const int grp = cell >> 2, q = cell & 3;
+        auto put = [&](int c, const float (&x)[8]) {
+            uint4 f;
+            f.x = pack_half2(x[0], x[4]);
+            f.y = pack_half2(x[2], x[6]);
+            f.z = pack_half2(x[1] * 0.0625f, x[5] * 0.0625f);
+            f.w = pack_half2(x[3] * 0.0625f, x[7] * 0.0625f);
+            *reinterpret_cast<uint4 *>(frag + ((size_t)(grp * L::COLS + c) * 4 + q) * 16) = f;
+        };
+        if constexpr (XB) {
+            put(t, v);
+        } else {
+            // the lower part of the values that carry 1/16 is what the rounded upper part leaves there
+            float lo[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float f = (k & 1) ? 0.0625f : 1.f;
+                lo[k] = v[k] - __half2float(__float2half_rn(v[k] * f)) * (1.f / f);
+            }
+            put(2 * t, v);
+            put(2 * t + 1, lo);
+        }
+        if (q == 0) sum[grp * L::TOK + t] = ss * (TYPE == GX_Q4_0 ? -8.f * 0x1p-24f : 0x1p-24f);
+        if ((cell & 15) == 0) inv[(cell >> 4) * L::TOK + t] = __uint_as_float((254u - se) << 23);
+    }
+}
+
+// acc += the unit's products. acc[nt]: XB: (row g, token 2q), (g, 2q + 1), (g + 8, 2q), (g + 8, 2q + 1);
+// f32: (row g, token q), (row g + 8, token q).
+template <uint32_t TYPE, bool XB, int NT>
+__device__ __forceinline__ void unit_product(const Unit &u, int ul, const uint8_t *frag, const float *sum,
+                                             const float *inv, int lane, bool (&live)[NT], float (&acc)[NT][XB ? 4 : 2]) {
+    using L = XLayout<XB, NT>;
+    const int q = lane & 3;
+    const uint32_t c0[4] = {u.c0.x, u.c0.y, u.c0.z, u.c0.w}, c1[4] = {u.c1.x, u.c1.y, u.c1.z, u.c1.w};
+    const uint32_t dw[4] = {u.d.x, u.d.y, u.d.z, u.d.w}, mw[4] = {u.m.x, u.m.y, u.m.z, u.m.w};
+    float part[NT][XB ? 4 : 2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < (XB ? 4 : 2); ++k) part[n][k] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t s0 = c0[j] >> 8, s1 = c1[j] >> 8;
+        const uint32_t a0[4] = {c0[j] & 0x000f000fu, c1[j] & 0x000f000fu, s0 & 0x000f000fu, s1 & 0x000f000fu};
+        const uint32_t a1[4] = {c0[j] & 0x00f000f0u, c1[j] & 0x00f000f0u, s0 & 0x00f000f0u, s1 & 0x00f000f0u};
+        auto half_of = [&](const uint32_t (&w)[4], int hi) {
+            const __half2 h = *reinterpret_cast<const __half2 *>(&w[2 * hi + (j >> 1)]);
+            return (j & 1) ? __high2float(h) : __low2float(h);
+        };
+        const float d0 = half_of(dw, 0), d1 = half_of(dw, 1);
+        const int grp = 4 * ul + j;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            uint4 b = make_uint4(0u, 0u, 0u, 0u);
+            if (live[n]) b = *reinterpret_cast<const uint4 *>(frag + ((size_t)(grp * L::COLS + 8 * n) * 4 + lane) * 16);
+            if constexpr (XB) {
+                const float2 sx = *reinterpret_cast<const float2 *>(sum + grp * L::TOK + 8 * n + 2 * q);
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (TYPE == GX_Q4_0) {
+                    c[0] = c[2] = sx.x;
+                    c[1] = c[3] = sx.y;
+                }
+                mma16816(c, a0, b.x, b.y);
+                mma16816(c, a1, b.z, b.w);
+                part[n][0] = fmaf(d0, c[0], part[n][0]);
+                part[n][1] = fmaf(d0, c[1], part[n][1]);
+                part[n][2] = fmaf(d1, c[2], part[n][2]);
+                part[n][3] = fmaf(d1, c[3], part[n][3]);
+                if constexpr (TYPE == GX_Q4_1) {
+                    const float m0 = half_of(mw, 0), m1 = half_of(mw, 1);
+                    part[n][0] = fmaf(m0, sx.x, part[n][0]);
+                    part[n][1] = fmaf(m0, sx.y, part[n][1]);
+                    part[n][2] = fmaf(m1, sx.x, part[n][2]);
+                    part[n][3] = fmaf(m1, sx.y, part[n][3]);
+                }
+            } else {
+                const float sx = sum[grp * L::TOK + 4 * n + q];
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (TYPE == GX_Q4_0) c[0] = c[2] = sx;
+                mma16816(c, a0, b.x, b.y);
+                mma16816(c, a1, b.z, b.w);
+                part[n][0] = fmaf(d0, c[0] + c[1], part[n][0]);
+                part[n][1] = fmaf(d1, c[2] + c[3], part[n][1]);
+                if constexpr (TYPE == GX_Q4_1) {
+                    part[n][0] = fmaf(half_of(mw, 0), sx, part[n][0]);
+                    part[n][1] = fmaf(half_of(mw, 1), sx, part[n][1]);
+                }
+            }
+        }
+    }
+    // 2^24 and the unit's scale apart: together they may pass f32 where the product does not
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        if constexpr (XB) {
+            const float2 iv = *reinterpret_cast<const float2 *>(inv + ul * L::TOK + 8 * n + 2 * q);
+            acc[n][0] = fmaf(part[n][0] * 0x1p24f, iv.x, acc[n][0]);
+            acc[n][1] = fmaf(part[n][1] * 0x1p24f, iv.y, acc[n][1]);
+            acc[n][2] = fmaf(part[n][2] * 0x1p24f, iv.x, acc[n][2]);
+            acc[n][3] = fmaf(part[n][3] * 0x1p24f, iv.y, acc[n][3]);
+        } else {
+            const float iv = inv[ul * L::TOK + 4 * n + q];
+            acc[n][0] = fmaf(part[n][0] * 0x1p24f, iv, acc[n][0]);
+            acc[n][1] = fmaf(part[n][1] * 0x1p24f, iv, acc[n][1]);
+        }
+    }
+}
+
+struct GemvPlan {
+    int RT, KT;      // row tiles, units in a row
+    int S;           // CTAs of a cluster that split the columns
+    int WK;          // warps of a CTA that split its columns; W / WK row tiles at a time
+    int t0, nt;      // tokens of this launch
+    int vec;         // activations can be read 16 bytes at a time
+    int sum_off, inv_off, red_off;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(const float *p, uint32_t rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
+// Row tiles go to groups of WK warps, in turn over the grid; the warps of a group take the units of
+// a row tile in turn, with kDepth units in flight in registers across row tiles, and add their parts
+// in shared memory. With S > 1 each cluster has one pass of row tiles, its CTAs take S ranges of the
+// units, and rank 0 adds their parts.
+constexpr int gemv_ctas(int NT, int W) { return W == 16 ? 1 : NT == 1 ? 3 : 2; }  // resident on an SM
+
+template <uint32_t TYPE, bool XB, int NT, int W>
+__global__ void __launch_bounds__(W * 32, gemv_ctas(NT, W)) q4_gemv_kernel(Q4Args a, GemvPlan p) {
+    using L = XLayout<XB, NT>;
+    constexpr int kDepth = TYPE == GX_Q4_0 ? 3 : 2;
+    constexpr int NA = XB ? 4 : 2, RED = kTileRows * L::TOK;
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint8_t *frag = smem;
+    float *sum = reinterpret_cast<float *>(smem + p.sum_off), *inv = reinterpret_cast<float *>(smem + p.inv_off);
+    float *red = reinterpret_cast<float *>(smem + p.red_off);  // [2][W][RED]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = p.S > 1 ? (int)cluster_rank() : 0;
+    const int u0 = (int)((long long)p.KT * rank / p.S), u1 = (int)((long long)p.KT * (rank + 1) / p.S), nu = u1 - u0;
+    const int groups = W / p.WK, wg = warp / p.WK, wk = warp % p.WK;
+    const int step = (int)(gridDim.x / p.S) * groups;
+    const int rt0 = (int)(blockIdx.x / p.S) * groups + wg;
+
+    // cursor of the loads: row tile and unit
+    int lrt = rt0, lu = wk;
+    const bool idle = wk >= nu;  // more warps than units: this one only takes part in the sums
+    Unit buf[kDepth];
+    auto fetch = [&](Unit &u) {
+        if (!idle && lrt < p.RT) {
+            load_unit<TYPE>(u, a.w + ((size_t)lrt * p.KT + u0 + lu) * unit_bytes(TYPE), lane);
+            lu += p.WK;
+            if (lu >= nu) {
+                lu = wk;
+                lrt += step;
+            }
+        }
+    };
+#pragma unroll
+    for (int k = 0; k < kDepth; ++k) fetch(buf[k]);
+    pdl_launch_dependents();
+    pdl_wait();  // the weights never change; the activations may come from the kernel before
+    stage_x<TYPE, XB, NT>(a, p.t0, p.nt, u0, nu, frag, sum, inv, p.vec != 0, tid, W * 32);
+    __syncthreads();
+
+    bool live[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) live[n] = 8 * n + (lane >> 2) < (XB ? p.nt : 2 * p.nt);
+    float acc[NT][NA];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < NA; ++k) acc[n][k] = 0.f;
+    int rt = rt0, ul = wk, parity = 0;
+    auto put = [&](float *dst) {  // the warp's part as [token][16 rows]
+        const int g = lane >> 2, q = lane & 3;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            if constexpr (XB) {
+                dst[(8 * n + 2 * q) * 16 + g] = acc[n][0];
+                dst[(8 * n + 2 * q + 1) * 16 + g] = acc[n][1];
+                dst[(8 * n + 2 * q) * 16 + g + 8] = acc[n][2];
+                dst[(8 * n + 2 * q + 1) * 16 + g + 8] = acc[n][3];
+            } else {
+                dst[(4 * n + q) * 16 + g] = acc[n][0];
+                dst[(4 * n + q) * 16 + g + 8] = acc[n][1];
+            }
+        }
+    };
+    auto finish = [&]() {  // the row tile rt is complete in this warp
+        float *mine = red + (size_t)(parity * W + warp) * RED;
+        put(mine);
+        if (p.WK > 1) {
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + wg), "r"(32 * p.WK) : "memory");
+        } else {
+            __syncwarp();
+        }
+        const float *all = red + (size_t)(parity * W + wg * p.WK) * RED;
+        float *keep = red + (size_t)(parity * W + wg * p.WK) * RED;
+        for (int i = wk * 32 + lane; i < 16 * p.nt; i += 32 * p.WK) {
+            float s = all[i];
+            for (int k = 1; k < p.WK; ++k) s += all[(size_t)k * RED + i];
+            if (p.S > 1) keep[i] = s;
+            else if (rt * 16 + (i & 15) < a.rows)
+                store_act(a.y, a.y_bf16, (size_t)(p.t0 + (i >> 4)) * a.ldy + rt * 16 + (i & 15), s);
+        }
+        if (p.WK == 1) __syncwarp();
+        parity ^= 1;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < NA; ++k) acc[n][k] = 0.f;
+    };
+    while (rt < p.RT) {
+        if (idle) {
+            finish();
+            rt += step;
+            continue;
+        }
+#pragma unroll
+        for (int k = 0; k < kDepth; ++k) {
+            if (rt >= p.RT) break;
+            unit_product<TYPE, XB, NT>(buf[k], ul, frag, sum, inv, lane, live, acc);
+            fetch(buf[k]);
+            ul += p.WK;
+            if (ul >= nu) {
+                finish();
+                ul = wk;
+                rt += step;
+            }
+        }
+    }
+    if (p.S > 1) {  // one pass: the sums lie in parity 0
+        cluster_sync_all();
+        if (rank == 0 && rt0 < p.RT) {
+            const float *all = red + (size_t)(wg * p.WK) * RED;
+            for (int i = wk * 32 + lane; i < 16 * p.nt; i += 32 * p.WK) {
+                float s = all[i];
+                for (int r = 1; r < p.S; ++r) s += ld_cluster(all + i, (uint32_t)r);
+                if (rt0 * 16 + (i & 15) < a.rows)
+                    store_act(a.y, a.y_bf16, (size_t)(p.t0 + (i >> 4)) * a.ldy + rt0 * 16 + (i & 15), s);
+            }
+        }
+        cluster_sync_all();  // no CTA leaves while its part is read
+    }
+}
+
+template <uint32_t TYPE, bool XB, int NT, int W>
+cudaError_t launch_gemv_w(const Q4Args &a, GemvPlan p, int smem, int grid, cudaStream_t s) {
+    auto *k = q4_gemv_kernel<TYPE, XB, NT, W>;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(W * 32);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)p.S;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.S > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, k, a, p);
+}
+
+// Largest shared memory of a CTA.
+constexpr int kMaxSmem = 227 * 1024;
+
+template <uint32_t TYPE, bool XB, int NT>
+cudaError_t launch_gemv(const Q4Args &a, int t0, int nt, int sm_count, cudaStream_t s) {
+    using L = XLayout<XB, NT>;
+    GemvPlan p{};
+    p.RT = (a.rows + kTileRows - 1) / kTileRows;
+    p.KT = (a.cols + kUnitCols - 1) / kUnitCols;
+    p.t0 = t0;
+    p.nt = nt;
+    const size_t esz = XB ? 2 : 4;
+    p.vec = ((uintptr_t)a.x & 15) == 0 && (a.ldx * esz) % 16 == 0;
+    // Enough warps for 16 on every SM: first the warps of a CTA split a row's units (down to two
+    // units a warp), then the CTAs of a cluster do.
+    const long long want = 16ll * sm_count;
+    p.S = 1;
+    p.WK = 1;
+    while (p.WK < 8 && (long long)p.RT * p.WK < want && p.KT >= 4 * p.WK) p.WK *= 2;
+    while (p.S < 8 && (long long)p.RT * p.WK * p.S < want && p.KT >= 4 * p.WK * p.S) p.S *= 2;
+    // the activations of a CTA's units have to fit
+    while (p.S < 8 && (long long)((p.KT + p.S - 1) / p.S) * L::UNIT_BYTES > 100 * 1024) p.S *= 2;
+    const int nu = (p.KT + p.S - 1) / p.S;
+    const int xbytes = nu * L::UNIT_BYTES;
+    const bool wide = xbytes > 56 * 1024;  // few CTAs fit an SM: 16 warps each instead of 8
+    const int W = wide ? 16 : 8;
+    p.sum_off = nu * 4 * L::GROUP_BYTES;
+    p.inv_off = p.sum_off + nu * 4 * L::TOK * 4;
+    p.red_off = (p.inv_off + nu * L::TOK * 4 + 15) / 16 * 16;
+    const int smem = p.red_off + 2 * W * kTileRows * L::TOK * 4;
+    if (smem > kMaxSmem) return cudaErrorInvalidValue;
+    const int groups = W / p.WK, need = (p.RT + groups - 1) / groups;
+    const int resident = sm_count * gemv_ctas(NT, W);
+    const int grid = p.S > 1 ? need * p.S : need < resident ? need : resident;
+    return wide ? launch_gemv_w<TYPE, XB, NT, 16>(a, p, smem, grid, s) : launch_gemv_w<TYPE, XB, NT, 8>(a, p, smem, grid, s);
+}
+
+template <uint32_t TYPE, bool XB>
+cudaError_t launch_tokens(const Q4Args &a, int sm_count, cudaStream_t s) {
+    constexpr int T1 = XB ? 8 : 4;
+    const int KT = (a.cols + kUnitCols - 1) / kUnitCols;
+    const int most = ((KT + 7) / 8) * XLayout<XB, 2>::UNIT_BYTES <= 160 * 1024 ? 2 * T1 : T1;
+    for (int t0 = 0; t0 < a.n_tok; t0 += most) {
+        const int nt = a.n_tok - t0 < most ? a.n_tok - t0 : most;
+        const cudaError_t e = nt <= T1 ? launch_gemv<TYPE, XB, 1>(a, t0, nt, sm_count, s)
+                                       : launch_gemv<TYPE, XB, 2>(a, t0, nt, sm_count, s);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+uint64_t padded_units(uint64_t rows, uint64_t cols) {
+    return (rows + kTileRows - 1) / kTileRows * ((cols + kUnitCols - 1) / kUnitCols);
 }
 
 }  // namespace
@@ -72,17 +477,22 @@ uint64_t q4_row_bytes(uint32_t type, uint64_t cols) {
     return cols / 32 * (type == GX_Q4_0 ? 18 : 20);
 }
 
-uint64_t q4_bytes(uint32_t type, uint64_t rows, uint64_t cols) { return rows * q4_row_bytes(type, cols); }
+uint64_t q4_bytes(uint32_t type, uint64_t rows, uint64_t cols) { return padded_units(rows, cols) * unit_bytes(type); }
 
 cudaError_t launch_q4_repack(uint32_t type, const uint8_t *raw, uint32_t rows, uint32_t cols, uint8_t *w,
                              cudaStream_t s) {
-    return cudaMemcpyAsync(w, raw, q4_bytes(type, rows, cols), cudaMemcpyDeviceToDevice, s);
+    const long long n = (long long)padded_units(rows, cols) * kTileRows * 4;
+    const long long blocks = (n + 255) / 256;
+    if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+    q4_repack_kernel<<<(unsigned)blocks, 256, 0, s>>>(type, raw, (int)rows, (int)cols, w, n);
+    return cudaGetLastError();
 }
 
 cudaError_t launch_q4_linear(const Q4Args &a, int sm_count, cudaStream_t s) {
     if (a.n_tok <= 0 || a.rows <= 0) return cudaSuccess;
-    q4_rows_kernel<<<(a.rows + kQ4Warps - 1) / kQ4Warps, kQ4Warps * 32, 0, s>>>(a);
-    return cudaGetLastError();
+    if (a.type == GX_Q4_0)
+        return a.x_bf16 ? launch_tokens<GX_Q4_0, true>(a, sm_count, s) : launch_tokens<GX_Q4_0, false>(a, sm_count, s);
+    return a.x_bf16 ? launch_tokens<GX_Q4_1, true>(a, sm_count, s) : launch_tokens<GX_Q4_1, false>(a, sm_count, s);
 }
 
 }  // namespace gx
