@@ -128,6 +128,10 @@ struct gx_context {
         __half *Ylo = nullptr, *gate = nullptr;
         int *ints = nullptr;  // tile_expert | tile_rows | n_mtiles
     } hc;
+    // packed activations of gx_linear for the widest 4-bit matrix uploaded. A wider matrix gets a new
+    // workspace; the ones before stay until the context goes, since captured graphs may hold them.
+    std::vector<uint8_t *> q4_ws;
+    uint32_t q4_ws_cols = 0;
     float *norm_gate = nullptr;      // [max_tokens] gate logits of gx_norm_block (first gx_upload_norms)
     uint32_t *ids = nullptr;
     int *err = nullptr;
@@ -336,6 +340,7 @@ void release_all(gx_context *c) {
     void *pf[] = {c->pf.A, c->pf.A2, c->pf.act, c->pf.Y, c->pf.ints};
     for (void *p : pf) if (p) cudaFree(p);
     for (auto &m : c->mats) if (m.tiles) cudaFree(m.tiles);
+    for (uint8_t *p : c->q4_ws) cudaFree(p);
     void *dev[] = {c->codebook, c->codebook_image, c->router_done, c->logits, c->weights, c->xscale, c->ss, c->ids,
                    c->act, c->xbuf[0], c->xbuf[1], c->x_stage, c->y_stage, c->err, c->stack_table, c->stack_sync,
                    c->norm_gate};
@@ -2360,6 +2365,12 @@ GX_API gx_result gx_upload_matrix(gx_context *c, uint32_t type_id, uint32_t rows
     // the GEMV takes rows 16 at a time: an odd count of 8-row groups gets a zero group after it
     const uint64_t pad = !q4 && rows % 16 ? (uint64_t)gx::tile_bytes(type_id) * (cols / 128) : 0;
     const uint64_t bytes = q4 ? gx::q4_bytes(type_id, rows, cols) : packed_bytes + pad;
+    if (q4 && cols > c->q4_ws_cols) {
+        uint8_t *ws = nullptr;
+        GX_CUDA(cudaMalloc(&ws, gx::q4_workspace_bytes(cols)));
+        c->q4_ws.push_back(ws);
+        c->q4_ws_cols = cols;
+    }
     uint8_t *raw = nullptr, *tiles = nullptr;
     GX_CUDA(cudaMalloc(&tiles, bytes));
     cudaError_t e = cudaMalloc(&raw, packed_bytes);
@@ -2402,7 +2413,7 @@ gx_result enqueue_q4(gx_context *c, const Matrix &m, const void *x, uint32_t x_d
     a.rows = (int)m.rows;
     a.cols = (int)m.cols;
     a.n_tok = (int)n_tok;
-    GX_CUDA(gx::launch_q4_linear(a, c->sm_count, c->stream));
+    GX_CUDA(gx::launch_q4_linear(a, c->q4_ws.back(), c->sm_count, c->stream));
     return GX_OK;
 }
 

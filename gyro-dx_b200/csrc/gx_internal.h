@@ -413,7 +413,9 @@ uint64_t q4_row_bytes(uint32_t type, uint64_t cols);               // of the mod
 uint64_t q4_bytes(uint32_t type, uint64_t rows, uint64_t cols);    // of the device layout
 cudaError_t launch_q4_repack(uint32_t type, const uint8_t *raw, uint32_t rows, uint32_t cols, uint8_t *w,
                              cudaStream_t s);
-cudaError_t launch_q4_linear(const Q4Args &a, int sm_count, cudaStream_t s);
+// Bytes of the workspace that launch_q4_linear packs the activations of more than a few tokens into.
+uint64_t q4_workspace_bytes(uint64_t cols);
+cudaError_t launch_q4_linear(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s);
 
 struct NormArgs {
     const void *x;

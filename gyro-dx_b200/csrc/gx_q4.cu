@@ -5,12 +5,13 @@
 //
 // with fp16 d and m per group and 4-bit q.
 //
-// The sums over a group run on the tensor cores (mma.sync m16n8k16, f32 accumulation) with the codes
-// as they are stored: a 4-bit code in the low bits of an f16 is the subnormal q 2^-24, in the next
-// four bits q 2^-20, both exact, so two ands and one shift turn a word of 8 codes into its four
-// A registers, and no weight is ever rounded. The activations of the codes that land at 2^-20 carry a
-// factor 1/16. The scale d meets the group's sum in f32, where the offset -8 sum x already waits as
-// the product's initial accumulator (Q4_1: m sum x is added beside it).
+// The sums over a group run on the tensor cores (mma.sync m16n8k16, f32 accumulation) on the integers
+// q - 8 (Q4_1: q), which f16 holds exactly, and d meets the group's sum in f32, so no weight is ever
+// rounded. A code in the low bits of an f16 under the exponent of 1024 is 1024 + q, four bits higher
+// 1024 + 16 q: one shift, four and-ors and four half2 operations turn a word of 8 codes into its four
+// A registers. (Codes as f16 subnormals need no arithmetic at all, but the product then aligns its
+// terms by the subnormals' exponent and loses their leading zeros: 2e-6 to 4e-6 relative error
+// measured, against 1e-7.)
 //
 // Activations become f16 fragments in shared memory once per CTA: each unit of 128 columns of a token
 // is scaled by a power of two that brings its largest value to 2^14..2^15; an f32 value is split into
@@ -90,14 +91,59 @@ __device__ __forceinline__ void load_unit(Unit &u, const uint8_t *p, int lane) {
 
 // Activations of one CTA's units in shared memory, for NT tiles of 8 product columns: a column is a
 // token in bf16, or the upper or lower part of a token in f32.
-//   frag [group][8 NT columns][4 q] 16 B    x of columns (0,4) (2,6) (1,5)/16 (3,7)/16 of 8 q ..
-//   sum  [group][8 NT columns / parts]      Q4_0: -8 2^-24 sum x, Q4_1: 2^-24 sum x (scaled x)
+//   frag [group][8 NT columns][4 q] 16 B    x of columns (0,4) (2,6) (1,5) (3,7) of 8 q ..
+//   sum  [group][tokens]                    sum x (Q4_1 only)
 //   inv  [unit][tokens]                     1 / scale
 template <bool XB, int NT>
 struct XLayout {
     static constexpr int COLS = 8 * NT, TOK = XB ? 8 * NT : 4 * NT;
     static constexpr int GROUP_BYTES = COLS * 64, UNIT_BYTES = 4 * GROUP_BYTES + 4 * TOK * 4 + TOK * 4;
 };
+
+// The 8 scaled values of columns 8 q .. of a group as the fragment of token t (column t in bf16; 2 t
+// and 2 t + 1, the upper and lower part, in f32).
+template <bool XB>
+__device__ __forceinline__ void put_fragment(uint8_t *group, int t, int q, const float (&v)[8]) {
+    auto put = [&](int c, const float (&x)[8]) {
+        *reinterpret_cast<uint4 *>(group + ((size_t)c * 4 + q) * 16) =
+            make_uint4(pack_half2(x[0], x[4]), pack_half2(x[2], x[6]), pack_half2(x[1], x[5]), pack_half2(x[3], x[7]));
+    };
+    if constexpr (XB) {
+        put(t, v);
+    } else {
+        float hi[8], lo[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) split_hilo(v[k], hi[k], lo[k]);
+        put(2 * t, hi);
+        put(2 * t + 1, lo);
+    }
+}
+
+// The A registers of 8 codes of row g (r0) and of row g + 8 (r1): columns (0,4) (2,6) of each in a0,
+// (1,5) (3,7) in a1.
+template <uint32_t TYPE>
+__device__ __forceinline__ void code_fragments(uint32_t r0, uint32_t r1, uint32_t (&a0)[4], uint32_t (&a1)[4]) {
+    constexpr float off = TYPE == GX_Q4_0 ? 8.f : 0.f;
+    const __half2 sub = __float2half2_rn(-1024.f - off), mul = __float2half2_rn(0.0625f), sub16 = __float2half2_rn(-64.f - off);
+    auto low = [&](uint32_t v) {
+        const uint32_t h = (v & 0x000f000fu) | 0x64006400u;
+        const __half2 r = __hadd2(*reinterpret_cast<const __half2 *>(&h), sub);
+        return *reinterpret_cast<const uint32_t *>(&r);
+    };
+    auto high = [&](uint32_t v) {
+        const uint32_t h = (v & 0x00f000f0u) | 0x64006400u;
+        const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&h), mul, sub16);
+        return *reinterpret_cast<const uint32_t *>(&r);
+    };
+    a0[0] = low(r0);
+    a0[1] = low(r1);
+    a0[2] = low(r0 >> 8);
+    a0[3] = low(r1 >> 8);
+    a1[0] = high(r0);
+    a1[1] = high(r1);
+    a1[2] = high(r0 >> 8);
+    a1[3] = high(r1 >> 8);
+}
 
 template <uint32_t TYPE, bool XB, int NT>
 __device__ __forceinline__ void stage_x(const Q4Args &a, int t0, int nt, int u0, int nu, uint8_t *frag, float *sum,
@@ -137,28 +183,8 @@ __device__ __forceinline__ void stage_x(const Q4Args &a, int t0, int nt, int u0,
         ss += __shfl_xor_sync(0xffffffffu, ss, 2);
         if (!on) continue;
         const int grp = cell >> 2, q = cell & 3;
-        auto put = [&](int c, const float (&x)[8]) {
-            uint4 f;
-            f.x = pack_half2(x[0], x[4]);
-            f.y = pack_half2(x[2], x[6]);
-            f.z = pack_half2(x[1] * 0.0625f, x[5] * 0.0625f);
-            f.w = pack_half2(x[3] * 0.0625f, x[7] * 0.0625f);
-            *reinterpret_cast<uint4 *>(frag + ((size_t)(grp * L::COLS + c) * 4 + q) * 16) = f;
-        };
-        if constexpr (XB) {
-            put(t, v);
-        } else {
-            // the lower part of the values that carry 1/16 is what the rounded upper part leaves there
-            float lo[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float f = (k & 1) ? 0.0625f : 1.f;
-                lo[k] = v[k] - __half2float(__float2half_rn(v[k] * f)) * (1.f / f);
-            }
-            put(2 * t, v);
-            put(2 * t + 1, lo);
-        }
-        if (q == 0) sum[grp * L::TOK + t] = ss * (TYPE == GX_Q4_0 ? -8.f * 0x1p-24f : 0x1p-24f);
+        put_fragment<XB>(frag + (size_t)grp * L::COLS * 64, t, q, v);
+        if (TYPE == GX_Q4_1 && q == 0) sum[grp * L::TOK + t] = ss;
         if ((cell & 15) == 0) inv[(cell >> 4) * L::TOK + t] = __uint_as_float((254u - se) << 23);
     }
 }
@@ -179,9 +205,8 @@ __device__ __forceinline__ void unit_product(const Unit &u, int ul, const uint8_
         for (int k = 0; k < (XB ? 4 : 2); ++k) part[n][k] = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const uint32_t s0 = c0[j] >> 8, s1 = c1[j] >> 8;
-        const uint32_t a0[4] = {c0[j] & 0x000f000fu, c1[j] & 0x000f000fu, s0 & 0x000f000fu, s1 & 0x000f000fu};
-        const uint32_t a1[4] = {c0[j] & 0x00f000f0u, c1[j] & 0x00f000f0u, s0 & 0x00f000f0u, s1 & 0x00f000f0u};
+        uint32_t a0[4], a1[4];
+        code_fragments<TYPE>(c0[j], c1[j], a0, a1);
         auto half_of = [&](const uint32_t (&w)[4], int hi) {
             const __half2 h = *reinterpret_cast<const __half2 *>(&w[2 * hi + (j >> 1)]);
             return (j & 1) ? __high2float(h) : __low2float(h);
@@ -193,12 +218,7 @@ __device__ __forceinline__ void unit_product(const Unit &u, int ul, const uint8_
             uint4 b = make_uint4(0u, 0u, 0u, 0u);
             if (live[n]) b = *reinterpret_cast<const uint4 *>(frag + ((size_t)(grp * L::COLS + 8 * n) * 4 + lane) * 16);
             if constexpr (XB) {
-                const float2 sx = *reinterpret_cast<const float2 *>(sum + grp * L::TOK + 8 * n + 2 * q);
                 float c[4] = {0.f, 0.f, 0.f, 0.f};
-                if constexpr (TYPE == GX_Q4_0) {
-                    c[0] = c[2] = sx.x;
-                    c[1] = c[3] = sx.y;
-                }
                 mma16816(c, a0, b.x, b.y);
                 mma16816(c, a1, b.z, b.w);
                 part[n][0] = fmaf(d0, c[0], part[n][0]);
@@ -206,6 +226,7 @@ __device__ __forceinline__ void unit_product(const Unit &u, int ul, const uint8_
                 part[n][2] = fmaf(d1, c[2], part[n][2]);
                 part[n][3] = fmaf(d1, c[3], part[n][3]);
                 if constexpr (TYPE == GX_Q4_1) {
+                    const float2 sx = *reinterpret_cast<const float2 *>(sum + grp * L::TOK + 8 * n + 2 * q);
                     const float m0 = half_of(mw, 0), m1 = half_of(mw, 1);
                     part[n][0] = fmaf(m0, sx.x, part[n][0]);
                     part[n][1] = fmaf(m0, sx.y, part[n][1]);
@@ -213,36 +234,36 @@ __device__ __forceinline__ void unit_product(const Unit &u, int ul, const uint8_
                     part[n][3] = fmaf(m1, sx.y, part[n][3]);
                 }
             } else {
-                const float sx = sum[grp * L::TOK + 4 * n + q];
                 float c[4] = {0.f, 0.f, 0.f, 0.f};
-                if constexpr (TYPE == GX_Q4_0) c[0] = c[2] = sx;
                 mma16816(c, a0, b.x, b.y);
                 mma16816(c, a1, b.z, b.w);
                 part[n][0] = fmaf(d0, c[0] + c[1], part[n][0]);
                 part[n][1] = fmaf(d1, c[2] + c[3], part[n][1]);
                 if constexpr (TYPE == GX_Q4_1) {
+                    const float sx = sum[grp * L::TOK + 4 * n + q];
                     part[n][0] = fmaf(half_of(mw, 0), sx, part[n][0]);
                     part[n][1] = fmaf(half_of(mw, 1), sx, part[n][1]);
                 }
             }
         }
     }
-    // 2^24 and the unit's scale apart: together they may pass f32 where the product does not
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         if constexpr (XB) {
             const float2 iv = *reinterpret_cast<const float2 *>(inv + ul * L::TOK + 8 * n + 2 * q);
-            acc[n][0] = fmaf(part[n][0] * 0x1p24f, iv.x, acc[n][0]);
-            acc[n][1] = fmaf(part[n][1] * 0x1p24f, iv.y, acc[n][1]);
-            acc[n][2] = fmaf(part[n][2] * 0x1p24f, iv.x, acc[n][2]);
-            acc[n][3] = fmaf(part[n][3] * 0x1p24f, iv.y, acc[n][3]);
+            acc[n][0] = fmaf(part[n][0], iv.x, acc[n][0]);
+            acc[n][1] = fmaf(part[n][1], iv.y, acc[n][1]);
+            acc[n][2] = fmaf(part[n][2], iv.x, acc[n][2]);
+            acc[n][3] = fmaf(part[n][3], iv.y, acc[n][3]);
         } else {
             const float iv = inv[ul * L::TOK + 4 * n + q];
-            acc[n][0] = fmaf(part[n][0] * 0x1p24f, iv, acc[n][0]);
-            acc[n][1] = fmaf(part[n][1] * 0x1p24f, iv, acc[n][1]);
+            acc[n][0] = fmaf(part[n][0], iv, acc[n][0]);
+            acc[n][1] = fmaf(part[n][1], iv, acc[n][1]);
         }
     }
 }
+
+constexpr int kMaxSmem = 227 * 1024;  // of a CTA
 
 struct GemvPlan {
     int RT, KT;      // row tiles, units in a row
@@ -415,9 +436,6 @@ cudaError_t launch_gemv_w(const Q4Args &a, GemvPlan p, int smem, int grid, cudaS
     return cudaLaunchKernelEx(&cfg, k, a, p);
 }
 
-// Largest shared memory of a CTA.
-constexpr int kMaxSmem = 227 * 1024;
-
 template <uint32_t TYPE, bool XB, int NT>
 cudaError_t launch_gemv(const Q4Args &a, int t0, int nt, int sm_count, cudaStream_t s) {
     using L = XLayout<XB, NT>;
@@ -452,9 +470,330 @@ cudaError_t launch_gemv(const Q4Args &a, int t0, int nt, int sm_count, cudaStrea
     return wide ? launch_gemv_w<TYPE, XB, NT, 16>(a, p, smem, grid, s) : launch_gemv_w<TYPE, XB, NT, 8>(a, p, smem, grid, s);
 }
 
+// ---- more tokens: a tiled product on mma.sync ---------------------------------------------------
+// The activations are packed once per call (q4_pack_kernel) into the same fragments, at one scale per
+// token, in a workspace of the context: [unit][4 groups][COLS columns][4 q] 16 B, then the group sums
+// [4 groups][TOK tokens] of the unit; the tokens' inverse scales stand before the first unit.
+constexpr int kQ4InvBytes = 256;
+
+struct GemmPlan {
+    int RT, KT;
+    int WM, WN, WK;  // warps: row pairs of tiles, column groups, splits of the units
+    int S;           // CTAs of a cluster that split the units
+    int vec;
+};
+
+constexpr int kPackThreads = 512;
+
 template <uint32_t TYPE, bool XB>
-cudaError_t launch_tokens(const Q4Args &a, int sm_count, cudaStream_t s) {
+__global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(Q4Args a, uint8_t *ws, int KT, int cols_padded, int vec) {
+    __shared__ uint32_t red[kPackThreads / 32];
+    const int t = blockIdx.x, tid = threadIdx.x;
+    const int tok_padded = XB ? cols_padded : cols_padded / 2;
+    const size_t unit = (size_t)cols_padded * 256 + (size_t)tok_padded * 16;
+    pdl_launch_dependents();
+    pdl_wait();
+    auto load = [&](int cell, float (&v)[8]) {
+        const int col = cell * 8;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = 0.f;
+        if (col < a.cols) {
+            const size_t at = (size_t)t * a.ldx + col;
+            if (vec) load_x8(a.x, XB, at, v);
+            else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = load_act(a.x, XB, at + k);
+            }
+        }
+    };
+    const int cells = KT * 16;
+    float first[8];
+    uint32_t big = 0;
+    for (int cell = tid; cell < cells; cell += kPackThreads) {
+        float v[8];
+        load(cell, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            big = max(big, __float_as_uint(v[k]) & 0x7fffffffu);
+            if (cell == tid) first[k] = v[k];
+        }
+    }
+    big = __reduce_max_sync(0xffffffffu, big);
+    if ((tid & 31) == 0) red[tid >> 5] = big;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kPackThreads / 32; ++w) big = max(big, red[w]);
+    const uint32_t e = big >> 23, se = min(268u - e, 247u);
+    const float s = __uint_as_float(se << 23);
+    if (tid == 0) reinterpret_cast<float *>(ws)[t] = __uint_as_float((254u - se) << 23);
+    uint8_t *units = ws + kQ4InvBytes;
+    for (int base = 0; base < cells; base += kPackThreads) {  // cells is a multiple of 16: quads stay together
+        const int cell = base + tid;
+        float v[8];
+        if (base == 0) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = cell < cells ? first[k] : 0.f;
+        } else if (cell < cells) {
+            load(cell, v);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = 0.f;
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            v[k] = e == 255u ? __uint_as_float(0x7fffffffu) : v[k] * s;
+            ss += v[k];
+        }
+        ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+        ss += __shfl_xor_sync(0xffffffffu, ss, 2);
+        if (cell >= cells) continue;
+        const int q = cell & 3, j = (cell >> 2) & 3;
+        uint8_t *u = units + (size_t)(cell >> 4) * unit;
+        put_fragment<XB>(u + (size_t)j * cols_padded * 64, t, q, v);
+        if (TYPE == GX_Q4_1 && q == 0) reinterpret_cast<float *>(u + (size_t)cols_padded * 256)[j * tok_padded + t] = ss;
+    }
+}
+
+__device__ __forceinline__ void cp_async16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+constexpr int kGemmStages = 3;
+
+// A CTA takes 2 WM row tiles by all tokens over its range of units: warp (wk, wm, wn) two row tiles by
+// NB product tiles of every WK-th unit. Codes and fragments come through a ring of shared-memory
+// stages of WK units; the parts are added over wk and the cluster's CTAs at the end.
+template <uint32_t TYPE, bool XB, int NB>
+__global__ void __launch_bounds__(512, 1) q4_gemm_kernel(Q4Args a, const uint8_t *ws, GemmPlan p) {
+    constexpr int NA = XB ? 4 : 2, UB = unit_bytes(TYPE);
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int tid = threadIdx.x, nthr = blockDim.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+    const int wn = warp % p.WN, wm = warp / p.WN % p.WM, wk = warp / (p.WN * p.WM);
+    const int COLS = p.WN * NB * 8, TOK = XB ? COLS : COLS / 2;
+    const int bunit = COLS * 256 + TOK * 16, tiles = 2 * p.WM, sunit = bunit + tiles * UB, stage_bytes = p.WK * sunit;
+    const int rank = p.S > 1 ? (int)cluster_rank() : 0;
+    const int u0 = (int)((long long)p.KT * rank / p.S), u1 = (int)((long long)p.KT * (rank + 1) / p.S), nu = u1 - u0;
+    const int rt0 = (int)(blockIdx.x / p.S) * tiles, iters = (nu + p.WK - 1) / p.WK;
+    const uint8_t *units = ws + kQ4InvBytes;
+
+    auto load_codes = [&](int it) {
+        if (it >= iters) return;
+        uint8_t *st = smem + (it % kGemmStages) * stage_bytes;
+        const int per = UB / 16, total = p.WK * tiles * per;
+        for (int i = tid; i < total; i += nthr) {
+            const int c = i % per, tile = i / per % tiles, k = i / (per * tiles), u = it * p.WK + k;
+            if (u < nu && rt0 + tile < p.RT)
+                cp_async16(st + k * sunit + bunit + tile * UB + c * 16,
+                           a.w + ((size_t)(rt0 + tile) * p.KT + u0 + u) * UB + c * 16);
+        }
+    };
+    auto load_frags = [&](int it) {
+        if (it >= iters) return;
+        uint8_t *st = smem + (it % kGemmStages) * stage_bytes;
+        const int per = bunit / 16, total = p.WK * per;
+        for (int i = tid; i < total; i += nthr) {
+            const int k = i / per, c = i - k * per, u = it * p.WK + k;
+            if (u < nu) cp_async16(st + k * sunit + c * 16, units + (size_t)(u0 + u) * bunit + c * 16);
+        }
+    };
+    // the weights never change: they may be fetched before the activations are packed
+#pragma unroll
+    for (int s = 0; s < kGemmStages - 1; ++s) load_codes(s);
+    pdl_launch_dependents();
+    pdl_wait();
+#pragma unroll
+    for (int s = 0; s < kGemmStages - 1; ++s) {
+        load_frags(s);
+        cp_async_commit();
+    }
+    float acc[2][NB][NA];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int k = 0; k < NA; ++k) acc[m][n][k] = 0.f;
+    for (int it = 0; it < iters; ++it) {
+        cp_async_wait<kGemmStages - 2>();
+        __syncthreads();
+        load_codes(it + kGemmStages - 1);
+        load_frags(it + kGemmStages - 1);
+        cp_async_commit();
+        if (it * p.WK + wk >= nu) continue;
+        const uint8_t *st = smem + (it % kGemmStages) * stage_bytes + wk * sunit;
+        const float *sums = reinterpret_cast<const float *>(st + COLS * 256);
+        uint4 c0[2], c1[2], dv[2], mv[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const uint8_t *t = st + bunit + (2 * wm + m) * UB;
+            c0[m] = reinterpret_cast<const uint4 *>(t)[lane];
+            c1[m] = reinterpret_cast<const uint4 *>(t + 512)[lane];
+            dv[m] = reinterpret_cast<const uint4 *>(t + 1024)[g];
+            if constexpr (TYPE == GX_Q4_1) mv[m] = reinterpret_cast<const uint4 *>(t + 1152)[g];
+        }
+        auto word = [](const uint4 &v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; };
+        auto half_of = [&](const uint4 &v, int hi, int j) {
+            const uint32_t w = word(v, 2 * hi + (j >> 1));
+            const __half2 h = *reinterpret_cast<const __half2 *>(&w);
+            return (j & 1) ? __high2float(h) : __low2float(h);
+        };
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t a0[2][4], a1[2][4];
+            float d[2][2], mm[2][2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                code_fragments<TYPE>(word(c0[m], j), word(c1[m], j), a0[m], a1[m]);
+#pragma unroll
+                for (int hi = 0; hi < 2; ++hi) {
+                    d[m][hi] = half_of(dv[m], hi, j);
+                    if constexpr (TYPE == GX_Q4_1) mm[m][hi] = half_of(mv[m], hi, j);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                const int nn = wn * NB + n;
+                const uint4 b = *reinterpret_cast<const uint4 *>(st + ((size_t)(j * COLS + 8 * nn) * 4 + lane) * 16);
+                float sx = 0.f, sy = 0.f;
+                if constexpr (TYPE == GX_Q4_0) {
+                } else if constexpr (XB) {
+                    const float2 v = *reinterpret_cast<const float2 *>(sums + j * TOK + 8 * nn + 2 * q);
+                    sx = v.x;
+                    sy = v.y;
+                } else {
+                    sx = sums[j * TOK + 4 * nn + q];
+                }
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma16816(c, a0[m], b.x, b.y);
+                    mma16816(c, a1[m], b.z, b.w);
+                    if constexpr (XB) {
+                        acc[m][n][0] = fmaf(d[m][0], c[0], acc[m][n][0]);
+                        acc[m][n][1] = fmaf(d[m][0], c[1], acc[m][n][1]);
+                        acc[m][n][2] = fmaf(d[m][1], c[2], acc[m][n][2]);
+                        acc[m][n][3] = fmaf(d[m][1], c[3], acc[m][n][3]);
+                        if constexpr (TYPE == GX_Q4_1) {
+                            acc[m][n][0] = fmaf(mm[m][0], sx, acc[m][n][0]);
+                            acc[m][n][1] = fmaf(mm[m][0], sy, acc[m][n][1]);
+                            acc[m][n][2] = fmaf(mm[m][1], sx, acc[m][n][2]);
+                            acc[m][n][3] = fmaf(mm[m][1], sy, acc[m][n][3]);
+                        }
+                    } else {
+                        acc[m][n][0] = fmaf(d[m][0], c[0] + c[1], acc[m][n][0]);
+                        acc[m][n][1] = fmaf(d[m][1], c[2] + c[3], acc[m][n][1]);
+                        if constexpr (TYPE == GX_Q4_1) {
+                            acc[m][n][0] = fmaf(mm[m][0], sx, acc[m][n][0]);
+                            acc[m][n][1] = fmaf(mm[m][1], sx, acc[m][n][1]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    cp_async_wait<0>();
+    __syncthreads();
+    // parts [WK][TOK][rows + 8] over the stages
+    const int rows = tiles * 16, ld = rows + 8, part = TOK * ld;
+    float *mine = reinterpret_cast<float *>(smem) + wk * part;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const int r = (2 * wm + m) * 16 + g, nn = wn * NB + n;
+            if constexpr (XB) {
+                const int t = 8 * nn + 2 * q;
+                mine[t * ld + r] = acc[m][n][0];
+                mine[(t + 1) * ld + r] = acc[m][n][1];
+                mine[t * ld + r + 8] = acc[m][n][2];
+                mine[(t + 1) * ld + r + 8] = acc[m][n][3];
+            } else {
+                const int t = 4 * nn + q;
+                mine[t * ld + r] = acc[m][n][0];
+                mine[t * ld + r + 8] = acc[m][n][1];
+            }
+        }
+    if (p.S > 1) cluster_sync_all();
+    else __syncthreads();
+    // the CTAs of a cluster share the sums out by tokens
+    const float *all = reinterpret_cast<const float *>(smem);
+    for (int i = rank * nthr + tid; i < a.n_tok * rows; i += p.S * nthr) {
+        const int t = i / rows, r = i - t * rows, row = rt0 * 16 + r;
+        if (row >= a.rows) continue;
+        float s = 0.f;
+        for (int c = 0; c < p.S; ++c)
+            for (int k = 0; k < p.WK; ++k) {
+                const float *at = all + k * part + t * ld + r;
+                s += p.S > 1 ? ld_cluster(at, (uint32_t)c) : *at;
+            }
+        store_act(a.y, a.y_bf16, (size_t)t * a.ldy + row, s * reinterpret_cast<const float *>(ws)[t]);
+    }
+    if (p.S > 1) cluster_sync_all();  // no CTA leaves while its parts are read
+}
+
+template <uint32_t TYPE, bool XB, int NB>
+cudaError_t launch_gemm_nb(const Q4Args &a, uint8_t *ws, GemmPlan p, int sm_count, cudaStream_t s) {
+    const int COLS = p.WN * NB * 8, TOK = XB ? COLS : COLS / 2;
+    const int bunit = COLS * 256 + TOK * 16;
+    auto ctas = [&] { return (p.RT + 2 * p.WM - 1) / (2 * p.WM); };
+    p.WM = p.WN == 1 ? 8 : 4;
+    p.WK = 1;
+    p.S = 1;
+    while (p.S < 8 && ctas() * p.S < sm_count * 3 / 2 && p.KT >= 4 * p.S) p.S *= 2;
+    auto ring = [&](int wm, int wk) { return kGemmStages * wk * (bunit + 2 * wm * unit_bytes(TYPE)); };
+    while (p.WM > 1 && ctas() * p.S < sm_count && p.KT >= 4 * p.S * p.WK && ring(p.WM / 2, p.WK * 2) <= kMaxSmem) {
+        p.WM /= 2;
+        p.WK *= 2;
+    }
+    const int parts = p.WK * TOK * (2 * p.WM * 16 + 8) * 4;
+    const int smem = ring(p.WM, p.WK) > parts ? ring(p.WM, p.WK) : parts;
+    if (smem > kMaxSmem) return cudaErrorInvalidValue;
+    const size_t esz = XB ? 2 : 4;
+    p.vec = ((uintptr_t)a.x & 15) == 0 && (a.ldx * esz) % 16 == 0;
+    cudaError_t e = launch_chain_pdl(true, q4_pack_kernel<TYPE, XB>, dim3((unsigned)a.n_tok), dim3(kPackThreads), 0, s, a, ws,
+                                     p.KT, COLS, p.vec);
+    if (e != cudaSuccess) return e;
+    auto *k = q4_gemm_kernel<TYPE, XB, NB>;
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(ctas() * p.S));
+    cfg.blockDim = dim3((unsigned)(p.WM * p.WN * p.WK * 32));
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)p.S;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.S > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, k, a, (const uint8_t *)ws, p);
+}
+
+template <uint32_t TYPE, bool XB>
+cudaError_t launch_gemm(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s) {
+    GemmPlan p{};
+    p.RT = (a.rows + kTileRows - 1) / kTileRows;
+    p.KT = (a.cols + kUnitCols - 1) / kUnitCols;
+    const int t8 = ((XB ? a.n_tok : 2 * a.n_tok) + 7) / 8;
+    p.WN = (t8 + 3) / 4;
+    return (t8 + p.WN - 1) / p.WN <= 3 ? launch_gemm_nb<TYPE, XB, 3>(a, ws, p, sm_count, s)
+                                       : launch_gemm_nb<TYPE, XB, 4>(a, ws, p, sm_count, s);
+}
+
+template <uint32_t TYPE, bool XB>
+cudaError_t launch_tokens(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s) {
     constexpr int T1 = XB ? 8 : 4;
+    if (a.n_tok > 2 * T1) return launch_gemm<TYPE, XB>(a, ws, sm_count, s);
+    // NT = 2 where its activations fit the cluster's shared memory
     const int KT = (a.cols + kUnitCols - 1) / kUnitCols;
     const int most = ((KT + 7) / 8) * XLayout<XB, 2>::UNIT_BYTES <= 160 * 1024 ? 2 * T1 : T1;
     for (int t0 = 0; t0 < a.n_tok; t0 += most) {
@@ -488,11 +827,16 @@ cudaError_t launch_q4_repack(uint32_t type, const uint8_t *raw, uint32_t rows, u
     return cudaGetLastError();
 }
 
-cudaError_t launch_q4_linear(const Q4Args &a, int sm_count, cudaStream_t s) {
+uint64_t q4_workspace_bytes(uint64_t cols) {
+    // 64 tokens in f32: 128 product columns of 64 B in each of a unit's groups, and 64 sums
+    return kQ4InvBytes + (cols + kUnitCols - 1) / kUnitCols * (4 * (128 * 64 + 64 * 4));
+}
+
+cudaError_t launch_q4_linear(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s) {
     if (a.n_tok <= 0 || a.rows <= 0) return cudaSuccess;
     if (a.type == GX_Q4_0)
-        return a.x_bf16 ? launch_tokens<GX_Q4_0, true>(a, sm_count, s) : launch_tokens<GX_Q4_0, false>(a, sm_count, s);
-    return a.x_bf16 ? launch_tokens<GX_Q4_1, true>(a, sm_count, s) : launch_tokens<GX_Q4_1, false>(a, sm_count, s);
+        return a.x_bf16 ? launch_tokens<GX_Q4_0, true>(a, ws, sm_count, s) : launch_tokens<GX_Q4_0, false>(a, ws, sm_count, s);
+    return a.x_bf16 ? launch_tokens<GX_Q4_1, true>(a, ws, sm_count, s) : launch_tokens<GX_Q4_1, false>(a, ws, sm_count, s);
 }
 
 }  // namespace gx
