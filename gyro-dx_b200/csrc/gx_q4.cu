@@ -37,8 +37,8 @@ namespace {
 // columns 8 q .. 8 q + 7, the k-slices its A registers hold:
 //   [32 lanes][4 groups] words of row g     code of column 8 q + i in bits 4 i .. 4 i + 3
 //   [32 lanes][4 groups] words of row g + 8
-//   [8 g][row g: 4 groups, row g + 8: 4 groups] fp16 d
-//   [8 g][the same] fp16 m                  (Q4_1)
+//   [8 g][4 groups][row g, row g + 8] fp16 d
+//   [8 g][4 groups][row g, row g + 8] fp16 m   (Q4_1)
 constexpr int kUnitCols = 128, kTileRows = 16;
 __host__ __device__ constexpr int unit_bytes(uint32_t type) { return type == GX_Q4_0 ? 1152 : 1280; }
 
@@ -73,32 +73,61 @@ __global__ void __launch_bounds__(256) q4_repack_kernel(uint32_t type, const uin
     }
     uint32_t *codes = reinterpret_cast<uint32_t *>(u + 512 * hi);
     for (int q = 0; q < 4; ++q) codes[(4 * g + q) * 4 + j] = words[q];
-    reinterpret_cast<uint16_t *>(u + 1024)[g * 8 + hi * 4 + j] = d;
-    if (type == GX_Q4_1) reinterpret_cast<uint16_t *>(u + 1152)[g * 8 + hi * 4 + j] = m;
+    reinterpret_cast<uint16_t *>(u + 1024)[(g * 4 + j) * 2 + hi] = d;
+    if (type == GX_Q4_1) reinterpret_cast<uint16_t *>(u + 1152)[(g * 4 + j) * 2 + hi] = m;
 }
 
 // ---- few tokens: a GEMV on mma.sync ------------------------------------------------------------
-struct Unit {
-    uint4 c0, c1, d, m;
-};
-template <uint32_t TYPE>
-__device__ __forceinline__ void load_unit(Unit &u, const uint8_t *p, int lane) {
-    u.c0 = __ldcs(reinterpret_cast<const uint4 *>(p) + lane);
-    u.c1 = __ldcs(reinterpret_cast<const uint4 *>(p + 512) + lane);
-    u.d = __ldcs(reinterpret_cast<const uint4 *>(p + 1024) + (lane >> 2));
-    if constexpr (TYPE == GX_Q4_1) u.m = __ldcs(reinterpret_cast<const uint4 *>(p + 1152) + (lane >> 2));
+__device__ __forceinline__ float half_value(uint32_t w, int hi) {
+    const __half2 h = *reinterpret_cast<const __half2 *>(&w);
+    return hi ? __high2float(h) : __low2float(h);
 }
 
-// Activations of one CTA's units in shared memory, for NT tiles of 8 product columns: a column is a
-// token in bf16, or the upper or lower part of a token in f32.
-//   frag [group][8 NT columns][4 q] 16 B    x of columns (0,4) (2,6) (1,5) (3,7) of 8 q ..
-//   sum  [group][tokens]                    sum x (Q4_1 only)
-//   inv  [unit][tokens]                     1 / scale
-template <bool XB, int NT>
-struct XLayout {
-    static constexpr int COLS = 8 * NT, TOK = XB ? 8 * NT : 4 * NT;
-    static constexpr int GROUP_BYTES = COLS * 64, UNIT_BYTES = 4 * GROUP_BYTES + 4 * TOK * 4 + TOK * 4;
+// A product tile has 8 columns. A token takes one of them in bf16 and two in f32 (its upper and its
+// lower part). P = 8 or 16 columns: P / 8 tiles per group, whose sums meet d at once. Fewer tokens
+// leave columns free, and those take other groups: with P = 2 (4) columns a group, 4 (2) groups share
+// one accumulator, the fragment of a group being zero in the columns of the others, so the scales,
+// conversions and sums of a lane are those of one group in 4 (2) and no column is idle.
+template <bool XB, int P>
+struct Few {
+    static constexpr int NT = P <= 8 ? 1 : P / 8, GPC = P < 8 ? 8 / P : 1, SETS = 4 / GPC;
+    static constexpr int TOK = XB ? P : P / 2, NA = XB ? 4 : 2, ATS = GPC > 1 ? 4 : NT;
+    // Activations of a CTA's units in shared memory:
+    //   frag [unit][4 groups][P columns][4 q] 16 B    x of columns (0,4) (2,6) (1,5) (3,7) of 8 q ..;
+    //                                                 with GPC > 1 then 64 B of zeros
+    //   sum  [group][tokens]                          sum x (Q4_1 only)
+    //   inv  [unit][tokens]                           1 / scale
+    static constexpr int GROUP_BYTES = P * 64, FRAG_BYTES = 4 * GROUP_BYTES + (GPC > 1 ? 64 : 0);
+    static constexpr int UNIT_BYTES = FRAG_BYTES + 4 * TOK * 4 + TOK * 4;
 };
+
+// A lane's part of a unit: the words of its two rows, and the scales (row g in the low half, row g + 8
+// in the high one) of the groups whose sums it holds.
+template <uint32_t TYPE, int SETS>
+struct Unit {
+    uint4 c0, c1;
+    uint32_t d[SETS], m[SETS];
+};
+// p: the lane's words of row g; its scales lie scale bytes after them.
+template <uint32_t TYPE, int SETS>
+__device__ __forceinline__ void load_unit(Unit<TYPE, SETS> &u, const uint8_t *p, int scale) {
+    u.c0 = __ldcs(reinterpret_cast<const uint4 *>(p));
+    u.c1 = __ldcs(reinterpret_cast<const uint4 *>(p + 512));
+    auto scales = [&](uint32_t (&d)[SETS], const uint8_t *at) {
+        if constexpr (SETS == 4) {
+            const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(at));
+            d[0] = v.x;
+            d[1] = v.y;
+            d[2] = v.z;
+            d[3] = v.w;
+        } else {
+#pragma unroll
+            for (int s = 0; s < SETS; ++s) d[s] = __ldcs(reinterpret_cast<const uint32_t *>(at + s * 8));
+        }
+    };
+    scales(u.d, p + scale);
+    if constexpr (TYPE == GX_Q4_1) scales(u.m, p + scale + 128);
+}
 
 // The 8 scaled values of columns 8 q .. of a group as the fragment of token t (column t in bf16; 2 t
 // and 2 t + 1, the upper and lower part, in f32).
@@ -119,19 +148,31 @@ __device__ __forceinline__ void put_fragment(uint8_t *group, int t, int q, const
     }
 }
 
+// The product of a group's first half on nothing (mma16816 adds the second to it).
+__device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // The A registers of 8 codes of row g (r0) and of row g + 8 (r1): columns (0,4) (2,6) of each in a0,
 // (1,5) (3,7) in a1.
 template <uint32_t TYPE>
 __device__ __forceinline__ void code_fragments(uint32_t r0, uint32_t r1, uint32_t (&a0)[4], uint32_t (&a1)[4]) {
     constexpr float off = TYPE == GX_Q4_0 ? 8.f : 0.f;
     const __half2 sub = __float2half2_rn(-1024.f - off), mul = __float2half2_rn(0.0625f), sub16 = __float2half2_rn(-64.f - off);
+    auto and_or = [](uint32_t v, uint32_t mask) {  // (v & mask) | 0x64006400
+        uint32_t h;
+        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(h) : "r"(v), "r"(mask), "r"(0x64006400u));
+        return h;
+    };
     auto low = [&](uint32_t v) {
-        const uint32_t h = (v & 0x000f000fu) | 0x64006400u;
+        const uint32_t h = and_or(v, 0x000f000fu);
         const __half2 r = __hadd2(*reinterpret_cast<const __half2 *>(&h), sub);
         return *reinterpret_cast<const uint32_t *>(&r);
     };
     auto high = [&](uint32_t v) {
-        const uint32_t h = (v & 0x00f000f0u) | 0x64006400u;
+        const uint32_t h = and_or(v, 0x00f000f0u);
         const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&h), mul, sub16);
         return *reinterpret_cast<const uint32_t *>(&r);
     };
@@ -145,10 +186,10 @@ __device__ __forceinline__ void code_fragments(uint32_t r0, uint32_t r1, uint32_
     a1[3] = high(r1 >> 8);
 }
 
-template <uint32_t TYPE, bool XB, int NT>
+template <uint32_t TYPE, bool XB, int P>
 __device__ __forceinline__ void stage_x(const Q4Args &a, int t0, int nt, int u0, int nu, uint8_t *frag, float *sum,
                                         float *inv, bool vec, int tid, int nthreads) {
-    using L = XLayout<XB, NT>;
+    using L = Few<XB, P>;
     const int cells = nu * 16, total = nt * cells;
     for (int base = 0; base < total; base += nthreads) {
         const int i = base + tid;
@@ -183,80 +224,88 @@ __device__ __forceinline__ void stage_x(const Q4Args &a, int t0, int nt, int u0,
         ss += __shfl_xor_sync(0xffffffffu, ss, 2);
         if (!on) continue;
         const int grp = cell >> 2, q = cell & 3;
-        put_fragment<XB>(frag + (size_t)grp * L::COLS * 64, t, q, v);
+        put_fragment<XB>(frag + (cell >> 4) * L::FRAG_BYTES + ((cell >> 2) & 3) * L::GROUP_BYTES, t, q, v);
         if (TYPE == GX_Q4_1 && q == 0) sum[grp * L::TOK + t] = ss;
         if ((cell & 15) == 0) inv[(cell >> 4) * L::TOK + t] = __uint_as_float((254u - se) << 23);
     }
 }
 
-// acc += the unit's products. acc[nt]: XB: (row g, token 2q), (g, 2q + 1), (g + 8, 2q), (g + 8, 2q + 1);
-// f32: (row g, token q), (row g + 8, token q).
-template <uint32_t TYPE, bool XB, int NT>
-__device__ __forceinline__ void unit_product(const Unit &u, int ul, const uint8_t *frag, const float *sum,
-                                             const float *inv, int lane, bool (&live)[NT], float (&acc)[NT][XB ? 4 : 2]) {
-    using L = XLayout<XB, NT>;
+// acc += the unit's products. acc[n]: XB: (row g, token c), (g, c + 1), (g + 8, c), (g + 8, c + 1) with
+// c = 8 n + 2 q mod P; f32: (row g, token c / 2), (row g + 8, token c / 2). at: the lane's fragment in a
+// group, for GPC == 1 in each product tile; for GPC > 1 in each group of the unit, the zeros for the
+// groups that its column does not belong to.
+template <uint32_t TYPE, bool XB, int P>
+__device__ __forceinline__ void unit_product(const Unit<TYPE, Few<XB, P>::SETS> &u, int ul, const uint8_t *frag,
+                                             const float *sum, const float *inv, int lane, const int (&at)[Few<XB, P>::ATS],
+                                             float (&acc)[Few<XB, P>::NT][Few<XB, P>::NA]) {
+    using L = Few<XB, P>;
     const int q = lane & 3;
     const uint32_t c0[4] = {u.c0.x, u.c0.y, u.c0.z, u.c0.w}, c1[4] = {u.c1.x, u.c1.y, u.c1.z, u.c1.w};
-    const uint32_t dw[4] = {u.d.x, u.d.y, u.d.z, u.d.w}, mw[4] = {u.m.x, u.m.y, u.m.z, u.m.w};
-    float part[NT][XB ? 4 : 2];
+    const uint8_t *fr = frag + ul * L::FRAG_BYTES;
+    float part[L::NT][L::NA], c[L::NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < L::NT; ++n)
 #pragma unroll
-        for (int k = 0; k < (XB ? 4 : 2); ++k) part[n][k] = 0.f;
+        for (int k = 0; k < L::NA; ++k) part[n][k] = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         uint32_t a0[4], a1[4];
         code_fragments<TYPE>(c0[j], c1[j], a0, a1);
-        auto half_of = [&](const uint32_t (&w)[4], int hi) {
-            const __half2 h = *reinterpret_cast<const __half2 *>(&w[2 * hi + (j >> 1)]);
-            return (j & 1) ? __high2float(h) : __low2float(h);
-        };
-        const float d0 = half_of(dw, 0), d1 = half_of(dw, 1);
-        const int grp = 4 * ul + j;
+        const int jj = j % L::GPC, set = j / L::GPC;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            uint4 b = make_uint4(0u, 0u, 0u, 0u);
-            if (live[n]) b = *reinterpret_cast<const uint4 *>(frag + ((size_t)(grp * L::COLS + 8 * n) * 4 + lane) * 16);
+        for (int n = 0; n < L::NT; ++n) {
+            if constexpr (L::GPC == 1) {
+                const uint4 b = *reinterpret_cast<const uint4 *>(fr + j * L::GROUP_BYTES + at[n]);
+                mma16816_first(c[n], a0, b.x, b.y);
+                mma16816(c[n], a1, b.z, b.w);
+            } else {
+                const uint4 b = *reinterpret_cast<const uint4 *>(fr + at[j]);
+                if (jj == 0) mma16816_first(c[0], a0, b.x, b.y);
+                else mma16816(c[0], a0, b.x, b.y);
+                mma16816(c[0], a1, b.z, b.w);
+            }
+        }
+        if (jj != L::GPC - 1) continue;
+        const float d0 = half_value(u.d[set], 0), d1 = half_value(u.d[set], 1);
+        const int grp = ul * 4 + set * L::GPC + (2 * q) / P;
+#pragma unroll
+        for (int n = 0; n < L::NT; ++n) {
+            const int col = 8 * n + (2 * q) % P;
             if constexpr (XB) {
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816(c, a0, b.x, b.y);
-                mma16816(c, a1, b.z, b.w);
-                part[n][0] = fmaf(d0, c[0], part[n][0]);
-                part[n][1] = fmaf(d0, c[1], part[n][1]);
-                part[n][2] = fmaf(d1, c[2], part[n][2]);
-                part[n][3] = fmaf(d1, c[3], part[n][3]);
+                part[n][0] = fmaf(d0, c[n][0], part[n][0]);
+                part[n][1] = fmaf(d0, c[n][1], part[n][1]);
+                part[n][2] = fmaf(d1, c[n][2], part[n][2]);
+                part[n][3] = fmaf(d1, c[n][3], part[n][3]);
                 if constexpr (TYPE == GX_Q4_1) {
-                    const float2 sx = *reinterpret_cast<const float2 *>(sum + grp * L::TOK + 8 * n + 2 * q);
-                    const float m0 = half_of(mw, 0), m1 = half_of(mw, 1);
+                    const float2 sx = *reinterpret_cast<const float2 *>(sum + grp * L::TOK + col);
+                    const float m0 = half_value(u.m[set], 0), m1 = half_value(u.m[set], 1);
                     part[n][0] = fmaf(m0, sx.x, part[n][0]);
                     part[n][1] = fmaf(m0, sx.y, part[n][1]);
                     part[n][2] = fmaf(m1, sx.x, part[n][2]);
                     part[n][3] = fmaf(m1, sx.y, part[n][3]);
                 }
             } else {
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816(c, a0, b.x, b.y);
-                mma16816(c, a1, b.z, b.w);
-                part[n][0] = fmaf(d0, c[0] + c[1], part[n][0]);
-                part[n][1] = fmaf(d1, c[2] + c[3], part[n][1]);
+                part[n][0] = fmaf(d0, c[n][0] + c[n][1], part[n][0]);
+                part[n][1] = fmaf(d1, c[n][2] + c[n][3], part[n][1]);
                 if constexpr (TYPE == GX_Q4_1) {
-                    const float sx = sum[grp * L::TOK + 4 * n + q];
-                    part[n][0] = fmaf(half_of(mw, 0), sx, part[n][0]);
-                    part[n][1] = fmaf(half_of(mw, 1), sx, part[n][1]);
+                    const float sx = sum[grp * L::TOK + col / 2];
+                    part[n][0] = fmaf(half_value(u.m[set], 0), sx, part[n][0]);
+                    part[n][1] = fmaf(half_value(u.m[set], 1), sx, part[n][1]);
                 }
             }
         }
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < L::NT; ++n) {
+        const int col = 8 * n + (2 * q) % P;
         if constexpr (XB) {
-            const float2 iv = *reinterpret_cast<const float2 *>(inv + ul * L::TOK + 8 * n + 2 * q);
+            const float2 iv = *reinterpret_cast<const float2 *>(inv + ul * L::TOK + col);
             acc[n][0] = fmaf(part[n][0], iv.x, acc[n][0]);
             acc[n][1] = fmaf(part[n][1], iv.y, acc[n][1]);
             acc[n][2] = fmaf(part[n][2], iv.x, acc[n][2]);
             acc[n][3] = fmaf(part[n][3], iv.y, acc[n][3]);
         } else {
-            const float iv = inv[ul * L::TOK + 4 * n + q];
+            const float iv = inv[ul * L::TOK + col / 2];
             acc[n][0] = fmaf(part[n][0], iv, acc[n][0]);
             acc[n][1] = fmaf(part[n][1], iv, acc[n][1]);
         }
@@ -294,13 +343,12 @@ __device__ __forceinline__ float ld_cluster(const float *p, uint32_t rank) {
 // a row tile in turn, with kDepth units in flight in registers across row tiles, and add their parts
 // in shared memory. With S > 1 each cluster has one pass of row tiles, its CTAs take S ranges of the
 // units, and rank 0 adds their parts.
-constexpr int gemv_ctas(int NT, int W) { return W == 16 ? 1 : NT == 1 ? 3 : 2; }  // resident on an SM
+constexpr int gemv_ctas(int P, int W) { return W == 16 ? 1 : P <= 8 ? 3 : 2; }  // resident on an SM
 
-template <uint32_t TYPE, bool XB, int NT, int W>
-__global__ void __launch_bounds__(W * 32, gemv_ctas(NT, W)) q4_gemv_kernel(Q4Args a, GemvPlan p) {
-    using L = XLayout<XB, NT>;
-    constexpr int kDepth = TYPE == GX_Q4_0 ? 3 : 2;
-    constexpr int NA = XB ? 4 : 2, RED = kTileRows * L::TOK;
+template <uint32_t TYPE, bool XB, int P, int W>
+__global__ void __launch_bounds__(W * 32, gemv_ctas(P, W)) q4_gemv_kernel(Q4Args a, GemvPlan p) {
+    using L = Few<XB, P>;
+    constexpr int kDepth = TYPE == GX_Q4_0 || P < 8 ? 3 : 2, NT = L::NT, NA = L::NA, RED = kTileRows * L::TOK;
     extern __shared__ __align__(16) uint8_t smem[];
     uint8_t *frag = smem;
     float *sum = reinterpret_cast<float *>(smem + p.sum_off), *inv = reinterpret_cast<float *>(smem + p.inv_off);
@@ -312,17 +360,25 @@ __global__ void __launch_bounds__(W * 32, gemv_ctas(NT, W)) q4_gemv_kernel(Q4Arg
     const int step = (int)(gridDim.x / p.S) * groups;
     const int rt0 = (int)(blockIdx.x / p.S) * groups + wg;
 
-    // cursor of the loads: row tile and unit
-    int lrt = rt0, lu = wk;
+    // cursor of the loads: the next unit of this warp, units left of its row tile, row tiles left
+    constexpr int UB = unit_bytes(TYPE);
     const bool idle = wk >= nu;  // more warps than units: this one only takes part in the sums
-    Unit buf[kDepth];
-    auto fetch = [&](Unit &u) {
-        if (!idle && lrt < p.RT) {
-            load_unit<TYPE>(u, a.w + ((size_t)lrt * p.KT + u0 + lu) * unit_bytes(TYPE), lane);
-            lu += p.WK;
-            if (lu >= nu) {
-                lu = wk;
-                lrt += step;
+    const int per = idle ? 0 : (nu - wk + p.WK - 1) / p.WK, scale_at = P == 2 ? lane * 4 : P == 4 ? (lane >> 1) * 4 + (lane >> 2) * 8 : (lane >> 2) * 16,
+              scale = 1024 + scale_at - lane * 16;
+    const uint8_t *lp = a.w + ((size_t)rt0 * p.KT + u0 + wk) * UB + lane * 16;
+    int lleft = per, ltiles = rt0 < p.RT && !idle ? (p.RT - rt0 + step - 1) / step : 0;
+    const int unit_step = p.WK * UB;
+    const long long tile_step = (long long)step * p.KT * UB - (long long)(per - 1) * unit_step;
+    Unit<TYPE, L::SETS> buf[kDepth];
+    auto fetch = [&](Unit<TYPE, L::SETS> &u) {
+        if (ltiles > 0) {
+            load_unit(u, lp, scale);
+            if (--lleft == 0) {
+                lleft = per;
+                --ltiles;
+                lp += tile_step;
+            } else {
+                lp += unit_step;
             }
         }
     };
@@ -330,12 +386,23 @@ __global__ void __launch_bounds__(W * 32, gemv_ctas(NT, W)) q4_gemv_kernel(Q4Arg
     for (int k = 0; k < kDepth; ++k) fetch(buf[k]);
     pdl_launch_dependents();
     pdl_wait();  // the weights never change; the activations may come from the kernel before
-    stage_x<TYPE, XB, NT>(a, p.t0, p.nt, u0, nu, frag, sum, inv, p.vec != 0, tid, W * 32);
+    if constexpr (L::GPC > 1)
+        for (int i = tid; i < nu * 4; i += W * 32)
+            *reinterpret_cast<uint4 *>(frag + (i >> 2) * L::FRAG_BYTES + 4 * L::GROUP_BYTES + (i & 3) * 16) = make_uint4(0u, 0u, 0u, 0u);
+    stage_x<TYPE, XB, P>(a, p.t0, p.nt, u0, nu, frag, sum, inv, p.vec != 0, tid, W * 32);
     __syncthreads();
 
-    bool live[NT];
+    // Columns without a token read the first one's fragment where nothing is stored of their sums, and
+    // the zeros where a column's sums meet those of others.
+    int at[L::ATS];
+    const int g = lane >> 2, live = XB ? p.nt : 2 * p.nt;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) live[n] = 8 * n + (lane >> 2) < (XB ? p.nt : 2 * p.nt);
+    for (int k = 0; k < L::ATS; ++k) {
+        if constexpr (L::GPC > 1)
+            at[k] = (g / P == k % L::GPC && g % P < live ? k * L::GROUP_BYTES + g % P * 64 : 4 * L::GROUP_BYTES) + (lane & 3) * 16;
+        else
+            at[k] = (8 * k + g < live ? 8 * k + g : 0) * 64 + (lane & 3) * 16;
+    }
     float acc[NT][NA];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -343,17 +410,26 @@ __global__ void __launch_bounds__(W * 32, gemv_ctas(NT, W)) q4_gemv_kernel(Q4Arg
         for (int k = 0; k < NA; ++k) acc[n][k] = 0.f;
     int rt = rt0, ul = wk, parity = 0;
     auto put = [&](float *dst) {  // the warp's part as [token][16 rows]
-        const int g = lane >> 2, q = lane & 3;
+        const int q = lane & 3;
+        if constexpr (L::GPC > 1) {  // the lanes of a row add up their groups
+#pragma unroll
+            for (int k = 0; k < NA; ++k) {
+                if (P == 2) acc[0][k] += __shfl_xor_sync(0xffffffffu, acc[0][k], 1);
+                acc[0][k] += __shfl_xor_sync(0xffffffffu, acc[0][k], 2);
+            }
+            if (q >= P / 2) return;
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+            const int col = 8 * n + 2 * q;
             if constexpr (XB) {
-                dst[(8 * n + 2 * q) * 16 + g] = acc[n][0];
-                dst[(8 * n + 2 * q + 1) * 16 + g] = acc[n][1];
-                dst[(8 * n + 2 * q) * 16 + g + 8] = acc[n][2];
-                dst[(8 * n + 2 * q + 1) * 16 + g + 8] = acc[n][3];
+                dst[col * 16 + g] = acc[n][0];
+                dst[(col + 1) * 16 + g] = acc[n][1];
+                dst[col * 16 + g + 8] = acc[n][2];
+                dst[(col + 1) * 16 + g + 8] = acc[n][3];
             } else {
-                dst[(4 * n + q) * 16 + g] = acc[n][0];
-                dst[(4 * n + q) * 16 + g + 8] = acc[n][1];
+                dst[col / 2 * 16 + g] = acc[n][0];
+                dst[col / 2 * 16 + g + 8] = acc[n][1];
             }
         }
     };
@@ -390,7 +466,7 @@ __global__ void __launch_bounds__(W * 32, gemv_ctas(NT, W)) q4_gemv_kernel(Q4Arg
 #pragma unroll
         for (int k = 0; k < kDepth; ++k) {
             if (rt >= p.RT) break;
-            unit_product<TYPE, XB, NT>(buf[k], ul, frag, sum, inv, lane, live, acc);
+            unit_product<TYPE, XB, P>(buf[k], ul, frag, sum, inv, lane, at, acc);
             fetch(buf[k]);
             ul += p.WK;
             if (ul >= nu) {
@@ -415,9 +491,9 @@ __global__ void __launch_bounds__(W * 32, gemv_ctas(NT, W)) q4_gemv_kernel(Q4Arg
     }
 }
 
-template <uint32_t TYPE, bool XB, int NT, int W>
+template <uint32_t TYPE, bool XB, int P, int W>
 cudaError_t launch_gemv_w(const Q4Args &a, GemvPlan p, int smem, int grid, cudaStream_t s) {
-    auto *k = q4_gemv_kernel<TYPE, XB, NT, W>;
+    auto *k = q4_gemv_kernel<TYPE, XB, P, W>;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -436,9 +512,9 @@ cudaError_t launch_gemv_w(const Q4Args &a, GemvPlan p, int smem, int grid, cudaS
     return cudaLaunchKernelEx(&cfg, k, a, p);
 }
 
-template <uint32_t TYPE, bool XB, int NT>
+template <uint32_t TYPE, bool XB, int P>
 cudaError_t launch_gemv(const Q4Args &a, int t0, int nt, int sm_count, cudaStream_t s) {
-    using L = XLayout<XB, NT>;
+    using L = Few<XB, P>;
     GemvPlan p{};
     p.RT = (a.rows + kTileRows - 1) / kTileRows;
     p.KT = (a.cols + kUnitCols - 1) / kUnitCols;
@@ -459,15 +535,15 @@ cudaError_t launch_gemv(const Q4Args &a, int t0, int nt, int sm_count, cudaStrea
     const int xbytes = nu * L::UNIT_BYTES;
     const bool wide = xbytes > 56 * 1024;  // few CTAs fit an SM: 16 warps each instead of 8
     const int W = wide ? 16 : 8;
-    p.sum_off = nu * 4 * L::GROUP_BYTES;
+    p.sum_off = nu * L::FRAG_BYTES;
     p.inv_off = p.sum_off + nu * 4 * L::TOK * 4;
     p.red_off = (p.inv_off + nu * L::TOK * 4 + 15) / 16 * 16;
     const int smem = p.red_off + 2 * W * kTileRows * L::TOK * 4;
     if (smem > kMaxSmem) return cudaErrorInvalidValue;
     const int groups = W / p.WK, need = (p.RT + groups - 1) / groups;
-    const int resident = sm_count * gemv_ctas(NT, W);
+    const int resident = sm_count * gemv_ctas(P, W);
     const int grid = p.S > 1 ? need * p.S : need < resident ? need : resident;
-    return wide ? launch_gemv_w<TYPE, XB, NT, 16>(a, p, smem, grid, s) : launch_gemv_w<TYPE, XB, NT, 8>(a, p, smem, grid, s);
+    return wide ? launch_gemv_w<TYPE, XB, P, 16>(a, p, smem, grid, s) : launch_gemv_w<TYPE, XB, P, 8>(a, p, smem, grid, s);
 }
 
 // ---- more tokens: a tiled product on mma.sync ---------------------------------------------------
@@ -638,11 +714,7 @@ __global__ void __launch_bounds__(512, 1) q4_gemm_kernel(Q4Args a, const uint8_t
             if constexpr (TYPE == GX_Q4_1) mv[m] = reinterpret_cast<const uint4 *>(t + 1152)[g];
         }
         auto word = [](const uint4 &v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; };
-        auto half_of = [&](const uint4 &v, int hi, int j) {
-            const uint32_t w = word(v, 2 * hi + (j >> 1));
-            const __half2 h = *reinterpret_cast<const __half2 *>(&w);
-            return (j & 1) ? __high2float(h) : __low2float(h);
-        };
+        auto half_of = [&](const uint4 &v, int hi, int j) { return half_value(word(v, j), hi); };
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             uint32_t a0[2][4], a1[2][4];
@@ -671,8 +743,8 @@ __global__ void __launch_bounds__(512, 1) q4_gemm_kernel(Q4Args a, const uint8_t
                 }
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma16816(c, a0[m], b.x, b.y);
+                    float c[4];
+                    mma16816_first(c, a0[m], b.x, b.y);
                     mma16816(c, a1[m], b.z, b.w);
                     if constexpr (XB) {
                         acc[m][n][0] = fmaf(d[m][0], c[0], acc[m][n][0]);
@@ -793,13 +865,15 @@ template <uint32_t TYPE, bool XB>
 cudaError_t launch_tokens(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s) {
     constexpr int T1 = XB ? 8 : 4;
     if (a.n_tok > 2 * T1) return launch_gemm<TYPE, XB>(a, ws, sm_count, s);
-    // NT = 2 where its activations fit the cluster's shared memory
+    // 16 columns where their activations fit the cluster's shared memory, else 8 at a time
     const int KT = (a.cols + kUnitCols - 1) / kUnitCols;
-    const int most = ((KT + 7) / 8) * XLayout<XB, 2>::UNIT_BYTES <= 160 * 1024 ? 2 * T1 : T1;
+    const int most = ((KT + 7) / 8) * Few<XB, 16>::UNIT_BYTES <= 160 * 1024 ? 2 * T1 : T1;
     for (int t0 = 0; t0 < a.n_tok; t0 += most) {
-        const int nt = a.n_tok - t0 < most ? a.n_tok - t0 : most;
-        const cudaError_t e = nt <= T1 ? launch_gemv<TYPE, XB, 1>(a, t0, nt, sm_count, s)
-                                       : launch_gemv<TYPE, XB, 2>(a, t0, nt, sm_count, s);
+        const int nt = a.n_tok - t0 < most ? a.n_tok - t0 : most, cols = XB ? nt : 2 * nt;
+        const cudaError_t e = cols <= 2   ? launch_gemv<TYPE, XB, 2>(a, t0, nt, sm_count, s)
+                              : cols <= 4 ? launch_gemv<TYPE, XB, 4>(a, t0, nt, sm_count, s)
+                              : cols <= 8 ? launch_gemv<TYPE, XB, 8>(a, t0, nt, sm_count, s)
+                                          : launch_gemv<TYPE, XB, 16>(a, t0, nt, sm_count, s);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
