@@ -83,24 +83,6 @@ __device__ __forceinline__ float half_value(uint32_t w, int hi) {
     return hi ? __high2float(h) : __low2float(h);
 }
 
-// A product tile has 8 columns. A token takes one of them in bf16 and two in f32 (its upper and its
-// lower part). P = 8 or 16 columns: P / 8 tiles per group, whose sums meet d at once. Fewer tokens
-// leave columns free, and those take other groups: with P = 2 (4) columns a group, 4 (2) groups share
-// one accumulator, the fragment of a group being zero in the columns of the others, so the scales,
-// conversions and sums of a lane are those of one group in 4 (2) and no column is idle.
-template <bool XB, int P>
-struct Few {
-    static constexpr int NT = P <= 8 ? 1 : P / 8, GPC = P < 8 ? 8 / P : 1, SETS = 4 / GPC;
-    static constexpr int TOK = XB ? P : P / 2, NA = XB ? 4 : 2, ATS = GPC > 1 ? 4 : NT;
-    // Activations of a CTA's units in shared memory:
-    //   frag [unit][4 groups][P columns][4 q] 16 B    x of columns (0,4) (2,6) (1,5) (3,7) of 8 q ..;
-    //                                                 with GPC > 1 then 64 B of zeros
-    //   sum  [group][tokens]                          sum x (Q4_1 only)
-    //   inv  [unit][tokens]                           1 / scale
-    static constexpr int GROUP_BYTES = P * 64, FRAG_BYTES = 4 * GROUP_BYTES + (GPC > 1 ? 64 : 0);
-    static constexpr int UNIT_BYTES = FRAG_BYTES + 4 * TOK * 4 + TOK * 4;
-};
-
 // A lane's part of a unit: the words of its two rows, and the scales (row g in the low half, row g + 8
 // in the high one) of the groups whose sums it holds.
 template <uint32_t TYPE, int SETS>
@@ -186,131 +168,329 @@ __device__ __forceinline__ void code_fragments(uint32_t r0, uint32_t r1, uint32_
     a1[3] = high(r1 >> 8);
 }
 
-template <uint32_t TYPE, bool XB, int P>
-__device__ __forceinline__ void stage_x(const Q4Args &a, int t0, int nt, int u0, int nu, uint8_t *frag, float *sum,
-                                        float *inv, bool vec, int tid, int nthreads) {
-    using L = Few<XB, P>;
-    const int cells = nu * 16, total = nt * cells;
-    for (int base = 0; base < total; base += nthreads) {
-        const int i = base + tid;
-        const bool on = i < total;
-        const int t = on ? i / cells : 0, cell = on ? i % cells : 0, col = u0 * kUnitCols + cell * 8;
-        float v[8];
+// One token's 8 columns of a unit of a CTA's range: its values (0 past the matrix), and the largest
+// magnitude of the unit by its bits (16 lanes hold a unit; an Inf or NaN has the largest exponent).
+template <bool XB>
+__device__ __forceinline__ uint32_t load_cell(const Q4Args &a, int t, int col, bool on, bool vec, float (&v)[8]) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = 0.f;
-        if (on && col < a.cols) {  // cols is a multiple of 32: a cell is inside or outside
-            const size_t at = (size_t)(t0 + t) * a.ldx + col;
-            if (vec) load_x8(a.x, XB, at, v);
-            else {
+    for (int k = 0; k < 8; ++k) v[k] = 0.f;
+    if (on && col < a.cols) {  // cols is a multiple of 32: a cell is inside or outside
+        const size_t at = (size_t)t * a.ldx + col;
+        if (vec) load_x8(a.x, XB, at, v);
+        else {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = load_act(a.x, XB, at + k);
-            }
+            for (int k = 0; k < 8; ++k) v[k] = load_act(a.x, XB, at + k);
         }
-        // the unit's largest magnitude, by its bits (an Inf or NaN has the largest exponent)
-        uint32_t big = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) big = max(big, __float_as_uint(v[k]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
-        const uint32_t e = big >> 23, se = min(268u - e, 247u);
-        const float s = __uint_as_float(se << 23);
-        float ss = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            v[k] = e == 255u ? __uint_as_float(0x7fffffffu) : v[k] * s;
-            ss += v[k];
-        }
-        ss += __shfl_xor_sync(0xffffffffu, ss, 1);
-        ss += __shfl_xor_sync(0xffffffffu, ss, 2);
-        if (!on) continue;
-        const int grp = cell >> 2, q = cell & 3;
-        put_fragment<XB>(frag + (cell >> 4) * L::FRAG_BYTES + ((cell >> 2) & 3) * L::GROUP_BYTES, t, q, v);
-        if (TYPE == GX_Q4_1 && q == 0) sum[grp * L::TOK + t] = ss;
-        if ((cell & 15) == 0) inv[(cell >> 4) * L::TOK + t] = __uint_as_float((254u - se) << 23);
     }
+    uint32_t big = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) big = max(big, __float_as_uint(v[k]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+    return big;
+}
+template <typename T>
+__device__ __forceinline__ T quad_sum(T v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
 
-// acc += the unit's products. acc[n]: XB: (row g, token c), (g, c + 1), (g + 8, c), (g + 8, c + 1) with
-// c = 8 n + 2 q mod P; f32: (row g, token c / 2), (row g + 8, token c / 2). at: the lane's fragment in a
-// group, for GPC == 1 in each product tile; for GPC > 1 in each group of the unit, the zeros for the
-// groups that its column does not belong to.
-template <uint32_t TYPE, bool XB, int P>
-__device__ __forceinline__ void unit_product(const Unit<TYPE, Few<XB, P>::SETS> &u, int ul, const uint8_t *frag,
-                                             const float *sum, const float *inv, int lane, const int (&at)[Few<XB, P>::ATS],
-                                             float (&acc)[Few<XB, P>::NT][Few<XB, P>::NA]) {
-    using L = Few<XB, P>;
-    const int q = lane & 3;
-    const uint32_t c0[4] = {u.c0.x, u.c0.y, u.c0.z, u.c0.w}, c1[4] = {u.c1.x, u.c1.y, u.c1.z, u.c1.w};
-    const uint8_t *fr = frag + ul * L::FRAG_BYTES;
-    float part[L::NT][L::NA], c[L::NT][4];
+// Two ways to multiply a unit by few tokens. Each stages the activations of a CTA's units in shared
+// memory, a block of BYTES per unit, and gives a lane's part of the sums of rows g and g + 8.
+//
+// Ints: one or two tokens on the integer tensor cores. Here the arithmetic around the product is what
+// costs, and codes are integers already: two ands and a shift turn a word of 8 into A registers
+// of m16n8k32 (u8), a third of the work of the f16 form. A value becomes a whole number of 2^-29 of its
+// unit's power of two (30 bits), its four signed base-256 digits four columns of the product, exact in
+// 32 bits; -8 sum of digits is the initial accumulator, under an offset (2^23 + 2^22 as f32 bits) that
+// makes the result a float by itself. One token's 4 columns leave 4 free: two groups share an
+// accumulator, the fragment of each being zero in the columns of the other.
+template <uint32_t TYPE, bool XB, int T>
+struct Ints {
+    static constexpr int TOK = T, NA = 2, SETS = T == 1 ? 2 : 4, kDepth = 3;  // units in flight
+    static constexpr int CTAS(int W) { return W == 16 ? 1 : 3; }             // resident on an SM
+    // [4 groups][T tokens][4 digits][4 q] 8 B: the digit of columns (0 2 4 6) and (1 3 5 7) of 8 q ..
+    static constexpr int GROUP = T * 128, ZERO = 4 * GROUP;       // T == 1: 32 B of zeros
+    static constexpr int INIT = ZERO + (T == 1 ? 32 : 0);         // Q4_0: [group][token][digit pair] int4 accumulators
+    static constexpr int SUM = INIT;                              // Q4_1: [group][token][digit pair] float: sum x, 0
+    static constexpr int INV = TYPE == GX_Q4_0 ? INIT + T * 128 : SUM + T * 32;  // [token] float: 2^24 units of the numbers
+    static constexpr int BYTES = (INV + T * 4 + 15) / 16 * 16;
+    static constexpr uint32_t kOffset = 0x4b400000u;              // 2^23 + 2^22 as a float
+
+    int at[4];       // the lane's fragment in each group
+    float w0, w1;    // weights of the digits that its accumulator columns hold
+    float acc[NA];   // rows g and g + 8; T == 2: token q >> 1
+
+    __device__ __forceinline__ void init(int lane, int nt) {
+        const int g = lane >> 2, q = lane & 3;
 #pragma unroll
-    for (int n = 0; n < L::NT; ++n)
+        for (int j = 0; j < 4; ++j)
+            at[j] = T == 2 ? j * GROUP + ((g >> 2) < nt ? g : (g & 3)) * 32 + q * 8
+                           : (g >> 2 == (j & 1) ? j * GROUP + (g & 3) * 32 : ZERO) + q * 8;
+        w0 = (q & 1) ? 0x1p-16f : 1.f;
+        w1 = (q & 1) ? 0x1p-24f : 0x1p-8f;
+    }
+    static __device__ __forceinline__ int scale_offset(int lane) {
+        return T == 1 ? (lane >> 1) * 4 + (lane >> 2) * 8 : (lane >> 2) * 16;
+    }
+    static __device__ void stage(const Q4Args &a, int t0, int nt, int u0, int nu, uint8_t *smem, bool vec, int tid, int nthreads) {
+        const int cells = nu * 16, total = nt * cells;
+        for (int base = 0; base < total; base += nthreads) {
+            const int i = base + tid;
+            const bool on = i < total;
+            const int t = on ? i / cells : 0, cell = on ? i % cells : 0, q = cell & 3, j = (cell >> 2) & 3;
+            float v[8];
+            const uint32_t big = load_cell<XB>(a, t0 + t, u0 * kUnitCols + cell * 8, on, vec, v), e = big >> 23;
+            // 2^k with the unit's largest value below 2^30, as two factors: it may pass the f32 range
+            const int k = 29 + 127 - (int)max(min(e, 254u), 1u), k1 = k / 2, k2 = k - k1;
+            const float s1 = __uint_as_float((uint32_t)(127 + k1) << 23), s2 = __uint_as_float((uint32_t)(127 + k2) << 23);
+            uint32_t b[8];
+            float fs = 0.f;
 #pragma unroll
-        for (int k = 0; k < L::NA; ++k) part[n][k] = 0.f;
+            for (int c = 0; c < 8; ++c) {
+                const float x = e == 255u ? 0.f : v[c] * s1 * s2;
+                b[c] = ((uint32_t)__float2int_rn(x) + 0x00808080u) ^ 0x00808080u;  // signed digits, byte by byte
+                fs += v[c];
+            }
+            uint32_t w[2][4];  // [half of the columns][digit, most significant first]
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        uint32_t a0[4], a1[4];
-        code_fragments<TYPE>(c0[j], c1[j], a0, a1);
-        const int jj = j % L::GPC, set = j / L::GPC;
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t lo01 = __byte_perm(b[h], b[h + 2], 0x5140), hi01 = __byte_perm(b[h], b[h + 2], 0x7362);
+                const uint32_t lo23 = __byte_perm(b[h + 4], b[h + 6], 0x5140), hi23 = __byte_perm(b[h + 4], b[h + 6], 0x7362);
+                w[h][3] = __byte_perm(lo01, lo23, 0x5410);
+                w[h][2] = __byte_perm(lo01, lo23, 0x7632);
+                w[h][1] = __byte_perm(hi01, hi23, 0x5410);
+                w[h][0] = __byte_perm(hi01, hi23, 0x7632);
+            }
+            int ds[4];
 #pragma unroll
-        for (int n = 0; n < L::NT; ++n) {
-            if constexpr (L::GPC == 1) {
-                const uint4 b = *reinterpret_cast<const uint4 *>(fr + j * L::GROUP_BYTES + at[n]);
-                mma16816_first(c[n], a0, b.x, b.y);
-                mma16816(c[n], a1, b.z, b.w);
+            for (int d = 0; d < 4; ++d) ds[d] = __dp4a((int)w[0][d], 0x01010101, __dp4a((int)w[1][d], 0x01010101, 0));
+            if constexpr (TYPE == GX_Q4_0) {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) ds[d] = (int)kOffset - 8 * quad_sum(ds[d]);
             } else {
-                const uint4 b = *reinterpret_cast<const uint4 *>(fr + at[j]);
-                if (jj == 0) mma16816_first(c[0], a0, b.x, b.y);
-                else mma16816(c[0], a0, b.x, b.y);
-                mma16816(c[0], a1, b.z, b.w);
+                fs = quad_sum(fs);
+            }
+            if (!on) continue;
+            uint8_t *u = smem + (cell >> 4) * BYTES;
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+                *reinterpret_cast<uint2 *>(u + j * GROUP + (t * 4 + d) * 32 + q * 8) = make_uint2(w[0][d], w[1][d]);
+            if (q == 0) {
+                if constexpr (TYPE == GX_Q4_0) {
+                    int4 *n = reinterpret_cast<int4 *>(u + INIT) + (j * T + t) * 2;
+                    n[0] = make_int4(ds[0], ds[1], ds[0], ds[1]);
+                    n[1] = make_int4(ds[2], ds[3], ds[2], ds[3]);
+                } else {
+                    reinterpret_cast<float2 *>(u + SUM)[j * T + t] = make_float2(fs, 0.f);
+                }
+            }
+            if ((cell & 15) == 0) {
+                reinterpret_cast<float *>(u + INV)[t] =
+                    e == 255u ? __uint_as_float(0x7fffffffu)
+                              : __uint_as_float((uint32_t)(151 - k1) << 23) * __uint_as_float((uint32_t)(127 - k2) << 23);
+                if constexpr (T == 1) {
+                    reinterpret_cast<uint4 *>(u + ZERO)[0] = make_uint4(0u, 0u, 0u, 0u);
+                    reinterpret_cast<uint4 *>(u + ZERO)[1] = make_uint4(0u, 0u, 0u, 0u);
+                }
             }
         }
-        if (jj != L::GPC - 1) continue;
-        const float d0 = half_value(u.d[set], 0), d1 = half_value(u.d[set], 1);
-        const int grp = ul * 4 + set * L::GPC + (2 * q) / P;
+    }
+    __device__ __forceinline__ void unit(const Unit<TYPE, SETS> &u, const uint8_t *x, int lane) {
+        const int q = lane & 3;
+        const uint32_t c0[4] = {u.c0.x, u.c0.y, u.c0.z, u.c0.w}, c1[4] = {u.c1.x, u.c1.y, u.c1.z, u.c1.w};
+        const float inv = reinterpret_cast<const float *>(x + INV)[T == 1 ? 0 : q >> 1], v0 = inv * w0, v1 = inv * w1;
+        int4 c;
 #pragma unroll
-        for (int n = 0; n < L::NT; ++n) {
+        for (int j = 0; j < 4; ++j) {
+            constexpr uint32_t M = 0x0f0f0f0fu;
+            const uint32_t a[4] = {c0[j] & M, c1[j] & M, (c0[j] >> 4) & M, (c1[j] >> 4) & M};
+            const bool first = T == 2 || (j & 1) == 0, last = T == 2 || (j & 1) == 1;
+            const int set = T == 2 ? j : j >> 1;
+            const int row = set * 4 + q;  // [group][token][digit pair] of the lane's columns
+            if (first) {
+                if constexpr (TYPE == GX_Q4_0) c = reinterpret_cast<const int4 *>(x + INIT)[row];
+                else c = make_int4(kOffset, kOffset, kOffset, kOffset);
+            }
+            const uint2 b = *reinterpret_cast<const uint2 *>(x + at[j]);
+            asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                : "+r"(c.x), "+r"(c.y), "+r"(c.z), "+r"(c.w)
+                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+            if (!last) continue;
+            constexpr float off = 12582912.f;
+            const float f0 = __int_as_float(c.x) - off, f1 = __int_as_float(c.y) - off;
+            const float f2 = __int_as_float(c.z) - off, f3 = __int_as_float(c.w) - off;
+            acc[0] = fmaf(half_value(u.d[set], 0), fmaf(f1, v1, f0 * v0), acc[0]);
+            acc[1] = fmaf(half_value(u.d[set], 1), fmaf(f3, v1, f2 * v0), acc[1]);
+            if constexpr (TYPE == GX_Q4_1) {
+                const float sx = reinterpret_cast<const float *>(x + SUM)[row];
+                acc[0] = fmaf(half_value(u.m[set], 0), sx, acc[0]);
+                acc[1] = fmaf(half_value(u.m[set], 1), sx, acc[1]);
+            }
+        }
+    }
+    __device__ __forceinline__ void put(float *dst, int lane) {  // [token][16 rows]
+        const int g = lane >> 2, q = lane & 3;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], 1);
+            if (T == 1) acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], 2);
+        }
+        if (T == 1 ? q == 0 : (q & 1) == 0) {
+            dst[(q >> 1) * 16 + g] = acc[0];
+            dst[(q >> 1) * 16 + g + 8] = acc[1];
+        }
+    }
+    __device__ __forceinline__ void clear() { acc[0] = acc[1] = 0.f; }
+};
+
+// Halves: more tokens, P product columns of f16: a token takes one in bf16 and two in f32 (its upper
+// and lower part). P = 4 leaves columns free, which a second group takes as in Ints.
+template <uint32_t TYPE, bool XB, int P>
+struct Halves {
+    static constexpr int NT = P <= 8 ? 1 : P / 8, GPC = P < 8 ? 8 / P : 1, SETS = 4 / GPC, ATS = GPC > 1 ? 4 : NT;
+    static constexpr int TOK = XB ? P : P / 2, NA = XB ? 4 : 2, kDepth = TYPE == GX_Q4_0 || P < 8 ? 3 : 2;
+    static constexpr int CTAS(int W) { return W == 16 ? 1 : P <= 8 ? 3 : 2; }
+    // [4 groups][P columns][4 q] 16 B: x of columns (0,4) (2,6) (1,5) (3,7) of 8 q ..
+    static constexpr int GROUP = P * 64, ZERO = 4 * GROUP;        // GPC > 1: 64 B of zeros
+    static constexpr int SUM = ZERO + (GPC > 1 ? 64 : 0);         // Q4_1: [group][token] float: sum x
+    static constexpr int INV = SUM + (TYPE == GX_Q4_1 ? 4 * TOK * 4 : 0);  // [token] float: 1 / scale
+    static constexpr int BYTES = (INV + TOK * 4 + 15) / 16 * 16;
+
+    int at[ATS];          // the lane's fragment in each tile of a group; GPC > 1: in each group
+    float acc[NT][NA];    // XB: (row g, token c), (g, c + 1), (g + 8, c), (g + 8, c + 1), c = 8 n + 2 q mod P;
+                          // f32: (row g, token c / 2), (row g + 8, token c / 2)
+
+    __device__ __forceinline__ void init(int lane, int nt) {
+        // Columns without a token read the first one's fragment where nothing is stored of their sums,
+        // and the zeros where a column's sums meet those of others.
+        const int g = lane >> 2, q = lane & 3, live = XB ? nt : 2 * nt;
+#pragma unroll
+        for (int k = 0; k < ATS; ++k) {
+            if constexpr (GPC > 1) at[k] = (g / P == k % GPC && g % P < live ? k * GROUP + g % P * 64 : ZERO) + q * 16;
+            else at[k] = (8 * k + g < live ? 8 * k + g : 0) * 64 + q * 16;
+        }
+    }
+    static __device__ __forceinline__ int scale_offset(int lane) {
+        return P == 4 ? (lane >> 1) * 4 + (lane >> 2) * 8 : (lane >> 2) * 16;
+    }
+    static __device__ void stage(const Q4Args &a, int t0, int nt, int u0, int nu, uint8_t *smem, bool vec, int tid, int nthreads) {
+        const int cells = nu * 16, total = nt * cells;
+        for (int base = 0; base < total; base += nthreads) {
+            const int i = base + tid;
+            const bool on = i < total;
+            const int t = on ? i / cells : 0, cell = on ? i % cells : 0, q = cell & 3, j = (cell >> 2) & 3;
+            float v[8];
+            const uint32_t e = load_cell<XB>(a, t0 + t, u0 * kUnitCols + cell * 8, on, vec, v) >> 23, se = min(268u - e, 247u);
+            const float s = __uint_as_float(se << 23);
+            float ss = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                v[k] = e == 255u ? __uint_as_float(0x7fffffffu) : v[k] * s;
+                ss += v[k];
+            }
+            if constexpr (TYPE == GX_Q4_1) ss = quad_sum(ss);
+            if (!on) continue;
+            uint8_t *u = smem + (cell >> 4) * BYTES;
+            put_fragment<XB>(u + j * GROUP, t, q, v);
+            if (TYPE == GX_Q4_1 && q == 0) reinterpret_cast<float *>(u + SUM)[j * TOK + t] = ss;
+            if ((cell & 15) == 0) reinterpret_cast<float *>(u + INV)[t] = __uint_as_float((254u - se) << 23);
+            if (GPC > 1 && (cell & 12) == 0) reinterpret_cast<uint4 *>(u + ZERO)[q] = make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+    __device__ __forceinline__ void unit(const Unit<TYPE, SETS> &u, const uint8_t *x, int lane) {
+        const int q = lane & 3;
+        const uint32_t c0[4] = {u.c0.x, u.c0.y, u.c0.z, u.c0.w}, c1[4] = {u.c1.x, u.c1.y, u.c1.z, u.c1.w};
+        float part[NT][NA], c[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < NA; ++k) part[n][k] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t a0[4], a1[4];
+            code_fragments<TYPE>(c0[j], c1[j], a0, a1);
+            const int jj = j % GPC, set = j / GPC;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const uint4 b = *reinterpret_cast<const uint4 *>(x + (GPC > 1 ? at[j] : j * GROUP + at[n]));
+                if (jj == 0) mma16816_first(c[n], a0, b.x, b.y);
+                else mma16816(c[n], a0, b.x, b.y);
+                mma16816(c[n], a1, b.z, b.w);
+            }
+            if (jj != GPC - 1) continue;
+            const float d0 = half_value(u.d[set], 0), d1 = half_value(u.d[set], 1);
+            const float *sum = reinterpret_cast<const float *>(x + SUM) + (set * GPC + (2 * q) / P) * TOK;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int col = 8 * n + (2 * q) % P;
+                if constexpr (XB) {
+                    part[n][0] = fmaf(d0, c[n][0], part[n][0]);
+                    part[n][1] = fmaf(d0, c[n][1], part[n][1]);
+                    part[n][2] = fmaf(d1, c[n][2], part[n][2]);
+                    part[n][3] = fmaf(d1, c[n][3], part[n][3]);
+                    if constexpr (TYPE == GX_Q4_1) {
+                        const float2 sx = *reinterpret_cast<const float2 *>(sum + col);
+                        const float m0 = half_value(u.m[set], 0), m1 = half_value(u.m[set], 1);
+                        part[n][0] = fmaf(m0, sx.x, part[n][0]);
+                        part[n][1] = fmaf(m0, sx.y, part[n][1]);
+                        part[n][2] = fmaf(m1, sx.x, part[n][2]);
+                        part[n][3] = fmaf(m1, sx.y, part[n][3]);
+                    }
+                } else {
+                    part[n][0] = fmaf(d0, c[n][0] + c[n][1], part[n][0]);
+                    part[n][1] = fmaf(d1, c[n][2] + c[n][3], part[n][1]);
+                    if constexpr (TYPE == GX_Q4_1) {
+                        part[n][0] = fmaf(half_value(u.m[set], 0), sum[col / 2], part[n][0]);
+                        part[n][1] = fmaf(half_value(u.m[set], 1), sum[col / 2], part[n][1]);
+                    }
+                }
+            }
+        }
+        const float *inv = reinterpret_cast<const float *>(x + INV);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
             const int col = 8 * n + (2 * q) % P;
             if constexpr (XB) {
-                part[n][0] = fmaf(d0, c[n][0], part[n][0]);
-                part[n][1] = fmaf(d0, c[n][1], part[n][1]);
-                part[n][2] = fmaf(d1, c[n][2], part[n][2]);
-                part[n][3] = fmaf(d1, c[n][3], part[n][3]);
-                if constexpr (TYPE == GX_Q4_1) {
-                    const float2 sx = *reinterpret_cast<const float2 *>(sum + grp * L::TOK + col);
-                    const float m0 = half_value(u.m[set], 0), m1 = half_value(u.m[set], 1);
-                    part[n][0] = fmaf(m0, sx.x, part[n][0]);
-                    part[n][1] = fmaf(m0, sx.y, part[n][1]);
-                    part[n][2] = fmaf(m1, sx.x, part[n][2]);
-                    part[n][3] = fmaf(m1, sx.y, part[n][3]);
-                }
+                const float2 iv = *reinterpret_cast<const float2 *>(inv + col);
+                acc[n][0] = fmaf(part[n][0], iv.x, acc[n][0]);
+                acc[n][1] = fmaf(part[n][1], iv.y, acc[n][1]);
+                acc[n][2] = fmaf(part[n][2], iv.x, acc[n][2]);
+                acc[n][3] = fmaf(part[n][3], iv.y, acc[n][3]);
             } else {
-                part[n][0] = fmaf(d0, c[n][0] + c[n][1], part[n][0]);
-                part[n][1] = fmaf(d1, c[n][2] + c[n][3], part[n][1]);
-                if constexpr (TYPE == GX_Q4_1) {
-                    const float sx = sum[grp * L::TOK + col / 2];
-                    part[n][0] = fmaf(half_value(u.m[set], 0), sx, part[n][0]);
-                    part[n][1] = fmaf(half_value(u.m[set], 1), sx, part[n][1]);
-                }
+                acc[n][0] = fmaf(part[n][0], inv[col / 2], acc[n][0]);
+                acc[n][1] = fmaf(part[n][1], inv[col / 2], acc[n][1]);
             }
         }
     }
+    __device__ __forceinline__ void put(float *dst, int lane) {
+        const int g = lane >> 2, q = lane & 3;
+        if constexpr (GPC > 1) {  // P == 4: lanes q and q + 2 hold two groups of the same tokens
 #pragma unroll
-    for (int n = 0; n < L::NT; ++n) {
-        const int col = 8 * n + (2 * q) % P;
-        if constexpr (XB) {
-            const float2 iv = *reinterpret_cast<const float2 *>(inv + ul * L::TOK + col);
-            acc[n][0] = fmaf(part[n][0], iv.x, acc[n][0]);
-            acc[n][1] = fmaf(part[n][1], iv.y, acc[n][1]);
-            acc[n][2] = fmaf(part[n][2], iv.x, acc[n][2]);
-            acc[n][3] = fmaf(part[n][3], iv.y, acc[n][3]);
-        } else {
-            const float iv = inv[ul * L::TOK + col / 2];
-            acc[n][0] = fmaf(part[n][0], iv, acc[n][0]);
-            acc[n][1] = fmaf(part[n][1], iv, acc[n][1]);
+            for (int k = 0; k < NA; ++k) acc[0][k] += __shfl_xor_sync(0xffffffffu, acc[0][k], 2);
+            if (q >= P / 2) return;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int col = 8 * n + 2 * q;
+            if constexpr (XB) {
+                dst[col * 16 + g] = acc[n][0];
+                dst[(col + 1) * 16 + g] = acc[n][1];
+                dst[col * 16 + g + 8] = acc[n][2];
+                dst[(col + 1) * 16 + g + 8] = acc[n][3];
+            } else {
+                dst[col / 2 * 16 + g] = acc[n][0];
+                dst[col / 2 * 16 + g + 8] = acc[n][1];
+            }
         }
     }
-}
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < NA; ++k) acc[n][k] = 0.f;
+    }
+};
 
 constexpr int kMaxSmem = 227 * 1024;  // of a CTA
 
@@ -320,7 +500,7 @@ struct GemvPlan {
     int WK;          // warps of a CTA that split its columns; W / WK row tiles at a time
     int t0, nt;      // tokens of this launch
     int vec;         // activations can be read 16 bytes at a time
-    int sum_off, inv_off, red_off;
+    int red_off;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -343,15 +523,10 @@ __device__ __forceinline__ float ld_cluster(const float *p, uint32_t rank) {
 // a row tile in turn, with kDepth units in flight in registers across row tiles, and add their parts
 // in shared memory. With S > 1 each cluster has one pass of row tiles, its CTAs take S ranges of the
 // units, and rank 0 adds their parts.
-constexpr int gemv_ctas(int P, int W) { return W == 16 ? 1 : P <= 8 ? 3 : 2; }  // resident on an SM
-
-template <uint32_t TYPE, bool XB, int P, int W>
-__global__ void __launch_bounds__(W * 32, gemv_ctas(P, W)) q4_gemv_kernel(Q4Args a, GemvPlan p) {
-    using L = Few<XB, P>;
-    constexpr int kDepth = TYPE == GX_Q4_0 || P < 8 ? 3 : 2, NT = L::NT, NA = L::NA, RED = kTileRows * L::TOK;
+template <uint32_t TYPE, class M, int W>
+__global__ void __launch_bounds__(W * 32, M::CTAS(W)) q4_gemv_kernel(Q4Args a, GemvPlan p) {
+    constexpr int kDepth = M::kDepth, RED = kTileRows * M::TOK;
     extern __shared__ __align__(16) uint8_t smem[];
-    uint8_t *frag = smem;
-    float *sum = reinterpret_cast<float *>(smem + p.sum_off), *inv = reinterpret_cast<float *>(smem + p.inv_off);
     float *red = reinterpret_cast<float *>(smem + p.red_off);  // [2][W][RED]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = p.S > 1 ? (int)cluster_rank() : 0;
@@ -363,14 +538,13 @@ __global__ void __launch_bounds__(W * 32, gemv_ctas(P, W)) q4_gemv_kernel(Q4Args
     // cursor of the loads: the next unit of this warp, units left of its row tile, row tiles left
     constexpr int UB = unit_bytes(TYPE);
     const bool idle = wk >= nu;  // more warps than units: this one only takes part in the sums
-    const int per = idle ? 0 : (nu - wk + p.WK - 1) / p.WK, scale_at = P == 2 ? lane * 4 : P == 4 ? (lane >> 1) * 4 + (lane >> 2) * 8 : (lane >> 2) * 16,
-              scale = 1024 + scale_at - lane * 16;
+    const int per = idle ? 0 : (nu - wk + p.WK - 1) / p.WK, scale = 1024 + M::scale_offset(lane) - lane * 16;
     const uint8_t *lp = a.w + ((size_t)rt0 * p.KT + u0 + wk) * UB + lane * 16;
     int lleft = per, ltiles = rt0 < p.RT && !idle ? (p.RT - rt0 + step - 1) / step : 0;
     const int unit_step = p.WK * UB;
     const long long tile_step = (long long)step * p.KT * UB - (long long)(per - 1) * unit_step;
-    Unit<TYPE, L::SETS> buf[kDepth];
-    auto fetch = [&](Unit<TYPE, L::SETS> &u) {
+    Unit<TYPE, M::SETS> buf[kDepth];
+    auto fetch = [&](Unit<TYPE, M::SETS> &u) {
         if (ltiles > 0) {
             load_unit(u, lp, scale);
             if (--lleft == 0) {
@@ -386,56 +560,17 @@ __global__ void __launch_bounds__(W * 32, gemv_ctas(P, W)) q4_gemv_kernel(Q4Args
     for (int k = 0; k < kDepth; ++k) fetch(buf[k]);
     pdl_launch_dependents();
     pdl_wait();  // the weights never change; the activations may come from the kernel before
-    if constexpr (L::GPC > 1)
-        for (int i = tid; i < nu * 4; i += W * 32)
-            *reinterpret_cast<uint4 *>(frag + (i >> 2) * L::FRAG_BYTES + 4 * L::GROUP_BYTES + (i & 3) * 16) = make_uint4(0u, 0u, 0u, 0u);
-    stage_x<TYPE, XB, P>(a, p.t0, p.nt, u0, nu, frag, sum, inv, p.vec != 0, tid, W * 32);
+    M::stage(a, p.t0, p.nt, u0, nu, smem, p.vec != 0, tid, W * 32);
     __syncthreads();
 
-    // Columns without a token read the first one's fragment where nothing is stored of their sums, and
-    // the zeros where a column's sums meet those of others.
-    int at[L::ATS];
-    const int g = lane >> 2, live = XB ? p.nt : 2 * p.nt;
-#pragma unroll
-    for (int k = 0; k < L::ATS; ++k) {
-        if constexpr (L::GPC > 1)
-            at[k] = (g / P == k % L::GPC && g % P < live ? k * L::GROUP_BYTES + g % P * 64 : 4 * L::GROUP_BYTES) + (lane & 3) * 16;
-        else
-            at[k] = (8 * k + g < live ? 8 * k + g : 0) * 64 + (lane & 3) * 16;
-    }
-    float acc[NT][NA];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int k = 0; k < NA; ++k) acc[n][k] = 0.f;
-    int rt = rt0, ul = wk, parity = 0;
-    auto put = [&](float *dst) {  // the warp's part as [token][16 rows]
-        const int q = lane & 3;
-        if constexpr (L::GPC > 1) {  // the lanes of a row add up their groups
-#pragma unroll
-            for (int k = 0; k < NA; ++k) {
-                if (P == 2) acc[0][k] += __shfl_xor_sync(0xffffffffu, acc[0][k], 1);
-                acc[0][k] += __shfl_xor_sync(0xffffffffu, acc[0][k], 2);
-            }
-            if (q >= P / 2) return;
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int col = 8 * n + 2 * q;
-            if constexpr (XB) {
-                dst[col * 16 + g] = acc[n][0];
-                dst[(col + 1) * 16 + g] = acc[n][1];
-                dst[col * 16 + g + 8] = acc[n][2];
-                dst[(col + 1) * 16 + g + 8] = acc[n][3];
-            } else {
-                dst[col / 2 * 16 + g] = acc[n][0];
-                dst[col / 2 * 16 + g + 8] = acc[n][1];
-            }
-        }
-    };
+    M m;
+    m.init(lane, p.nt);
+    m.clear();
+    int rt = rt0, left = per, parity = 0;
+    const uint8_t *x = smem + wk * M::BYTES;  // the activations of the next unit
     auto finish = [&]() {  // the row tile rt is complete in this warp
         float *mine = red + (size_t)(parity * W + warp) * RED;
-        put(mine);
+        m.put(mine, lane);
         if (p.WK > 1) {
             asm volatile("bar.sync %0, %1;" ::"r"(1 + wg), "r"(32 * p.WK) : "memory");
         } else {
@@ -452,27 +587,23 @@ __global__ void __launch_bounds__(W * 32, gemv_ctas(P, W)) q4_gemv_kernel(Q4Args
         }
         if (p.WK == 1) __syncwarp();
         parity ^= 1;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int k = 0; k < NA; ++k) acc[n][k] = 0.f;
+        rt += step;
+        m.clear();
     };
+    if (idle) {
+        while (rt < p.RT) finish();
+    }
     while (rt < p.RT) {
-        if (idle) {
-            finish();
-            rt += step;
-            continue;
-        }
 #pragma unroll
         for (int k = 0; k < kDepth; ++k) {
             if (rt >= p.RT) break;
-            unit_product<TYPE, XB, P>(buf[k], ul, frag, sum, inv, lane, at, acc);
+            m.unit(buf[k], x, lane);
             fetch(buf[k]);
-            ul += p.WK;
-            if (ul >= nu) {
+            x += p.WK * M::BYTES;
+            if (--left == 0) {
                 finish();
-                ul = wk;
-                rt += step;
+                left = per;
+                x = smem + wk * M::BYTES;
             }
         }
     }
@@ -491,9 +622,9 @@ __global__ void __launch_bounds__(W * 32, gemv_ctas(P, W)) q4_gemv_kernel(Q4Args
     }
 }
 
-template <uint32_t TYPE, bool XB, int P, int W>
+template <uint32_t TYPE, class M, int W>
 cudaError_t launch_gemv_w(const Q4Args &a, GemvPlan p, int smem, int grid, cudaStream_t s) {
-    auto *k = q4_gemv_kernel<TYPE, XB, P, W>;
+    auto *k = q4_gemv_kernel<TYPE, M, W>;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -512,9 +643,8 @@ cudaError_t launch_gemv_w(const Q4Args &a, GemvPlan p, int smem, int grid, cudaS
     return cudaLaunchKernelEx(&cfg, k, a, p);
 }
 
-template <uint32_t TYPE, bool XB, int P>
+template <uint32_t TYPE, bool XB, class M>
 cudaError_t launch_gemv(const Q4Args &a, int t0, int nt, int sm_count, cudaStream_t s) {
-    using L = Few<XB, P>;
     GemvPlan p{};
     p.RT = (a.rows + kTileRows - 1) / kTileRows;
     p.KT = (a.cols + kUnitCols - 1) / kUnitCols;
@@ -530,20 +660,17 @@ cudaError_t launch_gemv(const Q4Args &a, int t0, int nt, int sm_count, cudaStrea
     while (p.WK < 8 && (long long)p.RT * p.WK < want && p.KT >= 4 * p.WK) p.WK *= 2;
     while (p.S < 8 && (long long)p.RT * p.WK * p.S < want && p.KT >= 4 * p.WK * p.S) p.S *= 2;
     // the activations of a CTA's units have to fit
-    while (p.S < 8 && (long long)((p.KT + p.S - 1) / p.S) * L::UNIT_BYTES > 100 * 1024) p.S *= 2;
-    const int nu = (p.KT + p.S - 1) / p.S;
-    const int xbytes = nu * L::UNIT_BYTES;
+    while (p.S < 8 && (long long)((p.KT + p.S - 1) / p.S) * M::BYTES > 100 * 1024) p.S *= 2;
+    const int xbytes = (p.KT + p.S - 1) / p.S * M::BYTES;
     const bool wide = xbytes > 56 * 1024;  // few CTAs fit an SM: 16 warps each instead of 8
     const int W = wide ? 16 : 8;
-    p.sum_off = nu * L::FRAG_BYTES;
-    p.inv_off = p.sum_off + nu * 4 * L::TOK * 4;
-    p.red_off = (p.inv_off + nu * L::TOK * 4 + 15) / 16 * 16;
-    const int smem = p.red_off + 2 * W * kTileRows * L::TOK * 4;
+    p.red_off = xbytes;
+    const int smem = p.red_off + 2 * W * kTileRows * M::TOK * 4;
     if (smem > kMaxSmem) return cudaErrorInvalidValue;
     const int groups = W / p.WK, need = (p.RT + groups - 1) / groups;
-    const int resident = sm_count * gemv_ctas(P, W);
+    const int resident = sm_count * M::CTAS(W);
     const int grid = p.S > 1 ? need * p.S : need < resident ? need : resident;
-    return wide ? launch_gemv_w<TYPE, XB, P, 16>(a, p, smem, grid, s) : launch_gemv_w<TYPE, XB, P, 8>(a, p, smem, grid, s);
+    return wide ? launch_gemv_w<TYPE, M, 16>(a, p, smem, grid, s) : launch_gemv_w<TYPE, M, 8>(a, p, smem, grid, s);
 }
 
 // ---- more tokens: a tiled product on mma.sync ---------------------------------------------------
@@ -867,13 +994,14 @@ cudaError_t launch_tokens(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream
     if (a.n_tok > 2 * T1) return launch_gemm<TYPE, XB>(a, ws, sm_count, s);
     // 16 columns where their activations fit the cluster's shared memory, else 8 at a time
     const int KT = (a.cols + kUnitCols - 1) / kUnitCols;
-    const int most = ((KT + 7) / 8) * Few<XB, 16>::UNIT_BYTES <= 160 * 1024 ? 2 * T1 : T1;
+    const int most = ((KT + 7) / 8) * Halves<TYPE, XB, 16>::BYTES <= 160 * 1024 ? 2 * T1 : T1;
     for (int t0 = 0; t0 < a.n_tok; t0 += most) {
         const int nt = a.n_tok - t0 < most ? a.n_tok - t0 : most, cols = XB ? nt : 2 * nt;
-        const cudaError_t e = cols <= 2   ? launch_gemv<TYPE, XB, 2>(a, t0, nt, sm_count, s)
-                              : cols <= 4 ? launch_gemv<TYPE, XB, 4>(a, t0, nt, sm_count, s)
-                              : cols <= 8 ? launch_gemv<TYPE, XB, 8>(a, t0, nt, sm_count, s)
-                                          : launch_gemv<TYPE, XB, 16>(a, t0, nt, sm_count, s);
+        const cudaError_t e = nt == 1     ? launch_gemv<TYPE, XB, Ints<TYPE, XB, 1>>(a, t0, nt, sm_count, s)
+                              : nt == 2   ? launch_gemv<TYPE, XB, Ints<TYPE, XB, 2>>(a, t0, nt, sm_count, s)
+                              : cols <= 4 ? launch_gemv<TYPE, XB, Halves<TYPE, XB, 4>>(a, t0, nt, sm_count, s)
+                              : cols <= 8 ? launch_gemv<TYPE, XB, Halves<TYPE, XB, 8>>(a, t0, nt, sm_count, s)
+                                          : launch_gemv<TYPE, XB, Halves<TYPE, XB, 16>>(a, t0, nt, sm_count, s);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
