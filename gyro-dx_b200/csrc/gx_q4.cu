@@ -207,8 +207,8 @@ __device__ __forceinline__ T quad_sum(T v) {
 // accumulator, the fragment of each being zero in the columns of the other.
 template <uint32_t TYPE, bool XB, int T>
 struct Ints {
-    static constexpr int TOK = T, NA = 2, SETS = T == 1 ? 2 : 4, kDepth = 3;  // units in flight
-    static constexpr int CTAS(int W) { return W == 16 ? 1 : 3; }             // resident on an SM
+    static constexpr int TOK = T, NA = 2, SETS = T == 1 ? 2 : 4, kDepth = T == 1 ? 5 : 4;  // units in flight
+    static constexpr int CTAS(int W) { return W == 16 ? 1 : 2; }                       // resident on an SM
     // [4 groups][T tokens][4 digits][4 q] 8 B: the digit of columns (0 2 4 6) and (1 3 5 7) of 8 q ..
     static constexpr int GROUP = T * 128, ZERO = 4 * GROUP;       // T == 1: 32 B of zeros
     static constexpr int INIT = ZERO + (T == 1 ? 32 : 0);         // Q4_0: [group][token][digit pair] int4 accumulators
