@@ -1,15 +1,16 @@
 // gx_logprobs.cu — log probabilities of given tokens over rows of logits, with the entropy, the
-// given token's rank and the likeliest alternatives. With m = max x, t = scale (x - m), s = sum e^t:
+// given token's rank and the likeliest alternatives. With t = scale (x - ref), s = sum e^t:
 //
 //   logprob = t_token - ln s,   entropy = ln s - (sum e^t t) / s,
 //   rank = 1 + #{x > x_token},  the n_top largest x, equal ones by rising id.
 //
-// Bound by reading the logits once. A cluster of CTAs takes a row, each CTA a slice that it keeps in
-// shared memory: bulk copies bring it in chunks, and each chunk is scanned for its maximum as it
-// arrives. With the maximum known a second pass over shared memory sums e^t and e^t t, counts the
-// logits above the given one and picks candidates for the top: each thread's own maximum is known
-// too, and gives a floor that few logits pass. The CTAs' results meet
-// in the first one's shared memory. Nothing depends on the order in which threads run.
+// Bound by reading the logits once, 10 instructions a logit. A cluster of CTAs takes a row, each CTA a
+// slice that its threads stream through registers, four 16-byte words ahead. The reference ref need not be
+// the maximum, only near it: it is that of the slice's first words, and a thread that meets a logit more
+// than 2^8 times as likely moves on to a new one. Each lane's maximum in the first words also gives a
+// floor for the top, so that few logits are candidates; those enter the warp's sorted list, a key in a
+// lane. The lists and sums meet in shared memory, then in that of the cluster's first CTA. Nothing
+// depends on the order in which threads run.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,7 +29,7 @@ namespace {
 
 constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
-constexpr int kLpChunks = 4;      // bulk copies of a slice
+constexpr int kLpAhead = 4;       // 16-byte words of a thread in flight
 constexpr int kLpMaxCluster = 16;
 
 typedef unsigned long long u64;
@@ -63,7 +64,7 @@ __device__ __forceinline__ void warp_insert(u64 &list, u64 key, int lane) {
 
 // What a CTA hands to the first one of its cluster.
 struct Part {
-    float m, s, et;
+    float ref, s, et;
     unsigned above;
     u64 top[kMaxTop];
 };
@@ -79,6 +80,9 @@ struct Vec<float> {
         v[2] = __uint_as_float(q.z);
         v[3] = __uint_as_float(q.w);
     }
+    static __device__ __forceinline__ float pick(const uint4 &q, int k) {
+        return __uint_as_float(k < 2 ? (k < 1 ? q.x : q.y) : (k < 3 ? q.z : q.w));
+    }
 };
 template <>
 struct Vec<__nv_bfloat16> {
@@ -90,6 +94,10 @@ struct Vec<__nv_bfloat16> {
             v[2 * j] = __uint_as_float(w[j] << 16);
             v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
         }
+    }
+    static __device__ __forceinline__ float pick(const uint4 &q, int k) {
+        const uint32_t w = k < 4 ? (k < 2 ? q.x : q.y) : (k < 6 ? q.z : q.w);
+        return __uint_as_float((k & 1) ? w & 0xffff0000u : w << 16);
     }
 };
 __device__ __forceinline__ float to_f(float x) { return x; }
@@ -116,16 +124,29 @@ __device__ __forceinline__ void lp_cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
-// The n_top best of n keys in shared memory (distinct, 0 for none), in falling order, into out: a key's
-// place is the number of better ones.
-__device__ __forceinline__ void rank_keys(const u64 *keys, int n, int n_top, u64 *out, int tid) {
-    for (int i = tid; i < n; i += kLpThreads) {
-        const u64 k = keys[i];
-        if (k == 0) continue;
-        int place = 0;
-        for (int j = 0; j < n; ++j) place += keys[j] > k;
-        if (place < n_top) out[place] = k;
+// The best 32 keys of two falling lists, a key in a lane, as a falling list: one against the other
+// reversed leaves the best 32 in a bitonic order, which five exchanges sort.
+__device__ __forceinline__ u64 merge_lists(u64 a, u64 b, int lane) {
+    b = __shfl_sync(0xffffffffu, b, 31 - lane);
+    u64 k = a > b ? a : b;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        const u64 o = __shfl_xor_sync(0xffffffffu, k, d);
+        k = ((lane & d) == 0) == (k > o) ? k : o;
     }
+    return k;
+}
+// n lists (a power of two, at most 16) in shared memory, [n][32]: the merged list in warp 0. All threads.
+__device__ __forceinline__ u64 merge_all(u64 (*lists)[32], int n, int warp, int lane) {
+    u64 k = warp < n ? lists[warp][lane] : 0;
+    for (int h = n / 2; h > 0; h /= 2) {
+        if (warp < h) {
+            k = merge_lists(k, lists[warp + h][lane], lane);
+            lists[warp][lane] = k;
+        }
+        __syncthreads();
+    }
+    return k;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -134,29 +155,13 @@ __device__ __forceinline__ float ex2(float x) {
     return r;
 }
 
-// Running maximum of a thread over vectors, NaN included.
-template <typename T>
-struct RunMax;
-template <>
-struct RunMax<float> {
-    float m;
-    __device__ __forceinline__ RunMax() { m = -CUDART_INF_F; }
-    __device__ __forceinline__ void add(uint4 q) {
-        m = max_nan(max_nan(m, max_nan(__uint_as_float(q.x), __uint_as_float(q.y))),
-                    max_nan(__uint_as_float(q.z), __uint_as_float(q.w)));
-    }
-    __device__ __forceinline__ float get() const { return m; }
-};
 __device__ __forceinline__ __nv_bfloat162 as_bf2(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162 *>(&w); }
-template <>
-struct RunMax<__nv_bfloat16> {
-    __nv_bfloat162 m;
-    __device__ __forceinline__ RunMax() { m = __floats2bfloat162_rn(-CUDART_INF_F, -CUDART_INF_F); }
-    __device__ __forceinline__ void add(uint4 q) {
-        m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(as_bf2(q.x), as_bf2(q.y)), __hmax2_nan(as_bf2(q.z), as_bf2(q.w))));
-    }
-    __device__ __forceinline__ float get() const { return max_nan(__low2float(m), __high2float(m)); }
-};
+// What is read past a slice: masked tokens.
+template <typename T>
+__device__ __forceinline__ uint4 masked_word() {
+    const uint32_t w = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+    return make_uint4(w, w, w, w);
+}
 // The largest of a vector without NaN.
 template <typename T>
 __device__ __forceinline__ float vec_max(uint4 q);
@@ -178,16 +183,22 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 }
 __device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float((u >> 31) ? u & 0x7fffffffu : ~u); }
 
+// Sums relative to one reference, moved to another: a part with no weight there (masked tokens, or 2^-126
+// of the whole) counts nothing.
+__device__ __forceinline__ void move_sums(float &s, float &et, float from, float to, float c2) {
+    const float d = from == to ? 0.f : fmaxf((from - to) * c2, -200.f), w = ex2(d);
+    et = w * fmaf(s, d, et);
+    s *= w;
+}
+
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(LogprobsArgs a, int C, int slice) {
+__global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(LogprobsArgs a, int C, int slice) {
     constexpr int N = Vec<T>::N, SZ = (int)sizeof(T);
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ __align__(8) uint64_t bars[kLpChunks];
     __shared__ float redf[4][kLpWarps];
-    __shared__ unsigned redu[kLpWarps], counts[kLpWarps];
-    __shared__ u64 lists[kLpWarps * kMaxTop];
-    __shared__ u64 best[kMaxTop];
+    __shared__ unsigned redu[kLpWarps];
+    __shared__ u64 lists[kLpMaxCluster][32];  // of the warps, then of the cluster's CTAs
     __shared__ Part parts[kLpMaxCluster];
+    static_assert(kLpMaxCluster >= kLpWarps && kMaxTop == 32, "a list is a warp wide");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = C > 1 ? (int)lp_cluster_rank() : 0;
     const size_t r = blockIdx.x / C;
@@ -198,25 +209,16 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(LogprobsArgs a, in
     const T *src = row + i0;
     const int head = min(n, (int)((16 - ((uintptr_t)src & 15)) & 15) / SZ);
     const int words = (n - head) / N, tail0 = head + words * N;
-    uint4 *buf = reinterpret_cast<uint4 *>(smem);
-    const int per = (words + kLpChunks - 1) / kLpChunks;
-    if (tid == 0) {
-#pragma unroll
-        for (int c = 0; c < kLpChunks; ++c) mbar_init(&bars[c], 1);
-        fence_barrier_init();
-        pdl_wait();
-#pragma unroll
-        for (int c = 0; c < kLpChunks; ++c) {
-            const int w0 = c * per, w1 = min(words, w0 + per);
-            if (w0 >= w1) continue;
-            mbar_expect_tx(&bars[c], (uint32_t)(w1 - w0) * 16u);
-            bulk_g2s(buf + w0, reinterpret_cast<const uint4 *>(src + head) + w0, (uint32_t)(w1 - w0) * 16u, &bars[c]);
-        }
-    }
-    __syncthreads();
+    const uint4 *word = reinterpret_cast<const uint4 *>(src + head);
     if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA has started
     pdl_launch_dependents();
     pdl_wait();
+    uint4 next[kLpAhead];
+#pragma unroll
+    for (int j = 0; j < kLpAhead; ++j) {
+        const int w = j * kLpThreads + tid;
+        next[j] = w < words ? __ldcs(word + w) : masked_word<T>();
+    }
     // the slice's ends, one logit a thread (fewer than 2 N of them)
     const int ends = n - words * N;
     const int end_i = tid < head ? tid : tail0 + tid - head;
@@ -225,64 +227,51 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(LogprobsArgs a, in
     const uint32_t tok = a.tokens ? a.tokens[r] : GX_NO_TOKEN;
     const bool has = tok < (uint32_t)V;
     const float xt = has ? to_f(row[tok]) : CUDART_INF_F;
+    const bool xt_nan = isnan(xt);
+    const float mark = xt_nan ? CUDART_INF_F : xt;  // logits above this one are counted (above a NaN: all of them)
 
-    // pass 1, chunk by chunk: the thread's maximum
-    RunMax<T> run;
-    bool ok = true;
+    // the reference, and the floor of the candidates, from the first words
+    float own = vec_max<T>(next[0]);
 #pragma unroll
-    for (int c = 0; c < kLpChunks; ++c) {
-        const int w0 = c * per, w1 = min(words, w0 + per);
-        if (w0 >= w1) continue;
-        ok = ok && mbar_wait(&bars[c], 0u, a.err);
-        if (!ok) continue;
-#pragma unroll 4
-        for (int w = w0 + tid; w < w1; w += kLpThreads) run.add(buf[w]);
-    }
-    ok = __syncthreads_and(ok);
-    if (!ok && tid == 0) {  // an expired wait is reported; no copy may outlive the CTA
-        for (int c = 0; c < kLpChunks; ++c)
-            if (c * per < words) mbar_wait(&bars[c], 0u, nullptr);
-    }
-    const float own = max_nan(run.get(), end_x);
-    float m = own;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) redf[0][warp] = m;
+    for (int j = 1; j < kLpAhead; ++j) own = fmaxf(own, vec_max<T>(next[j]));
+    if (isnan(own)) own = -CUDART_INF_F;
+    uint32_t o = ordered(own), t = __reduce_max_sync(0xffffffffu, o);
+    if (lane == 0) redf[0][warp] = unordered(t);
     if (TOP) {
         // The k-th largest of the lanes' maxima, k = n_top / 8 rounded up: each maximum is a logit of its
         // own, so the least of the 8 warps' values is a floor that at least n_top logits reach.
-        uint32_t o = isnan(own) ? ordered(-CUDART_INF_F) : ordered(own), t = 0;
-        for (int k = (a.n_top + kLpWarps - 1) / kLpWarps; k > 0; --k) {
+        for (int k = (a.n_top + kLpWarps - 1) / kLpWarps; k > 1; --k) {
+            if (lane == __ffs(__ballot_sync(0xffffffffu, o == t)) - 1) o = 0;
             t = __reduce_max_sync(0xffffffffu, o);
-            const unsigned who = __ballot_sync(0xffffffffu, o == t);
-            if (lane == __ffs(who) - 1) o = 0;
         }
         if (lane == 0) redf[1][warp] = unordered(t);
     }
     __syncthreads();
-    m = redf[0][0];
-    float floor = TOP ? redf[1][0] : 0.f;
+    float ref = redf[0][0], floor = TOP ? redf[1][0] : 0.f;
 #pragma unroll
     for (int w = 1; w < kLpWarps; ++w) {
-        m = max_nan(m, redf[0][w]);
+        ref = fmaxf(ref, redf[0][w]);
         if (TOP) floor = fminf(floor, redf[1][w]);
     }
-    const bool has_nan = isnan(m);
+    ref = fmaxf(ref, -3.402823466e38f);  // a finite one where the first words are masked
 
-    // pass 2
-    const bool flat = m == -CUDART_INF_F;  // every token masked: a row of equal logits
-    const float c2 = a.scale * CUDART_L2E_F;
-    float s = 0.f, et = 0.f;
+    const float c2 = a.scale * CUDART_L2E_F, reach = 8.f / c2;  // t below in units of ln 2
+    float s = 0.f, et = 0.f, limit = ref + reach;
     unsigned above = 0;
     u64 list = 0, worst = 0;   // the warp's best keys by lane, its n_top-th
-    auto sums = [&](float x) {
-        const float t = flat ? 0.f : fmaxf((x - m) * c2, -200.f);  // e^t is 0 there, and 0 * t stays 0
-        const float e = ex2(t);
+    auto sum = [&](float x) {
+        const float d = max_nan((x - ref) * c2, -200.f);  // e^t is 0 there, and 0 * t stays 0; a NaN shows in s
+        const float e = ex2(d);
         s += e;
-        et = fmaf(e, t, et);
+        et = fmaf(e, d, et);
     };
-    // logits above the given one; NaN lies below all others
-    auto count = [&](float x) { above += isnan(xt) ? !isnan(x) : x > xt; };
+    auto reach_for = [&](float x) {  // a new reference for a logit far above
+        if (x > limit) {
+            move_sums(s, et, ref, x, c2);
+            ref = x;
+            limit = ref + reach;
+        }
+    };
     auto offer = [&](u64 key) {  // one key of each lane, 0 for none
         unsigned who = __ballot_sync(0xffffffffu, key > worst);
         while (who) {
@@ -293,89 +282,132 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(LogprobsArgs a, in
             who = (who & (who - 1)) & __ballot_sync(0xffffffffu, key > worst);
         }
     };
-    if (has_end) {
-        sums(end_x);
-        count(end_x);
-    }
-    if (TOP) offer(has_end ? logit_key(end_x, (uint32_t)(i0 + end_i)) : 0);
-    float least = worst ? key_value(worst) : -CUDART_INF_F;  // value of the n_top-th key
-    if (isnan(least)) least = -CUDART_INF_F;
-    for (int w0 = warp * 32; w0 < words; w0 += kLpThreads) {
-        const int w = w0 + lane;
-        const bool on = ok && w < words;
-        float v[N], top = -CUDART_INF_F;
-        if (on) {
-            const uint4 q = buf[w];
-            Vec<T>::get(q, v);
-            top = vec_max<T>(q);
+    // From step to step a warp meets its logits by rising id, so once its list is full only a larger value
+    // enters it: a logit above gate (before that, one at the floor too).
+    const float below = floor == 0.f ? -1.401298464e-45f : unordered(ordered(floor) - 1u);
+    float gate = floor == -CUDART_INF_F ? floor : below;
+    bool any_enters = TOP && floor == -CUDART_INF_F;  // masked tokens too, while the list is not full
+    for (int w0 = tid; w0 - tid < words; w0 += kLpAhead * kLpThreads) {
+        const bool inside = w0 - tid + 2 * kLpAhead * kLpThreads <= words;  // the next words all lie in the slice
+        unsigned hits = 0;  // words of the warp with candidates
 #pragma unroll
-            for (int k = 0; k < N; ++k) sums(v[k]);
-            if (top > xt || isnan(xt)) {
+        for (int j = 0; j < kLpAhead; ++j) {
+            const int ahead = w0 + (j + kLpAhead) * kLpThreads;
+            float v[N];
+            Vec<T>::get(next[j], v);
+            const float top = vec_max<T>(next[j]);
+            if (__any_sync(0xffffffffu, top > limit)) reach_for(top);
+            if (TOP) hits |= __any_sync(0xffffffffu, top > gate) ? 1u << j : 0u;
 #pragma unroll
-                for (int k = 0; k < N; ++k) count(v[k]);
+            for (int k = 0; k < N; ++k) sum(v[k]);
+            if (__any_sync(0xffffffffu, top > mark)) {
+#pragma unroll
+                for (int k = 0; k < N; ++k) above += v[k] > mark;
             }
+            if (inside) next[j] = __ldcs(word + ahead);
+            else next[j] = ahead < words ? __ldcs(word + ahead) : masked_word<T>();
         }
         if (TOP) {
-            const bool cand = on && (has_nan || (top >= floor && top >= least));
-            if (__any_sync(0xffffffffu, cand)) {
+            if (any_enters) hits = (1u << kLpAhead) - 1u;
+            while (hits) {  // rare: the words are read again, so that this code stands once
+                const int w = w0 + (__ffs(hits) - 1) * kLpThreads;
+                hits &= hits - 1;
+                const uint4 q = w < words ? word[w] : masked_word<T>();
+                float v[N];
+                Vec<T>::get(q, v);
+                unsigned mine = 0;  // the lane's candidates in the word
 #pragma unroll
-                for (int k = 0; k < N; ++k) offer(cand ? logit_key(v[k], (uint32_t)(i0 + head + w * N + k)) : 0);
-                least = worst ? key_value(worst) : -CUDART_INF_F;
-                if (isnan(least)) least = -CUDART_INF_F;
+                for (int k = 0; k < N; ++k) mine |= v[k] > gate || any_enters ? 1u << k : 0u;
+                if (w >= words) mine = 0;
+                while (__any_sync(0xffffffffu, mine != 0)) {  // one of each lane
+                    const int k = __ffs(mine) - 1;
+                    mine &= mine - 1;
+                    offer(k >= 0 ? logit_key(Vec<T>::pick(q, k), (uint32_t)(i0 + head + w * N + k)) : 0);
+                }
+                if (worst != 0) {
+                    gate = fmaxf(gate, key_value(worst));
+                    any_enters = false;
+                }
             }
         }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, o);
-        et += __shfl_xor_sync(0xffffffffu, et, o);
-        above += __shfl_xor_sync(0xffffffffu, above, o);
+    if (has_end) {
+        reach_for(end_x);
+        sum(end_x);
+        above += end_x > mark;
     }
+    if (TOP && warp == 0) offer(has_end ? logit_key(end_x, (uint32_t)(i0 + end_i)) : 0);
+    // A NaN lies below every number: where there is one (or +Inf, whose sums are NaN too), the counts and
+    // the list are made again the slow way.
+    if (xt_nan && tid == 0) above = (unsigned)n;
+    if (__syncthreads_or(isnan(s))) {
+        auto count = [&](float x) { above += xt_nan ? !isnan(x) : x > xt; };
+        above = 0;
+        list = worst = 0;
+        for (int w0 = warp * 32; w0 < words; w0 += kLpThreads) {
+            const bool on = w0 + lane < words;
+            const uint4 q = on ? word[w0 + lane] : masked_word<T>();
+#pragma unroll 1
+            for (int k = 0; k < N; ++k) {
+                const float x = Vec<T>::pick(q, k);
+                if (on) count(x);
+                if (TOP) offer(on ? logit_key(x, (uint32_t)(i0 + head + (w0 + lane) * N + k)) : 0);
+            }
+        }
+        if (has_end) count(end_x);
+        if (TOP && warp == 0) offer(has_end ? logit_key(end_x, (uint32_t)(i0 + end_i)) : 0);
+        s = CUDART_NAN_F;
+    }
+    {
+        float m = ref;
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+        move_sums(s, et, ref, m, c2);
+        ref = m;
+    }
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, k);
+        et += __shfl_xor_sync(0xffffffffu, et, k);
+    }
+    above = __reduce_add_sync(0xffffffffu, above);
     if (lane == 0) {
+        redf[0][warp] = ref;
         redf[2][warp] = s;
         redf[3][warp] = et;
         redu[warp] = above;
     }
-    if (TOP) {
-        const unsigned mine = __ballot_sync(0xffffffffu, lane < a.n_top && list != 0);
-        if (lane == 0) counts[warp] = __popc(mine);
-        if (tid < kMaxTop) best[tid] = 0;
-    }
+    if (TOP) lists[warp][lane] = list;
     __syncthreads();
-    if (TOP) {
-        int at = 0, all = 0;
-#pragma unroll
-        for (int w = 0; w < kLpWarps; ++w) {
-            at += w < warp ? (int)counts[w] : 0;
-            all += (int)counts[w];
-        }
-        if (lane < (int)counts[warp]) lists[at + lane] = list;
-        __syncthreads();
-        rank_keys(lists, all, a.n_top, best, tid);
-        __syncthreads();
-    }
+    u64 best = TOP ? merge_all(lists, kLpWarps, warp, lane) : 0;
     // into the first CTA's parts
     if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (warp == 0) {
-        float ss = 0.f, te = 0.f;
-        unsigned ab = 0;
+        // the warps' sums, one in a lane
+        float m = lane < kLpWarps ? redf[0][lane] : -CUDART_INF_F, ss = lane < kLpWarps ? redf[2][lane] : 0.f;
+        float te = lane < kLpWarps ? redf[3][lane] : 0.f, to = m;
+        unsigned ab = lane < kLpWarps ? redu[lane] : 0;
 #pragma unroll
-        for (int w = 0; w < kLpWarps; ++w) {
-            ss += redf[2][w];
-            te += redf[3][w];
-            ab += redu[w];
+        for (int k = 4; k > 0; k >>= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, k));
+        to = __shfl_sync(0xffffffffu, to, 0);
+        move_sums(ss, te, m, to, c2);
+#pragma unroll
+        for (int k = 4; k > 0; k >>= 1) {
+            ss += __shfl_xor_sync(0xffffffffu, ss, k);
+            te += __shfl_xor_sync(0xffffffffu, te, k);
         }
+        ab = __reduce_add_sync(0xffffffffu, ab);
         if (C > 1) {
             const uint32_t at = peer_addr(&parts[rank], 0u);
             if (lane == 0) {
-                st_peer(at + (uint32_t)offsetof(Part, m), __float_as_uint(m));
+                st_peer(at + (uint32_t)offsetof(Part, ref), __float_as_uint(to));
                 st_peer(at + (uint32_t)offsetof(Part, s), __float_as_uint(ss));
                 st_peer(at + (uint32_t)offsetof(Part, et), __float_as_uint(te));
                 st_peer(at + (uint32_t)offsetof(Part, above), ab);
             }
-            if (TOP && lane < a.n_top) st_peer(at + (uint32_t)offsetof(Part, top) + 8u * lane, best[lane]);
+            if (TOP) st_peer(at + (uint32_t)offsetof(Part, top) + 8u * lane, best);
         } else if (lane == 0) {
-            parts[0].m = m;
+            parts[0].ref = to;
             parts[0].s = ss;
             parts[0].et = te;
             parts[0].above = ab;
@@ -385,22 +417,23 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(LogprobsArgs a, in
     else __syncthreads();
     if (rank != 0) return;
     // the row: every thread computes the same totals
-    float M = parts[0].m;
-    for (int c = 1; c < C; ++c) M = max_nan(M, parts[c].m);
+    float M = parts[0].ref;
+    for (int c = 1; c < C; ++c) M = fmaxf(M, parts[c].ref);
     float S = 0.f, ET = 0.f;
     unsigned AB = 0;
     for (int c = 0; c < C; ++c) {
-        // a part's sums are relative to its own maximum; one of masked tokens only has no weight in a row
-        // that has others
-        const float pm = parts[c].m, t = pm == M ? 0.f : fmaxf((pm - M) * c2, -200.f), w = pm == M ? 1.f : ex2(t);
-        S = fmaf(parts[c].s, w, S);
-        ET = fmaf(w, fmaf(parts[c].s, t, parts[c].et), ET);
+        float ss = parts[c].s, te = parts[c].et;
+        move_sums(ss, te, parts[c].ref, M, c2);
+        S += ss;
+        ET += te;
         AB += parts[c].above;
     }
-    if (isnan(M) || M == CUDART_INF_F) S = CUDART_NAN_F;
+    const bool flat = S == 0.f;  // every token masked: a row of equal logits
+    if (flat) S = (float)V;
+    if (isinf(S)) S = CUDART_NAN_F;
     const float ls = logf(S);
     // halves, so that a difference beyond the f32 range that the scale brings back is not lost
-    auto lp = [&](float x) { return (M == -CUDART_INF_F ? 0.f : (0.5f * x - 0.5f * M) * (2.f * a.scale)) - ls; };
+    auto lp = [&](float x) { return (flat ? 0.f : (0.5f * x - 0.5f * M) * (2.f * a.scale)) - ls; };
     if (tid == 0) {
         const bool bad = a.tokens && !has && tok != GX_NO_TOKEN;
         if (bad) atomicExch(a.err, KERR_BOUNDS);
@@ -410,15 +443,13 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(LogprobsArgs a, in
     }
     if (TOP) {
         if (C > 1) {
-            u64 *all = reinterpret_cast<u64 *>(smem);  // the slice is no longer needed
-            for (int i = tid; i < C * a.n_top; i += kLpThreads) all[i] = parts[i / a.n_top].top[i % a.n_top];
+            for (int c = warp; c < C; c += kLpWarps) lists[c][lane] = parts[c].top[lane];
             __syncthreads();
-            rank_keys(all, C * a.n_top, a.n_top, best, tid);
-            __syncthreads();
+            best = merge_all(lists, C, warp, lane);
         }
         if (tid < a.n_top) {
-            if (a.top_ids) a.top_ids[r * a.n_top + tid] = key_id(best[tid]);
-            if (a.top_logprobs) a.top_logprobs[r * a.n_top + tid] = lp(key_value(best[tid]));
+            if (a.top_ids) a.top_ids[r * a.n_top + tid] = key_id(best);
+            if (a.top_logprobs) a.top_logprobs[r * a.n_top + tid] = lp(key_value(best));
         }
     }
 }
@@ -427,23 +458,21 @@ template <typename T, bool TOP>
 cudaError_t launch_lp(const LogprobsArgs &a, int sm_count, cudaStream_t s) {
     auto *k = logprobs_kernel<T, TOP>;
     constexpr int N = Vec<T>::N;
-    // Slices of at most 56 KB, so that three CTAs overlap on an SM; while the rows leave SMs idle, down to
-    // 8 KB.
+    // CTAs for every row until every SM has one, in slices of at least 16 KB: a CTA's floor, lists and
+    // merges cost as much as some 16 KB of logits (64 rows of 150001 in bf16: 35 us in 16 CTAs a row, 20 in
+    // 8, 12.7 in 4, 14.7 in 2)
     int C = 1;
-    auto bytes = [&] { return (((long long)a.n_vocab + C - 1) / C + N) * (long long)sizeof(T); };
-    while (C < kLpMaxCluster && bytes() > 56 * 1024) C *= 2;
-    while (C < kLpMaxCluster && (long long)a.n_rows * C < sm_count && bytes() > 8 * 1024) C *= 2;
+    auto bytes = [&] { return (long long)a.n_vocab / C * (long long)sizeof(T); };
+    while (C < kLpMaxCluster && (long long)a.n_rows * C < sm_count && bytes() >= 32 * 1024) C *= 2;
     if ((long long)a.n_rows * C > 0x7fffffffll) return cudaErrorInvalidValue;
     const int slice = ((a.n_vocab + C - 1) / C + N - 1) / N * N;
-    int smem = slice * (int)sizeof(T);
-    if (smem < C * kMaxTop * 8) smem = C * kMaxTop * 8;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess && C > 8) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
+    if (C > 8) {
+        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.n_rows * C));
     cfg.blockDim = dim3(kLpThreads);
-    cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
