@@ -4,9 +4,16 @@
 //   after:   v = y / sqrt(mean(y^2) + eps) * post   (or y itself)
 //            r = res_scale * res + block_scale * gate * v            gate: 1, sigmoid per token or per element
 //            res_out = r,  out = r / sqrt(mean(r^2) + eps) * next,   next_gate = next_gate_w . out
+//
+// Bound by reading and writing every row once. A group of G threads takes a row and holds it in
+// registers from the first read to the last write, 8 values in each of up to VPT vectors a thread; the
+// weights come through L1, which the streamed rows do not pass (16 CTAs and more on an SM share them).
+// Sums meet by shuffles, and across warps once in shared memory.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "../../include/gyro_moe.h"
 #include "gx_dense.cuh"
@@ -19,7 +26,8 @@ using namespace dense;
 
 namespace {
 
-constexpr int kNormThreads = 256;
+constexpr int kNormThreads = 256;    // of the long-row kernels
+constexpr int kNormRowMax = 16384;   // longest row held in registers: 512 threads of 4 vectors
 
 __device__ __forceinline__ void store_act(void *p, int bf16, size_t i, float v) {
     if (bf16) reinterpret_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
@@ -37,8 +45,11 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
     return t;
 }
 
-__global__ void __launch_bounds__(kNormThreads) norm_kernel(NormArgs a) {
+// ---- rows too long for registers: read again for each step -----------------------------------------
+__global__ void __launch_bounds__(kNormThreads) norm_long_kernel(NormArgs a) {
     __shared__ float red[kNormThreads / 32];
+    pdl_launch_dependents();
+    pdl_wait();
     const size_t t = blockIdx.x;
     float ss = 0.f;
     for (int i = threadIdx.x; i < a.E; i += kNormThreads) {
@@ -65,8 +76,10 @@ __device__ __forceinline__ float residual_value(const ResidualArgs &a, size_t t,
     return a.res_scale * load_act(a.res, a.res_bf16, t * a.ldr + i) + a.block_scale * tgate * v;
 }
 
-__global__ void __launch_bounds__(kNormThreads) norm_residual_kernel(ResidualArgs a) {
+__global__ void __launch_bounds__(kNormThreads) residual_long_kernel(ResidualArgs a) {
     __shared__ float red[kNormThreads / 32];
+    pdl_launch_dependents();
+    pdl_wait();
     const size_t t = blockIdx.x;
     float yscale = 1.f;
     if (a.post_norm) {
@@ -102,18 +115,253 @@ __global__ void __launch_bounds__(kNormThreads) norm_residual_kernel(ResidualArg
     }
 }
 
+// ---- rows held in registers --------------------------------------------------------------------
+// Thread l of a row's G has the elements (k G + l) 8 + j (VEC: 16-byte accesses; the width is a
+// multiple of 8 and every row aligned) or (8 k + j) G + l.
+template <int VPT, bool VEC>
+struct Row {
+    int G, l, E;
+    __device__ __forceinline__ int at(int k, int j) const { return VEC ? (k * G + l) * 8 + j : (8 * k + j) * G + l; }
+    __device__ __forceinline__ void load(const void *p, int bf16, size_t base, float (&v)[VPT][8]) const {
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
+            if constexpr (VEC) {
+                const int i = at(k, 0);
+                if (i >= E) continue;
+                if (bf16) {
+                    const uint4 q = __ldcs(reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(p) + base + i));
+                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        v[k][2 * j] = __uint_as_float(w[j] << 16);
+                        v[k][2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                    }
+                } else {
+                    const float4 *f = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + base + i);
+                    const float4 a = __ldcs(f), b = __ldcs(f + 1);
+                    v[k][0] = a.x; v[k][1] = a.y; v[k][2] = a.z; v[k][3] = a.w;
+                    v[k][4] = b.x; v[k][5] = b.y; v[k][6] = b.z; v[k][7] = b.w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (at(k, j) < E) v[k][j] = load_act(p, bf16, base + at(k, j));
+            }
+        }
+    }
+    __device__ __forceinline__ void store(void *p, int bf16, size_t base, const float (&v)[VPT][8]) const {
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            if constexpr (VEC) {
+                const int i = at(k, 0);
+                if (i >= E) continue;
+                if (bf16) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(v[k][2 * j], v[k][2 * j + 1]);
+                        w[j] = *reinterpret_cast<const uint32_t *>(&h);
+                    }
+                    *reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(p) + base + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+                    float4 *f = reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + base + i);
+                    f[0] = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
+                    f[1] = make_float4(v[k][4], v[k][5], v[k][6], v[k][7]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (at(k, j) < E) store_act(p, bf16, base + at(k, j), v[k][j]);
+            }
+        }
+    }
+    // weights of vector k (1 where there are none)
+    __device__ __forceinline__ void weights(const float *w, int k, float (&v)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 1.f;
+        if (!w) return;
+        if constexpr (VEC) {
+            const int i = at(k, 0);
+            if (i >= E) return;
+            const float4 a = __ldg(reinterpret_cast<const float4 *>(w + i)), b = __ldg(reinterpret_cast<const float4 *>(w + i) + 1);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (at(k, j) < E) v[j] = __ldg(w + at(k, j));
+        }
+    }
+};
+
+// Sum over a row's threads; red: a place of its own for each sum of a kernel.
+__device__ __forceinline__ float row_sum(float v, int G, float *red) {
+    v = warp_sum(v);
+    if (G == 32) return v;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float t = 0.f;
+    for (int w = 0; w < G / 32; ++w) t += red[w];
+    return t;
+}
+
+template <int VPT>
+__device__ __forceinline__ float square_sum(const float (&v)[VPT][8]) {
+    float ss[VPT];
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        ss[k] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss[k] = fmaf(v[k][j], v[k][j], ss[k]);
+    }
+#pragma unroll
+    for (int k = 1; k < VPT; ++k) ss[0] += ss[k];
+    return ss[0];
+}
+
+template <int VPT, bool VEC, int MAXT>
+__global__ void __launch_bounds__(MAXT) norm_row_kernel(NormArgs a, int G) {
+    __shared__ float red[2][32];
+    pdl_launch_dependents();
+    const size_t t = (size_t)blockIdx.x * (blockDim.x / G) + threadIdx.x / G;
+    if (t >= (size_t)a.n_tok) return;  // whole warps: G is 32 where a CTA has more than one row
+    const Row<VPT, VEC> row{G, (int)(threadIdx.x % G), a.E};
+    pdl_wait();
+    float v[VPT][8];
+    row.load(a.x, a.x_bf16, t * a.ldx, v);
+    const float scale = 1.0f / sqrtf(row_sum(square_sum(v), G, red[0]) / (float)a.E + a.eps);
+    float g = 0.f;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        float w[8];
+        row.weights(a.w, k, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[k][j] = v[k][j] * scale * w[j];
+        if (a.gate_w) {
+            row.weights(a.gate_w, k, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g = fmaf(w[j], v[k][j], g);
+        }
+    }
+    row.store(a.y, a.y_bf16, t * a.ldy, v);
+    if (a.gate_w) {
+        g = row_sum(g, G, red[1]);
+        if (row.l == 0) a.gate[t] = g;
+    }
+}
+
+template <int VPT, bool VEC, int MAXT>
+__global__ void __launch_bounds__(MAXT) residual_row_kernel(ResidualArgs a, int G) {
+    __shared__ float red[3][32];
+    pdl_launch_dependents();
+    const size_t t = (size_t)blockIdx.x * (blockDim.x / G) + threadIdx.x / G;
+    if (t >= (size_t)a.n_tok) return;
+    const Row<VPT, VEC> row{G, (int)(threadIdx.x % G), a.E};
+    pdl_wait();
+    float v[VPT][8], r[VPT][8], e[VPT][8];
+    row.load(a.y, a.y_bf16, t * a.ldy, v);
+    row.load(a.res, a.res_bf16, t * a.ldr, r);
+    if (a.gate_kind == GX_GATE_ELEMENT) row.load(a.gate, a.gate_bf16, t * a.ldg, e);
+    float tgate = a.block_scale;
+    if (a.gate_kind == GX_GATE_TOKEN) tgate *= sigmoid_ref(reinterpret_cast<const float *>(a.gate)[t]);
+    float yscale = 1.f;
+    if (a.post_norm) yscale = 1.0f / sqrtf(row_sum(square_sum(v), G, red[0]) / (float)a.E + a.eps);
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        float w[8];
+        row.weights(a.post, k, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float x = v[k][j] * yscale * w[j];
+            if (a.gate_kind == GX_GATE_ELEMENT) x *= sigmoid_ref(e[k][j]);
+            r[k][j] = a.res_scale * r[k][j] + tgate * x;
+        }
+    }
+    row.store(a.res_out, a.res_bf16, t * a.ldro, r);
+    if (!a.out) return;
+    const float rscale = 1.0f / sqrtf(row_sum(square_sum(r), G, red[1]) / (float)a.E + a.next_eps);
+    float g = 0.f;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        float w[8];
+        row.weights(a.next, k, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[k][j] = r[k][j] * rscale * w[j];
+        if (a.next_gate_w) {
+            row.weights(a.next_gate_w, k, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g = fmaf(w[j], r[k][j], g);
+        }
+    }
+    row.store(a.out, a.out_bf16, t * a.ldo, r);
+    if (a.next_gate_w) {
+        g = row_sum(g, G, red[2]);
+        if (row.l == 0) a.next_gate[t] = g;
+    }
+}
+
+// Whether rows of E elements at stride ld can be accessed 16 bytes at a time.
+bool vec_rows(const void *p, int bf16, long long ld) {
+    return !p || (((uintptr_t)p & 15) == 0 && ld * (bf16 ? 2 : 4) % 16 == 0);
+}
+bool vec_words(const float *p) { return ((uintptr_t)p & 15) == 0; }
+
+// Threads of a row, and rows of a CTA: rows of up to 512 values take one warp each, 8 in a CTA.
+struct Shape {
+    int G, block, grid;
+};
+Shape row_shape(int E, int n_tok, int vpt) {
+    Shape s;
+    const int lanes = (E + 8 * vpt - 1) / (8 * vpt);
+    s.G = (lanes + 31) / 32 * 32;
+    const int rows = s.G == 32 ? 8 : 1;
+    s.block = s.G * rows;
+    s.grid = (n_tok + rows - 1) / rows;
+    return s;
+}
+
+// Calls f with the kernel's vectors a thread (two; four for rows beyond 8192, one while the rows are
+// fewer than the SMs and latency is what counts), and whether accesses are 16 bytes wide.
+template <typename F>
+cudaError_t with_row_kernel(int E, int n_tok, bool vec, F f) {
+    constexpr int kFew = 148;
+    if (n_tok < kFew && E <= 4096)
+        return vec ? f(std::integral_constant<int, 1>{}, std::true_type{}) : f(std::integral_constant<int, 1>{}, std::false_type{});
+    if (E <= 8192)
+        return vec ? f(std::integral_constant<int, 2>{}, std::true_type{}) : f(std::integral_constant<int, 2>{}, std::false_type{});
+    return vec ? f(std::integral_constant<int, 4>{}, std::true_type{}) : f(std::integral_constant<int, 4>{}, std::false_type{});
+}
+
 }  // namespace
 
 cudaError_t launch_norm(const NormArgs &a, cudaStream_t s) {
     if (a.n_tok <= 0) return cudaSuccess;
-    norm_kernel<<<a.n_tok, kNormThreads, 0, s>>>(a);
-    return cudaGetLastError();
+    if (a.E > kNormRowMax)
+        return launch_chain_pdl(true, norm_long_kernel, dim3((unsigned)a.n_tok), dim3(kNormThreads), 0, s, a);
+    const bool vec = a.E % 8 == 0 && vec_rows(a.x, a.x_bf16, a.ldx) && vec_rows(a.y, a.y_bf16, a.ldy) && vec_words(a.w) &&
+                     vec_words(a.gate_w);
+    return with_row_kernel(a.E, a.n_tok, vec, [&](auto vpt, auto v) {
+        const Shape p = row_shape(a.E, a.n_tok, vpt.value);
+        return launch_chain_pdl(true, norm_row_kernel<vpt.value, v.value, 512>, dim3((unsigned)p.grid), dim3((unsigned)p.block),
+                                0, s, a, p.G);
+    });
 }
 
 cudaError_t launch_norm_residual(const ResidualArgs &a, cudaStream_t s) {
     if (a.n_tok <= 0) return cudaSuccess;
-    norm_residual_kernel<<<a.n_tok, kNormThreads, 0, s>>>(a);
-    return cudaGetLastError();
+    if (a.E > kNormRowMax)
+        return launch_chain_pdl(true, residual_long_kernel, dim3((unsigned)a.n_tok), dim3(kNormThreads), 0, s, a);
+    const bool vec = a.E % 8 == 0 && vec_rows(a.y, a.y_bf16, a.ldy) && vec_rows(a.res, a.res_bf16, a.ldr) &&
+                     vec_rows(a.res_out, a.res_bf16, a.ldro) && vec_rows(a.out, a.out_bf16, a.ldo) &&
+                     (a.gate_kind != GX_GATE_ELEMENT || vec_rows(a.gate, a.gate_bf16, a.ldg)) && vec_words(a.post) &&
+                     vec_words(a.next) && vec_words(a.next_gate_w);
+    return with_row_kernel(a.E, a.n_tok, vec, [&](auto vpt, auto v) {
+        const Shape p = row_shape(a.E, a.n_tok, vpt.value);
+        return launch_chain_pdl(true, residual_row_kernel<vpt.value, v.value, 512>, dim3((unsigned)p.grid),
+                                dim3((unsigned)p.block), 0, s, a, p.G);
+    });
 }
 
 }  // namespace gx
