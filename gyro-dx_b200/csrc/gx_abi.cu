@@ -2502,7 +2502,7 @@ GX_API gx_result gx_norm(gx_context *c, const gx_norm_desc *d, uint32_t n_tok, u
     a.n_tok = (int)n_tok;
     a.E = (int)d->n_embd;
     a.eps = d->eps;
-    GX_CUDA(gx::launch_norm(a, c->stream));
+    GX_CUDA(gx::launch_norm(a, c->sm_count, c->stream));
     return finish_call(c, capturing, out_ticket);
 }
 
@@ -2539,7 +2539,7 @@ GX_API gx_result gx_norm_residual(gx_context *c, const gx_residual_desc *d, uint
     a.eps = a.next_eps = d->eps;
     a.res_scale = d->res_scale;
     a.block_scale = d->block_scale;
-    GX_CUDA(gx::launch_norm_residual(a, c->stream));
+    GX_CUDA(gx::launch_norm_residual(a, c->sm_count, c->stream));
     return finish_call(c, capturing, out_ticket);
 }
 
@@ -2640,7 +2640,7 @@ GX_API gx_result gx_norm_block(gx_context *c, uint32_t first, uint32_t n_layers,
         a.n_tok = (int)n_tok;
         a.E = (int)E;
         a.eps = L.nm_eps;
-        GX_CUDA(gx::launch_norm(a, c->stream));
+        GX_CUDA(gx::launch_norm(a, c->sm_count, c->stream));
     }
     for (uint32_t i = 0; i < n_layers; ++i) {
         const Layer &L = c->layers[first + i];
@@ -2666,7 +2666,7 @@ GX_API gx_result gx_norm_block(gx_context *c, uint32_t first, uint32_t n_layers,
         a.next_eps = N ? N->nm_eps : 0.f;
         a.res_scale = L.nm_res_scale;
         a.block_scale = L.nm_block_scale;
-        GX_CUDA(gx::launch_norm_residual(a, c->stream));
+        GX_CUDA(gx::launch_norm_residual(a, c->sm_count, c->stream));
     }
     return record_ticket(c, out_ticket);
 }

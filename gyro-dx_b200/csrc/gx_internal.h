@@ -430,7 +430,7 @@ struct NormArgs {
     int n_tok, E;
     float eps;
 };
-cudaError_t launch_norm(const NormArgs &a, cudaStream_t s);
+cudaError_t launch_norm(const NormArgs &a, int sm_count, cudaStream_t s);
 
 struct ResidualArgs {
     const void *y;           // the block's output
@@ -456,7 +456,7 @@ struct ResidualArgs {
     int n_tok, E;
     float eps, next_eps, res_scale, block_scale;
 };
-cudaError_t launch_norm_residual(const ResidualArgs &a, cudaStream_t s);
+cudaError_t launch_norm_residual(const ResidualArgs &a, int sm_count, cudaStream_t s);
 
 constexpr int kMaxTop = 32;
 struct LogprobsArgs {

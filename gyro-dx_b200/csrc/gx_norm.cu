@@ -13,7 +13,6 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <type_traits>
 
 #include "../../include/gyro_moe.h"
 #include "gx_dense.cuh"
@@ -32,6 +31,19 @@ constexpr int kNormRowMax = 16384;   // longest row held in registers: 512 threa
 __device__ __forceinline__ void store_act(void *p, int bf16, size_t i, float v) {
     if (bf16) reinterpret_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
     else reinterpret_cast<float *>(p)[i] = v;
+}
+
+// 1 / (1 + e^-x) to about 4 units of 2^-24, in 10 instructions (expf and a division take four times as
+// many, which bounds the kernel that gates every element): 2^t with the rounding of t = -x log2 e put back.
+__device__ __forceinline__ float sigmoid(float x) {
+    constexpr float l2e = 1.44269504088896341f, l2e_rest = (float)(1.44269504088896341 - (double)1.44269504088896341f);
+    asm("min.NaN.f32 %0, %0, 0f461c4000;\n max.NaN.f32 %0, %0, 0fc61c4000;" : "+f"(x));  // +-10^4: 0 or 1 beyond
+    const float t = -x * l2e, rest = fmaf(-x, l2e_rest, fmaf(-x, l2e, -t));
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    e = fmaf(e, rest * 0.693147180559945309f, e);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return r;
 }
 
 __device__ __forceinline__ float block_sum(float v, float *red) {
@@ -72,7 +84,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_long_kernel(NormArgs a) {
 __device__ __forceinline__ float residual_value(const ResidualArgs &a, size_t t, int i, float yscale, float tgate) {
     float v = load_act(a.y, a.y_bf16, t * a.ldy + i) * yscale;
     if (a.post) v *= a.post[i];
-    if (a.gate_kind == GX_GATE_ELEMENT) v *= sigmoid_ref(load_act(a.gate, a.gate_bf16, t * a.ldg + i));
+    if (a.gate_kind == GX_GATE_ELEMENT) v *= sigmoid(load_act(a.gate, a.gate_bf16, t * a.ldg + i));
     return a.res_scale * load_act(a.res, a.res_bf16, t * a.ldr + i) + a.block_scale * tgate * v;
 }
 
@@ -90,7 +102,7 @@ __global__ void __launch_bounds__(kNormThreads) residual_long_kernel(ResidualArg
         }
         yscale = 1.0f / sqrtf(block_sum(ss, red) / (float)a.E + a.eps);
     }
-    const float tgate = a.gate_kind == GX_GATE_TOKEN ? sigmoid_ref(reinterpret_cast<const float *>(a.gate)[t]) : 1.f;
+    const float tgate = a.gate_kind == GX_GATE_TOKEN ? sigmoid(reinterpret_cast<const float *>(a.gate)[t]) : 1.f;
     // The sum of squares first: res_out may be res, so r is computed again before it is stored.
     float ss = 0.f;
     if (a.out)
@@ -117,7 +129,8 @@ __global__ void __launch_bounds__(kNormThreads) residual_long_kernel(ResidualArg
 
 // ---- rows held in registers --------------------------------------------------------------------
 // Thread l of a row's G has the elements (k G + l) 8 + j (VEC: 16-byte accesses; the width is a
-// multiple of 8 and every row aligned) or (8 k + j) G + l.
+// multiple of 8 and every row aligned) or (8 k + j) G + l. (Kernels for each combination of
+// encodings were no faster.)
 template <int VPT, bool VEC>
 struct Row {
     int G, l, E;
@@ -221,8 +234,8 @@ __device__ __forceinline__ float square_sum(const float (&v)[VPT][8]) {
     return ss[0];
 }
 
-template <int VPT, bool VEC, int MAXT>
-__global__ void __launch_bounds__(MAXT) norm_row_kernel(NormArgs a, int G) {
+template <int VPT, bool VEC>
+__global__ void __launch_bounds__(512) norm_row_kernel(NormArgs a, int G) {
     __shared__ float red[2][32];
     pdl_launch_dependents();
     const size_t t = (size_t)blockIdx.x * (blockDim.x / G) + threadIdx.x / G;
@@ -252,8 +265,81 @@ __global__ void __launch_bounds__(MAXT) norm_row_kernel(NormArgs a, int G) {
     }
 }
 
-template <int VPT, bool VEC, int MAXT>
-__global__ void __launch_bounds__(MAXT) residual_row_kernel(ResidualArgs a, int G) {
+// Many rows of G * 8 * VPT values exactly, 16-byte accesses, no gate: each CTA walks over rows with its
+// weights in registers and the next row already on its way.
+template <int VPT, bool XB, bool YB>
+__global__ void __launch_bounds__(512, 2) norm_stream_kernel(NormArgs a) {
+    __shared__ float red[2][32];
+    constexpr int Q = XB ? 1 : 2;  // 16-byte words of 8 values
+    const int G = blockDim.x, l = threadIdx.x;
+    pdl_launch_dependents();
+    pdl_wait();
+    uint4 raw[VPT][Q];
+    auto fetch = [&](size_t t) {
+#pragma unroll
+        for (int k = 0; k < VPT; ++k)
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+                raw[k][q] = __ldcs(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(a.x) + t * a.ldx * (XB ? 2 : 4)) +
+                                   (k * G + l) * Q + q);
+    };
+    size_t t = blockIdx.x;
+    fetch(t);
+    float w[VPT][8];
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[k][j] = 1.f;
+        if (a.w) {
+            const float4 *p = reinterpret_cast<const float4 *>(a.w) + (k * G + l) * 2;
+            const float4 u = __ldg(p), v = __ldg(p + 1);
+            w[k][0] = u.x; w[k][1] = u.y; w[k][2] = u.z; w[k][3] = u.w;
+            w[k][4] = v.x; w[k][5] = v.y; w[k][6] = v.z; w[k][7] = v.w;
+        }
+    }
+    const float mean = 1.0f / (float)a.E;
+    for (int parity = 0; t < (size_t)a.n_tok; t += gridDim.x, parity ^= 1) {
+        float v[VPT][8];
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const uint32_t *u = reinterpret_cast<const uint32_t *>(&raw[k][0]);
+#pragma unroll
+            for (int j = 0; j < 4 * Q; ++j) {
+                if constexpr (XB) {
+                    v[k][2 * j] = __uint_as_float(u[j] << 16);
+                    v[k][2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+                } else {
+                    v[k][j] = __uint_as_float(u[j]);
+                }
+            }
+        }
+        if (t + gridDim.x < (size_t)a.n_tok) fetch(t + gridDim.x);
+        // two places for the sums in turn: one barrier a row
+        const float ss = row_sum(square_sum(v), G, red[parity]);
+        const float scale = 1.0f / sqrtf(fmaf(ss, mean, a.eps));
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[k][j] = v[k][j] * scale * w[k][j];
+            if constexpr (YB) {
+                uint32_t o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[k][2 * j], v[k][2 * j + 1]);
+                    o[j] = *reinterpret_cast<const uint32_t *>(&h);
+                }
+                reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(a.y) + t * a.ldy)[k * G + l] = make_uint4(o[0], o[1], o[2], o[3]);
+            } else {
+                float4 *f = reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.y) + t * a.ldy) + (k * G + l) * 2;
+                f[0] = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
+                f[1] = make_float4(v[k][4], v[k][5], v[k][6], v[k][7]);
+            }
+        }
+    }
+}
+
+template <int VPT, bool VEC>
+__global__ void __launch_bounds__(512) residual_row_kernel(ResidualArgs a, int G) {
     __shared__ float red[3][32];
     pdl_launch_dependents();
     const size_t t = (size_t)blockIdx.x * (blockDim.x / G) + threadIdx.x / G;
@@ -265,7 +351,7 @@ __global__ void __launch_bounds__(MAXT) residual_row_kernel(ResidualArgs a, int 
     row.load(a.res, a.res_bf16, t * a.ldr, r);
     if (a.gate_kind == GX_GATE_ELEMENT) row.load(a.gate, a.gate_bf16, t * a.ldg, e);
     float tgate = a.block_scale;
-    if (a.gate_kind == GX_GATE_TOKEN) tgate *= sigmoid_ref(reinterpret_cast<const float *>(a.gate)[t]);
+    if (a.gate_kind == GX_GATE_TOKEN) tgate *= sigmoid(reinterpret_cast<const float *>(a.gate)[t]);
     float yscale = 1.f;
     if (a.post_norm) yscale = 1.0f / sqrtf(row_sum(square_sum(v), G, red[0]) / (float)a.E + a.eps);
 #pragma unroll
@@ -275,7 +361,7 @@ __global__ void __launch_bounds__(MAXT) residual_row_kernel(ResidualArgs a, int 
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             float x = v[k][j] * yscale * w[j];
-            if (a.gate_kind == GX_GATE_ELEMENT) x *= sigmoid_ref(e[k][j]);
+            if (a.gate_kind == GX_GATE_ELEMENT) x *= sigmoid(e[k][j]);
             r[k][j] = a.res_scale * r[k][j] + tgate * x;
         }
     }
@@ -322,34 +408,48 @@ Shape row_shape(int E, int n_tok, int vpt) {
     return s;
 }
 
-// Calls f with the kernel's vectors a thread (two; four for rows beyond 8192, one while the rows are
-// fewer than the SMs and latency is what counts), and whether accesses are 16 bytes wide.
-template <typename F>
-cudaError_t with_row_kernel(int E, int n_tok, bool vec, F f) {
-    constexpr int kFew = 148;
-    if (n_tok < kFew && E <= 4096)
-        return vec ? f(std::integral_constant<int, 1>{}, std::true_type{}) : f(std::integral_constant<int, 1>{}, std::false_type{});
-    if (E <= 8192)
-        return vec ? f(std::integral_constant<int, 2>{}, std::true_type{}) : f(std::integral_constant<int, 2>{}, std::false_type{});
-    return vec ? f(std::integral_constant<int, 4>{}, std::true_type{}) : f(std::integral_constant<int, 4>{}, std::false_type{});
+// The vectors of a thread: two; four for rows beyond 8192; one while the rows are fewer than the SMs and
+// latency is what counts.
+int row_vectors(int E, int n_tok, int sm_count) { return n_tok < sm_count && E <= 4096 ? 1 : E <= 8192 ? 2 : 4; }
+
+template <int VPT>
+cudaError_t launch_norm_row(const NormArgs &a, bool vec, cudaStream_t s) {
+    const Shape p = row_shape(a.E, a.n_tok, VPT);
+    auto *k = vec ? norm_row_kernel<VPT, true> : norm_row_kernel<VPT, false>;
+    return launch_chain_pdl(true, k, dim3((unsigned)p.grid), dim3((unsigned)p.block), 0, s, a, p.G);
+}
+
+template <int VPT>
+cudaError_t launch_residual_row(const ResidualArgs &a, bool vec, cudaStream_t s) {
+    const Shape p = row_shape(a.E, a.n_tok, VPT);
+    auto *k = vec ? residual_row_kernel<VPT, true> : residual_row_kernel<VPT, false>;
+    return launch_chain_pdl(true, k, dim3((unsigned)p.grid), dim3((unsigned)p.block), 0, s, a, p.G);
 }
 
 }  // namespace
 
-cudaError_t launch_norm(const NormArgs &a, cudaStream_t s) {
+cudaError_t launch_norm(const NormArgs &a, int sm_count, cudaStream_t s) {
     if (a.n_tok <= 0) return cudaSuccess;
     if (a.E > kNormRowMax)
         return launch_chain_pdl(true, norm_long_kernel, dim3((unsigned)a.n_tok), dim3(kNormThreads), 0, s, a);
     const bool vec = a.E % 8 == 0 && vec_rows(a.x, a.x_bf16, a.ldx) && vec_rows(a.y, a.y_bf16, a.ldy) && vec_words(a.w) &&
                      vec_words(a.gate_w);
-    return with_row_kernel(a.E, a.n_tok, vec, [&](auto vpt, auto v) {
-        const Shape p = row_shape(a.E, a.n_tok, vpt.value);
-        return launch_chain_pdl(true, norm_row_kernel<vpt.value, v.value, 512>, dim3((unsigned)p.grid), dim3((unsigned)p.block),
-                                0, s, a, p.G);
-    });
+    // Enough rows for every CTA to walk over several, in the widths that fill its threads (64 threads and
+    // more of two vectors).
+    const int G = a.E / 16, resident = sm_count * (1024 / (G ? G : 1));
+    if (vec && !a.gate_w && a.E % 512 == 0 && a.E >= 1024 && a.E <= 8192 && a.n_tok >= 4 * resident) {
+        auto *k = a.x_bf16 ? (a.y_bf16 ? norm_stream_kernel<2, true, true> : norm_stream_kernel<2, true, false>)
+                           : (a.y_bf16 ? norm_stream_kernel<2, false, true> : norm_stream_kernel<2, false, false>);
+        return launch_chain_pdl(true, k, dim3((unsigned)resident), dim3((unsigned)G), 0, s, a);
+    }
+    switch (row_vectors(a.E, a.n_tok, sm_count)) {
+        case 1: return launch_norm_row<1>(a, vec, s);
+        case 2: return launch_norm_row<2>(a, vec, s);
+        default: return launch_norm_row<4>(a, vec, s);
+    }
 }
 
-cudaError_t launch_norm_residual(const ResidualArgs &a, cudaStream_t s) {
+cudaError_t launch_norm_residual(const ResidualArgs &a, int sm_count, cudaStream_t s) {
     if (a.n_tok <= 0) return cudaSuccess;
     if (a.E > kNormRowMax)
         return launch_chain_pdl(true, residual_long_kernel, dim3((unsigned)a.n_tok), dim3(kNormThreads), 0, s, a);
@@ -357,11 +457,11 @@ cudaError_t launch_norm_residual(const ResidualArgs &a, cudaStream_t s) {
                      vec_rows(a.res_out, a.res_bf16, a.ldro) && vec_rows(a.out, a.out_bf16, a.ldo) &&
                      (a.gate_kind != GX_GATE_ELEMENT || vec_rows(a.gate, a.gate_bf16, a.ldg)) && vec_words(a.post) &&
                      vec_words(a.next) && vec_words(a.next_gate_w);
-    return with_row_kernel(a.E, a.n_tok, vec, [&](auto vpt, auto v) {
-        const Shape p = row_shape(a.E, a.n_tok, vpt.value);
-        return launch_chain_pdl(true, residual_row_kernel<vpt.value, v.value, 512>, dim3((unsigned)p.grid),
-                                dim3((unsigned)p.block), 0, s, a, p.G);
-    });
+    switch (row_vectors(a.E, a.n_tok, sm_count)) {
+        case 1: return launch_residual_row<1>(a, vec, s);
+        case 2: return launch_residual_row<2>(a, vec, s);
+        default: return launch_residual_row<4>(a, vec, s);
+    }
 }
 
 }  // namespace gx

@@ -317,6 +317,27 @@ def test_norm_residual_many_rows(ctx):
     check_residual(ctx, 1500, 520, "bf16", "bf16", "bf16", "bf16", seed=2, gate="token", in_place=False)
 
 
+@pytest.mark.parametrize("width,n", [(1024, 9473), (2560, 4100), (8192, 1300)])
+def test_norm_long_batches(ctx, width, n):
+    """Enough rows for every CTA to take several."""
+    rng = np.random.default_rng(width)
+    w = (1 + 0.3 * rng.normal(0, 1, width)).astype(np.float32)
+    for xk, yk, weight in (("bf16", "f32", w), ("f32", "bf16", None), ("f32", "f32", w), ("bf16", "bf16", w)):
+        x = refs.to_kind(rng.standard_normal((n, width), np.float32), xk)
+        y, buf = out_rows(n, width, yk, width + 8)
+        ctx.wait(ctx.norm(dev(x, xk), y, None if weight is None else dev(weight)))
+        near(y, *refs.norm(x, weight, 1e-6, yk)[0])
+        untouched(buf, n, width)
+
+
+@pytest.mark.parametrize("width,n", [(512, 7200), (2560, 1300), (4096, 700)])
+def test_norm_residual_long_batches(ctx, width, n):
+    for i, k in enumerate([("f32", "bf16", "bf16", "f32"), ("bf16", "f32", "f32", "bf16"), ("f32", "f32", "f32", "f32")]):
+        check_residual(ctx, n, width, *k, seed=i, gate="element", next_gate=i == 0, in_place=i == 1)
+        check_residual(ctx, n, width, *k, seed=i, gate="token" if i else None, next_gate=i == 1, post_norm=i != 2)
+        check_residual(ctx, n, width, *k, seed=i, gate="token", has_out=False, strides=(width + 8,) * 5, in_place=False)
+
+
 def test_norm_residual_refusals(ctx):
     y, r = torch.zeros(4, 64, device="cuda"), torch.ones(4, 64, device="cuda")
     for bad in [dict(out=y), dict(out=r), dict(res_out=y), dict(next_weight=torch.ones(64, device="cuda")),
