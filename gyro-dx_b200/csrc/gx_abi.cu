@@ -2413,6 +2413,7 @@ gx_result enqueue_q4(gx_context *c, const Matrix &m, const void *x, uint32_t x_d
     a.rows = (int)m.rows;
     a.cols = (int)m.cols;
     a.n_tok = (int)n_tok;
+    a.err = c->err;
     GX_CUDA(gx::launch_q4_linear(a, c->q4_ws.back(), c->sm_count, c->stream));
     return GX_OK;
 }

@@ -408,6 +408,7 @@ struct Q4Args {
     int y_bf16;
     long long ldy;
     int rows, cols, n_tok;
+    int *err;
 };
 uint64_t q4_row_bytes(uint32_t type, uint64_t cols);               // of the model file's layout
 uint64_t q4_bytes(uint32_t type, uint64_t rows, uint64_t cols);    // of the device layout

@@ -20,6 +20,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "../../include/gyro_moe.h"
 #include "gx_dense.cuh"
 #include "gx_device.cuh"
@@ -135,6 +137,17 @@ __device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// The product of a group: both halves of its 32 columns, on nothing.
+__device__ __forceinline__ void mma_group(float (&d)[4], const uint32_t (&a0)[4], const uint32_t (&a1)[4], const uint4 &b) {
+    asm("{\n"
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%12,%13}, {%16,%16,%16,%16};\n"
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%8,%9,%10,%11}, {%14,%15}, {%0,%1,%2,%3};\n"
+        "}\n"
+        : "=&f"(d[0]), "=&f"(d[1]), "=&f"(d[2]), "=&f"(d[3])
+        : "r"(a0[0]), "r"(a0[1]), "r"(a0[2]), "r"(a0[3]), "r"(a1[0]), "r"(a1[1]), "r"(a1[2]), "r"(a1[3]), "r"(b.x), "r"(b.y),
+          "r"(b.z), "r"(b.w), "f"(0.f));
 }
 
 // The A registers of 8 codes of row g (r0) and of row g + 8 (r1): columns (0,4) (2,6) of each in a0,
@@ -492,7 +505,21 @@ struct Halves {
     }
 };
 
-constexpr int kMaxSmem = 227 * 1024;  // of a CTA
+constexpr int kMaxSmem = 227 * 1024, kStaticSmem = 1024;  // of a CTA; what of it is not dynamic, at most
+
+// Lets a kernel use all of it, once per device (a call for every launch costs 0.5 us).
+struct SmemLimit {
+    std::atomic<uint64_t> done{0};
+    template <typename K>
+    cudaError_t raise(K *k) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return e;
+        e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem - kStaticSmem);
+        if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+        return e;
+    }
+};
 
 struct GemvPlan {
     int RT, KT;      // row tiles, units in a row
@@ -516,6 +543,14 @@ __device__ __forceinline__ float ld_cluster(const float *p, uint32_t rank) {
     float v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ float4 ld_cluster4(const float *p, uint32_t rank) {
+    uint32_t at;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
     return v;
 }
 
@@ -625,7 +660,8 @@ __global__ void __launch_bounds__(W * 32, M::CTAS(W)) q4_gemv_kernel(Q4Args a, G
 template <uint32_t TYPE, class M, int W>
 cudaError_t launch_gemv_w(const Q4Args &a, GemvPlan p, int smem, int grid, cudaStream_t s) {
     auto *k = q4_gemv_kernel<TYPE, M, W>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static SmemLimit limit;
+    const cudaError_t e = limit.raise(k);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
@@ -666,7 +702,7 @@ cudaError_t launch_gemv(const Q4Args &a, int t0, int nt, int sm_count, cudaStrea
     const int W = wide ? 16 : 8;
     p.red_off = xbytes;
     const int smem = p.red_off + 2 * W * kTileRows * M::TOK * 4;
-    if (smem > kMaxSmem) return cudaErrorInvalidValue;
+    if (smem > kMaxSmem - kStaticSmem) return cudaErrorInvalidValue;
     const int groups = W / p.WK, need = (p.RT + groups - 1) / groups;
     const int resident = sm_count * M::CTAS(W);
     const int grid = p.S > 1 ? need * p.S : need < resident ? need : resident;
@@ -676,22 +712,24 @@ cudaError_t launch_gemv(const Q4Args &a, int t0, int nt, int sm_count, cudaStrea
 // ---- more tokens: a tiled product on mma.sync ---------------------------------------------------
 // The activations are packed once per call (q4_pack_kernel) into the same fragments, at one scale per
 // token, in a workspace of the context: [unit][4 groups][COLS columns][4 q] 16 B, then the group sums
-// [4 groups][TOK tokens] of the unit; the tokens' inverse scales stand before the first unit.
-constexpr int kQ4InvBytes = 256;
+// [4 groups][TOK tokens] of the unit; the tokens' inverse scales stand before the first unit. (A scale and
+// a CTA per token and range of units packs no faster, and the product then waits 2 us longer for it.)
+constexpr int kQ4InvBytes = 64 * 4;
 
 struct GemmPlan {
     int RT, KT;
-    int WM, WN, WK;  // warps: row pairs of tiles, column groups, splits of the units
+    int WM, WK;      // warps: row tiles of a CTA, and splits of its units
     int S;           // CTAs of a cluster that split the units
     int vec;
 };
 
 constexpr int kPackThreads = 512;
 
+// One CTA per token.
 template <uint32_t TYPE, bool XB>
 __global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(Q4Args a, uint8_t *ws, int KT, int cols_padded, int vec) {
     __shared__ uint32_t red[kPackThreads / 32];
-    const int t = blockIdx.x, tid = threadIdx.x;
+    const int t = blockIdx.x, tid = threadIdx.x, cells = KT * 16;
     const int tok_padded = XB ? cols_padded : cols_padded / 2;
     const size_t unit = (size_t)cols_padded * 256 + (size_t)tok_padded * 16;
     pdl_launch_dependents();
@@ -700,7 +738,7 @@ __global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(Q4Args a, uint8_t
         const int col = cell * 8;
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = 0.f;
-        if (col < a.cols) {
+        if (cell < cells && col < a.cols) {
             const size_t at = (size_t)t * a.ldx + col;
             if (vec) load_x8(a.x, XB, at, v);
             else {
@@ -709,17 +747,16 @@ __global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(Q4Args a, uint8_t
             }
         }
     };
-    const int cells = KT * 16;
     float first[8];
+    load(tid, first);
     uint32_t big = 0;
-    for (int cell = tid; cell < cells; cell += kPackThreads) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) big = max(big, __float_as_uint(first[k]) & 0x7fffffffu);
+    for (int cell = tid + kPackThreads; cell < cells; cell += kPackThreads) {
         float v[8];
         load(cell, v);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            big = max(big, __float_as_uint(v[k]) & 0x7fffffffu);
-            if (cell == tid) first[k] = v[k];
-        }
+        for (int k = 0; k < 8; ++k) big = max(big, __float_as_uint(v[k]) & 0x7fffffffu);
     }
     big = __reduce_max_sync(0xffffffffu, big);
     if ((tid & 31) == 0) red[tid >> 5] = big;
@@ -735,12 +772,9 @@ __global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(Q4Args a, uint8_t
         float v[8];
         if (base == 0) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = cell < cells ? first[k] : 0.f;
-        } else if (cell < cells) {
-            load(cell, v);
+            for (int k = 0; k < 8; ++k) v[k] = first[k];
         } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = 0.f;
+            load(cell, v);
         }
         float ss = 0.f;
 #pragma unroll
@@ -748,8 +782,7 @@ __global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(Q4Args a, uint8_t
             v[k] = e == 255u ? __uint_as_float(0x7fffffffu) : v[k] * s;
             ss += v[k];
         }
-        ss += __shfl_xor_sync(0xffffffffu, ss, 1);
-        ss += __shfl_xor_sync(0xffffffffu, ss, 2);
+        if constexpr (TYPE == GX_Q4_1) ss = quad_sum(ss);
         if (cell >= cells) continue;
         const int q = cell & 3, j = (cell >> 2) & 3;
         uint8_t *u = units + (size_t)(cell >> 4) * unit;
@@ -758,212 +791,228 @@ __global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(Q4Args a, uint8_t
     }
 }
 
-__device__ __forceinline__ void cp_async16(void *dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+constexpr int kGemmWarps = 8;
+constexpr int gemm_stages(int MT) { return MT == 2 ? 3 : 2; }
+
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-constexpr int kGemmStages = 3;
-
-// A CTA takes 2 WM row tiles by all tokens over its range of units: warp (wk, wm, wn) two row tiles by
-// NB product tiles of every WK-th unit. Codes and fragments come through a ring of shared-memory
-// stages of WK units; the parts are added over wk and the cluster's CTAs at the end.
-template <uint32_t TYPE, bool XB, int NB>
-__global__ void __launch_bounds__(512, 1) q4_gemm_kernel(Q4Args a, const uint8_t *ws, GemmPlan p) {
-    constexpr int NA = XB ? 4 : 2, UB = unit_bytes(TYPE);
+// A CTA takes WM row tiles by all tokens over its range of units: warp (wk, wm) one row tile of every
+// WK-th unit, NB product tiles wide, so that a code is unpacked once. Codes and fragments come by bulk
+// copies through a ring of shared-memory stages of WK units; the parts are added over wk and the
+// cluster's CTAs at the end.
+template <uint32_t TYPE, bool XB, int NB, int MT>
+__global__ void __launch_bounds__(kGemmWarps * 32, 2) q4_gemm_kernel(Q4Args a, const uint8_t *ws, GemmPlan p) {
+    constexpr int NA = XB ? 4 : 2, UB = unit_bytes(TYPE), COLS = 8 * NB, TOK = XB ? COLS : COLS / 2;
+    constexpr int BU = COLS * 256 + TOK * 16;  // a unit's fragments and sums
+    constexpr int kGemmStages = gemm_stages(MT);
     extern __shared__ __align__(16) uint8_t smem[];
-    const int tid = threadIdx.x, nthr = blockDim.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-    const int wn = warp % p.WN, wm = warp / p.WN % p.WM, wk = warp / (p.WN * p.WM);
-    const int COLS = p.WN * NB * 8, TOK = XB ? COLS : COLS / 2;
-    const int bunit = COLS * 256 + TOK * 16, tiles = 2 * p.WM, sunit = bunit + tiles * UB, stage_bytes = p.WK * sunit;
+    __shared__ __align__(8) uint64_t bars[kGemmStages], empty[kGemmStages];  // a stage has come; all warps have read it
+    __shared__ float inv[64];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+    const int wm = warp % p.WM, wk = warp / p.WM;
+    const int unit_stage = BU + MT * p.WM * UB, stage_bytes = p.WK * unit_stage;
     const int rank = p.S > 1 ? (int)cluster_rank() : 0;
     const int u0 = (int)((long long)p.KT * rank / p.S), u1 = (int)((long long)p.KT * (rank + 1) / p.S), nu = u1 - u0;
-    const int rt0 = (int)(blockIdx.x / p.S) * tiles, iters = (nu + p.WK - 1) / p.WK;
+    const int rt0 = (int)(blockIdx.x / p.S) * p.WM * MT, iters = (nu + p.WK - 1) / p.WK;
+    const int tiles = min(p.WM * MT, p.RT - rt0);
     const uint8_t *units = ws + kQ4InvBytes;
 
-    auto load_codes = [&](int it) {
-        if (it >= iters) return;
-        uint8_t *st = smem + (it % kGemmStages) * stage_bytes;
-        const int per = UB / 16, total = p.WK * tiles * per;
-        for (int i = tid; i < total; i += nthr) {
-            const int c = i % per, tile = i / per % tiles, k = i / (per * tiles), u = it * p.WK + k;
-            if (u < nu && rt0 + tile < p.RT)
-                cp_async16(st + k * sunit + bunit + tile * UB + c * 16,
-                           a.w + ((size_t)(rt0 + tile) * p.KT + u0 + u) * UB + c * 16);
-        }
+    auto copy_codes = [&](int it) {  // and the bytes that the stage waits for
+        const int n = min(p.WK, nu - it * p.WK);
+        mbar_expect_tx(&bars[it % kGemmStages], (uint32_t)(n * (BU + tiles * UB)));
+        for (int k = 0; k < n; ++k)
+            for (int t = 0; t < tiles; ++t)
+                bulk_g2s(smem + (it % kGemmStages) * stage_bytes + k * unit_stage + BU + t * UB,
+                         a.w + ((size_t)(rt0 + t) * p.KT + u0 + it * p.WK + k) * UB, UB, &bars[it % kGemmStages]);
     };
-    auto load_frags = [&](int it) {
-        if (it >= iters) return;
-        uint8_t *st = smem + (it % kGemmStages) * stage_bytes;
-        const int per = bunit / 16, total = p.WK * per;
-        for (int i = tid; i < total; i += nthr) {
-            const int k = i / per, c = i - k * per, u = it * p.WK + k;
-            if (u < nu) cp_async16(st + k * sunit + c * 16, units + (size_t)(u0 + u) * bunit + c * 16);
-        }
+    auto copy_frags = [&](int it) {
+        const int n = min(p.WK, nu - it * p.WK);
+        for (int k = 0; k < n; ++k)
+            bulk_g2s(smem + (it % kGemmStages) * stage_bytes + k * unit_stage, units + (size_t)(u0 + it * p.WK + k) * BU, BU,
+                     &bars[it % kGemmStages]);
     };
-    // the weights never change: they may be fetched before the activations are packed
-#pragma unroll
-    for (int s = 0; s < kGemmStages - 1; ++s) load_codes(s);
+    if (tid == 0) {
+        for (int i = 0; i < kGemmStages; ++i) {
+            mbar_init(&bars[i], 1);
+            mbar_init(&empty[i], kGemmWarps);
+        }
+        fence_barrier_init();
+        // the weights never change: they may be fetched before the activations are packed
+        for (int i = 0; i < kGemmStages && i < iters; ++i) copy_codes(i);
+    }
+    __syncthreads();
     pdl_launch_dependents();
     pdl_wait();
+    if (tid == 0)
+        for (int i = 0; i < kGemmStages && i < iters; ++i) copy_frags(i);
+    if (tid < 64) inv[tid] = tid < a.n_tok ? reinterpret_cast<const float *>(ws)[tid] : 0.f;
+
+    float acc[MT][NB][NA];
 #pragma unroll
-    for (int s = 0; s < kGemmStages - 1; ++s) {
-        load_frags(s);
-        cp_async_commit();
-    }
-    float acc[2][NB][NA];
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
             for (int k = 0; k < NA; ++k) acc[m][n][k] = 0.f;
+    bool ok = true;  // an expired wait is reported and ends the warp's loop
+    int copied = min(iters, kGemmStages);
     for (int it = 0; it < iters; ++it) {
-        cp_async_wait<kGemmStages - 2>();
-        __syncthreads();
-        load_codes(it + kGemmStages - 1);
-        load_frags(it + kGemmStages - 1);
-        cp_async_commit();
-        if (it * p.WK + wk >= nu) continue;
-        const uint8_t *st = smem + (it % kGemmStages) * stage_bytes + wk * sunit;
-        const float *sums = reinterpret_cast<const float *>(st + COLS * 256);
-        uint4 c0[2], c1[2], dv[2], mv[2];
+        ok = mbar_wait(&bars[it % kGemmStages], (uint32_t)(it / kGemmStages & 1), a.err);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (it * p.WK + wk < nu && wm * MT < tiles) {
+            const uint8_t *st = smem + (it % kGemmStages) * stage_bytes + wk * unit_stage;
+            const float *sums = reinterpret_cast<const float *>(st + COLS * 256);
+            const uint8_t *t = st + BU + wm * MT * UB;  // a tile past the matrix holds what was there: nothing of it is stored
+            const uint32_t *codes = reinterpret_cast<const uint32_t *>(t) + lane * 4;
+            const uint32_t *scales = reinterpret_cast<const uint32_t *>(t + 1024) + g * 4;
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j) {
+                uint32_t a0[MT][4], a1[MT][4], mw[MT];
+                float d0[MT], d1[MT];
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            const uint8_t *t = st + bunit + (2 * wm + m) * UB;
-            c0[m] = reinterpret_cast<const uint4 *>(t)[lane];
-            c1[m] = reinterpret_cast<const uint4 *>(t + 512)[lane];
-            dv[m] = reinterpret_cast<const uint4 *>(t + 1024)[g];
-            if constexpr (TYPE == GX_Q4_1) mv[m] = reinterpret_cast<const uint4 *>(t + 1152)[g];
-        }
-        auto word = [](const uint4 &v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; };
-        auto half_of = [&](const uint4 &v, int hi, int j) { return half_value(word(v, j), hi); };
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t a0[2][4], a1[2][4];
-            float d[2][2], mm[2][2];
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                code_fragments<TYPE>(word(c0[m], j), word(c1[m], j), a0[m], a1[m]);
-#pragma unroll
-                for (int hi = 0; hi < 2; ++hi) {
-                    d[m][hi] = half_of(dv[m], hi, j);
-                    if constexpr (TYPE == GX_Q4_1) mm[m][hi] = half_of(mv[m], hi, j);
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                const int nn = wn * NB + n;
-                const uint4 b = *reinterpret_cast<const uint4 *>(st + ((size_t)(j * COLS + 8 * nn) * 4 + lane) * 16);
-                float sx = 0.f, sy = 0.f;
-                if constexpr (TYPE == GX_Q4_0) {
-                } else if constexpr (XB) {
-                    const float2 v = *reinterpret_cast<const float2 *>(sums + j * TOK + 8 * nn + 2 * q);
-                    sx = v.x;
-                    sy = v.y;
-                } else {
-                    sx = sums[j * TOK + 4 * nn + q];
+                for (int m = 0; m < MT; ++m) {
+                    code_fragments<TYPE>(codes[m * (UB / 4) + j], codes[m * (UB / 4) + j + 128], a0[m], a1[m]);
+                    d0[m] = half_value(scales[m * (UB / 4) + j], 0);
+                    d1[m] = half_value(scales[m * (UB / 4) + j], 1);
+                    if constexpr (TYPE == GX_Q4_1) mw[m] = scales[m * (UB / 4) + j + 32];
                 }
 #pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    float c[4];
-                    mma16816_first(c, a0[m], b.x, b.y);
-                    mma16816(c, a1[m], b.z, b.w);
-                    if constexpr (XB) {
-                        acc[m][n][0] = fmaf(d[m][0], c[0], acc[m][n][0]);
-                        acc[m][n][1] = fmaf(d[m][0], c[1], acc[m][n][1]);
-                        acc[m][n][2] = fmaf(d[m][1], c[2], acc[m][n][2]);
-                        acc[m][n][3] = fmaf(d[m][1], c[3], acc[m][n][3]);
-                        if constexpr (TYPE == GX_Q4_1) {
-                            acc[m][n][0] = fmaf(mm[m][0], sx, acc[m][n][0]);
-                            acc[m][n][1] = fmaf(mm[m][0], sy, acc[m][n][1]);
-                            acc[m][n][2] = fmaf(mm[m][1], sx, acc[m][n][2]);
-                            acc[m][n][3] = fmaf(mm[m][1], sy, acc[m][n][3]);
+                for (int n = 0; n < NB; ++n) {
+                    const uint4 b = *reinterpret_cast<const uint4 *>(st + ((j * COLS + 8 * n) * 4 + lane) * 16);
+                    float2 sx = make_float2(0.f, 0.f);
+                    if constexpr (TYPE == GX_Q4_1) {
+                        if constexpr (XB) sx = *reinterpret_cast<const float2 *>(sums + j * TOK + 8 * n + 2 * q);
+                        else sx.x = sums[j * TOK + 4 * n + q];
+                    }
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        float c[4];
+                        mma_group(c, a0[m], a1[m], b);
+                        if constexpr (XB) {
+                            acc[m][n][0] = fmaf(d0[m], c[0], acc[m][n][0]);
+                            acc[m][n][1] = fmaf(d0[m], c[1], acc[m][n][1]);
+                            acc[m][n][2] = fmaf(d1[m], c[2], acc[m][n][2]);
+                            acc[m][n][3] = fmaf(d1[m], c[3], acc[m][n][3]);
+                        } else {
+                            acc[m][n][0] = fmaf(d0[m], c[0] + c[1], acc[m][n][0]);
+                            acc[m][n][1] = fmaf(d1[m], c[2] + c[3], acc[m][n][1]);
                         }
-                    } else {
-                        acc[m][n][0] = fmaf(d[m][0], c[0] + c[1], acc[m][n][0]);
-                        acc[m][n][1] = fmaf(d[m][1], c[2] + c[3], acc[m][n][1]);
                         if constexpr (TYPE == GX_Q4_1) {
-                            acc[m][n][0] = fmaf(mm[m][0], sx, acc[m][n][0]);
-                            acc[m][n][1] = fmaf(mm[m][1], sx, acc[m][n][1]);
+                            const float m0 = half_value(mw[m], 0), m1 = half_value(mw[m], 1);
+                            if constexpr (XB) {
+                                acc[m][n][0] = fmaf(m0, sx.x, acc[m][n][0]);
+                                acc[m][n][1] = fmaf(m0, sx.y, acc[m][n][1]);
+                                acc[m][n][2] = fmaf(m1, sx.x, acc[m][n][2]);
+                                acc[m][n][3] = fmaf(m1, sx.y, acc[m][n][3]);
+                            } else {
+                                acc[m][n][0] = fmaf(m0, sx.x, acc[m][n][0]);
+                                acc[m][n][1] = fmaf(m1, sx.x, acc[m][n][1]);
+                            }
                         }
                     }
                 }
             }
         }
-    }
-    cp_async_wait<0>();
-    __syncthreads();
-    // parts [WK][TOK][rows + 8] over the stages
-    const int rows = tiles * 16, ld = rows + 8, part = TOK * ld;
-    float *mine = reinterpret_cast<float *>(smem) + wk * part;
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const int r = (2 * wm + m) * 16 + g, nn = wn * NB + n;
-            if constexpr (XB) {
-                const int t = 8 * nn + 2 * q;
-                mine[t * ld + r] = acc[m][n][0];
-                mine[(t + 1) * ld + r] = acc[m][n][1];
-                mine[t * ld + r + 8] = acc[m][n][2];
-                mine[(t + 1) * ld + r + 8] = acc[m][n][3];
-            } else {
-                const int t = 4 * nn + q;
-                mine[t * ld + r] = acc[m][n][0];
-                mine[t * ld + r + 8] = acc[m][n][1];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[it % kGemmStages]);
+        // the first warp refills the stage of the step before, which the others have likely left by now
+        if (tid == 0 && it > 0 && copied < iters && ok) {
+            ok = mbar_wait(&empty[(it - 1) % kGemmStages], (uint32_t)((it - 1) / kGemmStages & 1), a.err);
+            if (ok) {
+                copy_codes(copied);
+                copy_frags(copied);
+                ++copied;
             }
         }
+    }
+    if (!__syncthreads_and(ok) && tid == 0)  // no copy may outlive the CTA
+        for (int it = copied > kGemmStages ? copied - kGemmStages : 0; it < copied; ++it)
+            mbar_wait(&bars[it % kGemmStages], (uint32_t)(it / kGemmStages & 1), nullptr);
+    __syncthreads();
+    // parts [WK][TOK][rows + 8] over the stages
+    const int rows = MT * p.WM * 16, ld = rows + 8, part = TOK * ld;
+    float *mine = reinterpret_cast<float *>(smem) + wk * part;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const int t = XB ? 8 * n + 2 * q : 4 * n + q;
+        const float i0 = inv[t], i1 = XB ? inv[t + 1] : 0.f;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const int r = (wm * MT + m) * 16 + g;
+            if constexpr (XB) {
+                mine[t * ld + r] = acc[m][n][0] * i0;
+                mine[(t + 1) * ld + r] = acc[m][n][1] * i1;
+                mine[t * ld + r + 8] = acc[m][n][2] * i0;
+                mine[(t + 1) * ld + r + 8] = acc[m][n][3] * i1;
+            } else {
+                mine[t * ld + r] = acc[m][n][0] * i0;
+                mine[t * ld + r + 8] = acc[m][n][1] * i0;
+            }
+        }
+    }
     if (p.S > 1) cluster_sync_all();
     else __syncthreads();
-    // the CTAs of a cluster share the sums out by tokens
+    // the CTAs of a cluster share the sums out, four rows of a token to a thread
     const float *all = reinterpret_cast<const float *>(smem);
-    for (int i = rank * nthr + tid; i < a.n_tok * rows; i += p.S * nthr) {
-        const int t = i / rows, r = i - t * rows, row = rt0 * 16 + r;
+    for (int i = rank * kGemmWarps * 32 + tid; i < a.n_tok * rows / 4; i += p.S * kGemmWarps * 32) {
+        const int t = i / (rows / 4), r = (i - t * (rows / 4)) * 4, row = rt0 * 16 + r;
         if (row >= a.rows) continue;
-        float s = 0.f;
-        for (int c = 0; c < p.S; ++c)
-            for (int k = 0; k < p.WK; ++k) {
-                const float *at = all + k * part + t * ld + r;
-                s += p.S > 1 ? ld_cluster(at, (uint32_t)c) : *at;
-            }
-        store_act(a.y, a.y_bf16, (size_t)t * a.ldy + row, s * reinterpret_cast<const float *>(ws)[t]);
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < p.WK; ++k) {
+            const float *at = all + k * part + t * ld + r;
+            float4 v[8];  // all parts on their way before the first is added
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                if (c < p.S) v[c] = p.S > 1 ? ld_cluster4(at, (uint32_t)c) : *reinterpret_cast<const float4 *>(at);
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                if (c < p.S) {
+                    s.x += v[c].x;
+                    s.y += v[c].y;
+                    s.z += v[c].z;
+                    s.w += v[c].w;
+                }
+        }
+        const size_t o = (size_t)t * a.ldy + row;
+        const float out[4] = {s.x, s.y, s.z, s.w};
+        for (int k = 0; k < 4 && row + k < a.rows; ++k) store_act(a.y, a.y_bf16, o + k, out[k]);
     }
     if (p.S > 1) cluster_sync_all();  // no CTA leaves while its parts are read
 }
 
-template <uint32_t TYPE, bool XB, int NB>
-cudaError_t launch_gemm_nb(const Q4Args &a, uint8_t *ws, GemmPlan p, int sm_count, cudaStream_t s) {
-    const int COLS = p.WN * NB * 8, TOK = XB ? COLS : COLS / 2;
-    const int bunit = COLS * 256 + TOK * 16;
-    auto ctas = [&] { return (p.RT + 2 * p.WM - 1) / (2 * p.WM); };
-    p.WM = p.WN == 1 ? 8 : 4;
-    p.WK = 1;
-    p.S = 1;
-    while (p.S < 8 && ctas() * p.S < sm_count * 3 / 2 && p.KT >= 4 * p.S) p.S *= 2;
-    auto ring = [&](int wm, int wk) { return kGemmStages * wk * (bunit + 2 * wm * unit_bytes(TYPE)); };
-    while (p.WM > 1 && ctas() * p.S < sm_count && p.KT >= 4 * p.S * p.WK && ring(p.WM / 2, p.WK * 2) <= kMaxSmem) {
+template <uint32_t TYPE, bool XB, int NB, int MT>
+cudaError_t launch_gemm_mt(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s) {
+    constexpr int COLS = 8 * NB, TOK = XB ? COLS : COLS / 2, BU = COLS * 256 + TOK * 16;
+    GemmPlan p{};
+    p.RT = (a.rows + kTileRows - 1) / kTileRows;
+    p.KT = (a.cols + kUnitCols - 1) / kUnitCols;
+    p.WM = kGemmWarps;
+    p.WK = p.S = 1;
+    // CTAs for one and a half on every SM: first the CTAs of a cluster split the units (down to two units
+    // a CTA), then fewer row tiles and more splits in a CTA.
+    auto ctas = [&] { return (p.RT + MT * p.WM - 1) / (MT * p.WM) * p.S; };
+    auto ring = [&](int wm, int wk) { return gemm_stages(MT) * wk * (BU + MT * wm * unit_bytes(TYPE)); };
+    while (p.S < 8 && ctas() < sm_count * 3 / 2 && p.KT >= 4 * p.S) p.S *= 2;
+    while (p.WM > 1 && ctas() < sm_count * 3 / 2 && p.KT >= 4 * p.S * p.WK && ring(p.WM / 2, p.WK * 2) <= kMaxSmem / 2) {
         p.WM /= 2;
         p.WK *= 2;
     }
-    const int parts = p.WK * TOK * (2 * p.WM * 16 + 8) * 4;
+    const int parts = p.WK * TOK * (MT * p.WM * 16 + 8) * 4;
     const int smem = ring(p.WM, p.WK) > parts ? ring(p.WM, p.WK) : parts;
-    if (smem > kMaxSmem) return cudaErrorInvalidValue;
-    const size_t esz = XB ? 2 : 4;
-    p.vec = ((uintptr_t)a.x & 15) == 0 && (a.ldx * esz) % 16 == 0;
+    if (smem > kMaxSmem - kStaticSmem) return cudaErrorInvalidValue;
+    p.vec = ((uintptr_t)a.x & 15) == 0 && a.ldx * (XB ? 2 : 4) % 16 == 0;
     cudaError_t e = launch_chain_pdl(true, q4_pack_kernel<TYPE, XB>, dim3((unsigned)a.n_tok), dim3(kPackThreads), 0, s, a, ws,
                                      p.KT, COLS, p.vec);
     if (e != cudaSuccess) return e;
-    auto *k = q4_gemm_kernel<TYPE, XB, NB>;
-    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    auto *k = q4_gemm_kernel<TYPE, XB, NB, MT>;
+    static SmemLimit limit;
+    e = limit.raise(k);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(ctas() * p.S));
-    cfg.blockDim = dim3((unsigned)(p.WM * p.WN * p.WK * 32));
+    cfg.gridDim = dim3((unsigned)ctas());
+    cfg.blockDim = dim3(kGemmWarps * 32);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -977,21 +1026,25 @@ cudaError_t launch_gemm_nb(const Q4Args &a, uint8_t *ws, GemmPlan p, int sm_coun
     return cudaLaunchKernelEx(&cfg, k, a, (const uint8_t *)ws, p);
 }
 
-template <uint32_t TYPE, bool XB>
+template <uint32_t TYPE, bool XB, int NB>
 cudaError_t launch_gemm(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s) {
-    GemmPlan p{};
-    p.RT = (a.rows + kTileRows - 1) / kTileRows;
-    p.KT = (a.cols + kUnitCols - 1) / kUnitCols;
-    const int t8 = ((XB ? a.n_tok : 2 * a.n_tok) + 7) / 8;
-    p.WN = (t8 + 3) / 4;
-    return (t8 + p.WN - 1) / p.WN <= 3 ? launch_gemm_nb<TYPE, XB, 3>(a, ws, p, sm_count, s)
-                                       : launch_gemm_nb<TYPE, XB, 4>(a, ws, p, sm_count, s);
+    return a.rows >= 4096 ? launch_gemm_mt<TYPE, XB, NB, 2>(a, ws, sm_count, s)
+                          : launch_gemm_mt<TYPE, XB, NB, 1>(a, ws, sm_count, s);
 }
 
 template <uint32_t TYPE, bool XB>
 cudaError_t launch_tokens(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s) {
     constexpr int T1 = XB ? 8 : 4;
-    if (a.n_tok > 2 * T1) return launch_gemm<TYPE, XB>(a, ws, sm_count, s);
+    if (a.n_tok > 2 * T1) {  // up to 64 tokens: 8 product tiles in bf16, 16 in f32
+        const int tiles = (a.n_tok + T1 - 1) / T1;
+        if (tiles <= 4) return launch_gemm<TYPE, XB, 4>(a, ws, sm_count, s);
+        if (tiles <= 6) return launch_gemm<TYPE, XB, 6>(a, ws, sm_count, s);
+        if (tiles <= 8) return launch_gemm<TYPE, XB, 8>(a, ws, sm_count, s);
+        if constexpr (!XB) {
+            if (tiles <= 12) return launch_gemm<TYPE, XB, 12>(a, ws, sm_count, s);
+            return launch_gemm<TYPE, XB, 16>(a, ws, sm_count, s);
+        }
+    }
     // 16 columns where their activations fit the cluster's shared memory, else 8 at a time
     const int KT = (a.cols + kUnitCols - 1) / kUnitCols;
     const int most = ((KT + 7) / 8) * Halves<TYPE, XB, 16>::BYTES <= 160 * 1024 ? 2 * T1 : T1;

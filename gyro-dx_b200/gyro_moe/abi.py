@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -147,9 +148,9 @@ SIGNATURES = {
     "gx_upload_matrix": [_P, _U32, _U32, _U32, _P, _U64, ctypes.POINTER(_U32), _U32],
     "gx_matvec": [_P, _U32, _P, _U32, _P, ctypes.POINTER(_U64)],
     "gx_linear": [_P, _U32, _P, _U32, _U64, _U32, _P, _U32, _U64, ctypes.POINTER(_U64)],
-    "gx_norm": [_P, ctypes.POINTER(NormDesc), _U32, ctypes.POINTER(_U64)],
-    "gx_norm_residual": [_P, ctypes.POINTER(ResidualDesc), _U32, ctypes.POINTER(_U64)],
-    "gx_logprobs": [_P, ctypes.POINTER(LogprobsDesc), _U32, ctypes.POINTER(_U64)],
+    "gx_norm": [_P, _P, _U32, ctypes.POINTER(_U64)],
+    "gx_norm_residual": [_P, _P, _U32, ctypes.POINTER(_U64)],
+    "gx_logprobs": [_P, _P, _U32, ctypes.POINTER(_U64)],
     "gx_upload_norms": [_P, _U32, ctypes.POINTER(NormsDesc), _U32],
     "gx_norm_block": [_P, _U32, _U32, _P, _U32, ctypes.POINTER(_U64)],
     "gx_read_timings": [_P, ctypes.POINTER(Timings)],
@@ -223,31 +224,52 @@ def unique_id() -> bytes:
     return buf.raw
 
 
-def _rows(a, width: int | None = None) -> tuple[int, int, int]:
-    """(pointer, row stride in elements, dtype code) of a device tensor of rows (1-D: one row)."""
-    if a.ndim not in (1, 2) or a.stride(-1) != 1 and a.shape[-1] > 1:
-        raise ValueError("rows must be contiguous, in a tensor of one or two dimensions")
-    w = a.shape[-1]
-    if width is not None and w != width:
-        raise ValueError(f"rows of {w} values where {width} are needed")
-    n = a.shape[0] if a.ndim == 2 else 1
-    return a.data_ptr(), (a.stride(0) if n > 1 else w), _dtype_code(a)
+def _packer(desc):
+    """struct.Struct of a descriptor's fields: packing one costs a third of filling the ctypes structure."""
+    codes = {ctypes.c_void_p: "Q", ctypes.c_uint64: "Q", ctypes.c_uint32: "I", ctypes.c_float: "f"}
+    p = struct.Struct("=" + "".join(codes[t] for _, t in desc._fields_))
+    assert p.size == ctypes.sizeof(desc)
+    return p.pack
 
 
-def _n_rows(a) -> int:
-    return a.shape[0] if a.ndim == 2 else 1
+_PACK_NORM, _PACK_RESIDUAL, _PACK_LOGPROBS = _packer(NormDesc), _packer(ResidualDesc), _packer(LogprobsDesc)
+_CODES: dict = {}                # dtype -> encoding, of the dtypes seen
 
 
-def _words(a, n: int, what: str, dtypes=("float32",)) -> int | None:
-    """Pointer of a contiguous device vector of n 32-bit words, or None."""
+def _rows(a) -> tuple[int, int, int, int, int]:
+    """(rows, width, pointer, row stride in elements, encoding) of a device tensor of rows (1-D: one row)."""
+    shape, stride = a.shape, a.stride()
+    if len(shape) == 2:
+        n, w = shape
+        s = stride[0] if n > 1 else w
+    elif len(shape) == 1:
+        n, w = 1, shape[0]
+        s = w
+    else:
+        raise ValueError("rows must lie in a tensor of one or two dimensions")
+    if stride[-1] != 1 and w > 1:
+        raise ValueError("rows must be contiguous")
+    dt = a.dtype
+    code = _CODES.get(dt)
+    if code is None:
+        code = _CODES[dt] = _dtype_code(a)
+    return n, w, a.data_ptr(), s, code
+
+
+_WORDS: dict = {}                # dtype -> whether it is f32 (True) or a 32-bit integer (False)
+
+
+def _words(a, n: int, what: str, floats: bool = True) -> int:
+    """Pointer of a contiguous device vector of n 32-bit words (floats or integers); 0 for None."""
     if a is None:
-        return None
-    if a.numel() != n or not a.is_contiguous() or str(a.dtype).removeprefix("torch.") not in dtypes:
-        raise ValueError(f"{what}: {n} contiguous values of type {' or '.join(dtypes)} are needed")
+        return 0
+    dt = a.dtype
+    kind = _WORDS.get(dt)
+    if kind is None:
+        kind = _WORDS[dt] = {"float32": True, "int32": False, "uint32": False}.get(str(dt).removeprefix("torch."), str(dt))
+    if kind is not floats or a.numel() != n or not a.is_contiguous():
+        raise ValueError(f"{what}: {n} contiguous values of type {'f32' if floats else '32-bit integer'} are needed")
     return a.data_ptr()
-
-
-_IDS = ("int32", "uint32")
 
 
 class Context:
@@ -265,6 +287,8 @@ class Context:
         h = ctypes.c_void_p()
         _check(self.lib.gx_create(ctypes.byref(opts), ctypes.byref(h)), "gx_create")
         self.handle = h
+        self._ticket = ctypes.c_uint64()                 # of the operator calls (one thread uses a context)
+        self._ticket_ref = ctypes.byref(self._ticket)
         self.max_tokens = max_tokens
         self.layers: dict[int, dict] = {}
         self.matrices: dict[int, tuple[int, int]] = {}   # (rows, cols) by handle
@@ -454,33 +478,29 @@ class Context:
     # --- operators around the layer ----------------------------------------------------------
     # Device tensors of this context's device, rows in the last dimension; the work is enqueued on the
     # context's stream. Each returns the ticket, or 0 with ticket=False (calls captured into a graph).
-    def _call(self, name: str, *args, ticket: bool = True) -> int:
-        t = ctypes.c_uint64() if ticket else None
-        rc = getattr(self.lib, name)(self.handle, *args, ctypes.byref(t) if ticket else None)
+    def _done(self, rc: int, call: str, ticket: bool) -> int:
         if rc != GX_OK:
-            raise GxError(rc, name)
-        return t.value if ticket else 0
+            raise GxError(rc, call)
+        return self._ticket.value if ticket else 0
 
     def linear(self, handle: int, x, y, ticket: bool = True) -> int:
         """gx_linear: y = W x for a 4-bit matrix, x [n, cols] and y [n, rows] in f32 or bf16, n <= 64."""
-        xp, xs, xd = _rows(x)
-        yp, ys, yd = _rows(y)
-        n = _n_rows(x)
-        rows, cols = self.matrices[handle]
-        if _n_rows(y) != n or x.shape[-1] != cols or y.shape[-1] != rows:
+        n, cols, xp, xs, xd = _rows(x)
+        m, rows, yp, ys, yd = _rows(y)
+        if n != m or (rows, cols) != self.matrices[handle]:
             raise ValueError("gx_linear: x [n, cols] and y [n, rows] are needed")
-        return self._call("gx_linear", handle, xp, xd, xs, n, yp, yd, ys, ticket=ticket)
+        return self._done(self.lib.gx_linear(self.handle, handle, xp, xd, xs, n, yp, yd, ys,
+                                             self._ticket_ref if ticket else None), "gx_linear", ticket)
 
     def norm(self, x, y, weight=None, eps: float = 1e-6, gate_weight=None, gate=None, ticket: bool = True) -> int:
         """gx_norm: y = norm(x) * weight, and gate = gate_weight . y for each row."""
-        n, w = _n_rows(x), x.shape[-1]
-        xp, xs, xd = _rows(x)
-        yp, ys, yd = _rows(y, w)
-        if _n_rows(y) != n:
-            raise ValueError("gx_norm: as many rows in y as in x are needed")
-        d = NormDesc(xp, yp, _words(weight, w, "weight"), _words(gate_weight, w, "gate_weight"), _words(gate, n, "gate"),
-                     xs, ys, xd, yd, w, eps)
-        return self._call("gx_norm", ctypes.byref(d), n, ticket=ticket)
+        n, w, xp, xs, xd = _rows(x)
+        m, v, yp, ys, yd = _rows(y)
+        if n != m or v != w:
+            raise ValueError("gx_norm: x and y of one shape are needed")
+        d = _PACK_NORM(xp, yp, _words(weight, w, "weight"), _words(gate_weight, w, "gate_weight"), _words(gate, n, "gate"),
+                       xs, ys, xd, yd, w, eps)
+        return self._done(self.lib.gx_norm(self.handle, d, n, self._ticket_ref if ticket else None), "gx_norm", ticket)
 
     def norm_residual(self, y, res, res_out=None, post=None, post_norm: bool = True, eps: float = 1e-6,
                       res_scale: float = 1.0, block_scale: float = 1.0, gate=None, out=None, next_weight=None,
@@ -488,37 +508,37 @@ class Context:
         """gx_norm_residual: res_out = res_scale * res + block_scale * gate * norm(y; post) (y itself
         without post_norm), out = norm(res_out; next_weight). res_out None: res in place. gate: one f32
         logit per row (1-D) or one logit per element (2-D)."""
-        n, w = _n_rows(y), y.shape[-1]
-        yp, ys, yd = _rows(y)
-        rp, rs, rd = _rows(res, w)
-        op, os_, od = _rows(res_out, w) if res_out is not None else (rp, rs, rd)
-        gp, gs, gd, kind = None, 0, GX_F32, GX_GATE_NONE
+        n, w, yp, ys, yd = _rows(y)
+        rn, rw, rp, rs, rd = _rows(res)
+        on, ow, op, os_, od = _rows(res_out) if res_out is not None else (rn, rw, rp, rs, rd)
+        gn, gw, gp, gs, gd, kind = n, w, 0, 0, GX_F32, GX_GATE_NONE
         if gate is not None and gate.ndim == 1:
             gp, kind = _words(gate, n, "gate"), GX_GATE_TOKEN
         elif gate is not None:
-            (gp, gs, gd), kind = _rows(gate, w), GX_GATE_ELEMENT
-        hp, hs, hd = _rows(out, w) if out is not None else (None, 0, GX_F32)
-        if od != rd or any(_n_rows(a) != n for a in (res, res_out, out, gate if kind == GX_GATE_ELEMENT else None)
-                           if a is not None):
-            raise ValueError("gx_norm_residual: equal numbers of rows, and res_out in the type of res, are needed")
-        d = ResidualDesc(yp, rp, op, gp, _words(post, w, "post"), hp, _words(next_weight, w, "next_weight"),
-                         _words(next_gate_weight, w, "next_gate_weight"), _words(next_gate, n, "next_gate"),
-                         ys, rs, os_, gs, hs, yd, rd, gd, hd, w, GX_RES_POST_NORM if post_norm else 0, kind,
-                         eps, res_scale, block_scale)
-        return self._call("gx_norm_residual", ctypes.byref(d), n, ticket=ticket)
+            (gn, gw, gp, gs, gd), kind = _rows(gate), GX_GATE_ELEMENT
+        hn, hw, hp, hs, hd = _rows(out) if out is not None else (n, w, 0, 0, GX_F32)
+        if not (n == rn == on == gn == hn and w == rw == ow == gw == hw and od == rd):
+            raise ValueError("gx_norm_residual: rows of one shape, and res_out in the type of res, are needed")
+        d = _PACK_RESIDUAL(yp, rp, op, gp, _words(post, w, "post"), hp, _words(next_weight, w, "next_weight"),
+                           _words(next_gate_weight, w, "next_gate_weight"), _words(next_gate, n, "next_gate"),
+                           ys, rs, os_, gs, hs, yd, rd, gd, hd, w, GX_RES_POST_NORM if post_norm else 0, kind,
+                           eps, res_scale, block_scale)
+        return self._done(self.lib.gx_norm_residual(self.handle, d, n, self._ticket_ref if ticket else None),
+                          "gx_norm_residual", ticket)
 
     def logprobs(self, logits, tokens=None, n_top: int = 0, scale: float = 1.0, logprob=None, rank=None, entropy=None,
                  top_ids=None, top_logprobs=None, ticket: bool = True) -> int:
         """gx_logprobs over rows of logits [n, vocab]; tokens, rank and top_ids are 32-bit integers."""
-        n, v = _n_rows(logits), logits.shape[-1]
-        p, s, dt = _rows(logits)
-        d = LogprobsDesc(p, _words(tokens, n, "tokens", _IDS), _words(logprob, n, "logprob"),
-                         _words(rank, n, "rank", _IDS), _words(entropy, n, "entropy"),
-                         _words(top_ids, n * n_top, "top_ids", _IDS) if n_top or top_ids is not None and top_ids.numel() else None,
-                         _words(top_logprobs, n * n_top, "top_logprobs")
-                         if n_top or top_logprobs is not None and top_logprobs.numel() else None,
-                         s, dt, v, n_top, scale)
-        return self._call("gx_logprobs", ctypes.byref(d), n, ticket=ticket)
+        n, v, p, s, dt = _rows(logits)
+        if not n_top:       # empty outputs stand for none
+            top_ids = None if top_ids is not None and top_ids.numel() == 0 else top_ids
+            top_logprobs = None if top_logprobs is not None and top_logprobs.numel() == 0 else top_logprobs
+        d = _PACK_LOGPROBS(p, _words(tokens, n, "tokens", False), _words(logprob, n, "logprob"),
+                           _words(rank, n, "rank", False), _words(entropy, n, "entropy"),
+                           _words(top_ids, n * n_top, "top_ids", False), _words(top_logprobs, n * n_top, "top_logprobs"),
+                           s, dt, v, n_top, scale)
+        return self._done(self.lib.gx_logprobs(self.handle, d, n, self._ticket_ref if ticket else None), "gx_logprobs",
+                          ticket)
 
     def upload_norms(self, index: int, norms: dict | None, timeout_ms: int = 600000) -> None:
         """gx_upload_norms: pre, post and gate weights ([n_embd] f32 or None), post_norm, eps, res_scale and
