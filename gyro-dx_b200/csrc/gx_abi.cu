@@ -370,6 +370,17 @@ void release_all(gx_context *c) {
 
 using gx::dtype_size;
 
+// Room for one more element, so that adding it throws nothing through the C interface.
+template <typename T>
+bool reserve_one(std::vector<T> &v) {
+    try {
+        if (v.size() == v.capacity()) v.reserve(v.size() * 2 + 8);
+    } catch (...) {
+        return false;
+    }
+    return true;
+}
+
 // Phase event: a plain record on the stream, or an event-record node (external record) while
 // the stream is being captured into a graph (a plain record there only orders graph nodes).
 cudaError_t record_phase(cudaEvent_t ev, cudaStream_t s) {
@@ -2365,8 +2376,10 @@ GX_API gx_result gx_upload_matrix(gx_context *c, uint32_t type_id, uint32_t rows
     // the GEMV takes rows 16 at a time: an odd count of 8-row groups gets a zero group after it
     const uint64_t pad = !q4 && rows % 16 ? (uint64_t)gx::tile_bytes(type_id) * (cols / 128) : 0;
     const uint64_t bytes = q4 ? gx::q4_bytes(type_id, rows, cols) : packed_bytes + pad;
+    if (!reserve_one(c->mats)) return GX_E_OUTOFMEMORY;
     if (q4 && cols > c->q4_ws_cols) {
         uint8_t *ws = nullptr;
+        if (!reserve_one(c->q4_ws)) return GX_E_OUTOFMEMORY;
         GX_CUDA(cudaMalloc(&ws, gx::q4_workspace_bytes(cols)));
         c->q4_ws.push_back(ws);
         c->q4_ws_cols = cols;

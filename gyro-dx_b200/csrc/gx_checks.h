@@ -14,6 +14,7 @@ namespace gx {
 // Limits (include/gyro_moe.h).
 constexpr uint32_t kQ4MaxCols = 65536, kQ4MaxRows = 1u << 24, kLinearMaxTokens = 64;
 constexpr uint32_t kNormMaxWidth = 65536, kMaxVocab = 524288, kMaxRows = 1u << 24;
+constexpr float kMaxScale = 1e30f;           // scale * log2 e and its double stay finite
 constexpr uint64_t kMaxStride = 1ull << 32;  // elements: the bytes of kMaxRows rows stay below 2^63
 
 inline size_t dtype_size(uint32_t dt) { return dt == GX_BF16 ? 2 : 4; }
@@ -119,7 +120,7 @@ inline bool residual_args_ok(const gx_residual_desc &d, uint32_t n_tok) {
 
 inline bool logprobs_args_ok(const gx_logprobs_desc &d, uint32_t n_rows) {
     if (d.n_vocab == 0 || d.n_vocab > kMaxVocab || d.n_top > GX_MAX_TOP || d.n_top > d.n_vocab ||
-        n_rows > kMaxRows || !(d.scale > 0.f) || !std::isfinite(d.scale) || !act_dtype(d.dtype))
+        n_rows > kMaxRows || !(d.scale > 0.f) || !(d.scale <= kMaxScale) || !act_dtype(d.dtype))
         return false;
     if ((!d.tokens && (d.logprob || d.rank)) || (!d.n_top && (d.top_ids || d.top_logprobs)) || !words_ok(d.tokens) ||
         !words_ok(d.logprob) || !words_ok(d.rank) || !words_ok(d.entropy) || !words_ok(d.top_ids) ||

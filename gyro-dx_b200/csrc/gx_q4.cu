@@ -794,6 +794,14 @@ __global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(Q4Args a, uint8_t
 constexpr int kGemmWarps = 8;
 constexpr int gemm_stages(int MT) { return MT == 2 ? 3 : 2; }
 
+// acc += d * c, both halves in one instruction.
+__device__ __forceinline__ void fma2(float2 &acc, float d, float2 c) {
+    asm("{\n.reg .b64 a, b, d;\n"
+        "mov.b64 a, {%0, %1};\nmov.b64 d, {%2, %2};\nmov.b64 b, {%3, %4};\n"
+        "fma.rn.f32x2 a, d, b, a;\nmov.b64 {%0, %1}, a;\n}"
+        : "+f"(acc.x), "+f"(acc.y)
+        : "f"(d), "f"(c.x), "f"(c.y));
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -804,7 +812,7 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
 // cluster's CTAs at the end.
 template <uint32_t TYPE, bool XB, int NB, int MT>
 __global__ void __launch_bounds__(kGemmWarps * 32, 2) q4_gemm_kernel(Q4Args a, const uint8_t *ws, GemmPlan p) {
-    constexpr int NA = XB ? 4 : 2, UB = unit_bytes(TYPE), COLS = 8 * NB, TOK = XB ? COLS : COLS / 2;
+    constexpr int UB = unit_bytes(TYPE), COLS = 8 * NB, TOK = XB ? COLS : COLS / 2;
     constexpr int BU = COLS * 256 + TOK * 16;  // a unit's fragments and sums
     constexpr int kGemmStages = gemm_stages(MT);
     extern __shared__ __align__(16) uint8_t smem[];
@@ -849,13 +857,12 @@ __global__ void __launch_bounds__(kGemmWarps * 32, 2) q4_gemm_kernel(Q4Args a, c
         for (int i = 0; i < kGemmStages && i < iters; ++i) copy_frags(i);
     if (tid < 64) inv[tid] = tid < a.n_tok ? reinterpret_cast<const float *>(ws)[tid] : 0.f;
 
-    float acc[MT][NB][NA];
+    // sums of (row g; row g + 8) of columns 2 q and 2 q + 1: two tokens in bf16, the parts of one in f32
+    float2 acc[MT][NB][2];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int k = 0; k < NA; ++k) acc[m][n][k] = 0.f;
+        for (int n = 0; n < NB; ++n) acc[m][n][0] = acc[m][n][1] = make_float2(0.f, 0.f);
     bool ok = true;  // an expired wait is reported and ends the warp's loop
     int copied = min(iters, kGemmStages);
     for (int it = 0; it < iters; ++it) {
@@ -890,26 +897,11 @@ __global__ void __launch_bounds__(kGemmWarps * 32, 2) q4_gemm_kernel(Q4Args a, c
                     for (int m = 0; m < MT; ++m) {
                         float c[4];
                         mma_group(c, a0[m], a1[m], b);
-                        if constexpr (XB) {
-                            acc[m][n][0] = fmaf(d0[m], c[0], acc[m][n][0]);
-                            acc[m][n][1] = fmaf(d0[m], c[1], acc[m][n][1]);
-                            acc[m][n][2] = fmaf(d1[m], c[2], acc[m][n][2]);
-                            acc[m][n][3] = fmaf(d1[m], c[3], acc[m][n][3]);
-                        } else {
-                            acc[m][n][0] = fmaf(d0[m], c[0] + c[1], acc[m][n][0]);
-                            acc[m][n][1] = fmaf(d1[m], c[2] + c[3], acc[m][n][1]);
-                        }
+                        fma2(acc[m][n][0], d0[m], make_float2(c[0], c[1]));
+                        fma2(acc[m][n][1], d1[m], make_float2(c[2], c[3]));
                         if constexpr (TYPE == GX_Q4_1) {
-                            const float m0 = half_value(mw[m], 0), m1 = half_value(mw[m], 1);
-                            if constexpr (XB) {
-                                acc[m][n][0] = fmaf(m0, sx.x, acc[m][n][0]);
-                                acc[m][n][1] = fmaf(m0, sx.y, acc[m][n][1]);
-                                acc[m][n][2] = fmaf(m1, sx.x, acc[m][n][2]);
-                                acc[m][n][3] = fmaf(m1, sx.y, acc[m][n][3]);
-                            } else {
-                                acc[m][n][0] = fmaf(m0, sx.x, acc[m][n][0]);
-                                acc[m][n][1] = fmaf(m1, sx.x, acc[m][n][1]);
-                            }
+                            fma2(acc[m][n][0], half_value(mw[m], 0), sx);
+                            fma2(acc[m][n][1], half_value(mw[m], 1), sx);
                         }
                     }
                 }
@@ -942,13 +934,13 @@ __global__ void __launch_bounds__(kGemmWarps * 32, 2) q4_gemm_kernel(Q4Args a, c
         for (int m = 0; m < MT; ++m) {
             const int r = (wm * MT + m) * 16 + g;
             if constexpr (XB) {
-                mine[t * ld + r] = acc[m][n][0] * i0;
-                mine[(t + 1) * ld + r] = acc[m][n][1] * i1;
-                mine[t * ld + r + 8] = acc[m][n][2] * i0;
-                mine[(t + 1) * ld + r + 8] = acc[m][n][3] * i1;
+                mine[t * ld + r] = acc[m][n][0].x * i0;
+                mine[(t + 1) * ld + r] = acc[m][n][0].y * i1;
+                mine[t * ld + r + 8] = acc[m][n][1].x * i0;
+                mine[(t + 1) * ld + r + 8] = acc[m][n][1].y * i1;
             } else {
-                mine[t * ld + r] = acc[m][n][0] * i0;
-                mine[t * ld + r + 8] = acc[m][n][1] * i0;
+                mine[t * ld + r] = (acc[m][n][0].x + acc[m][n][0].y) * i0;
+                mine[t * ld + r + 8] = (acc[m][n][1].x + acc[m][n][1].y) * i0;
             }
         }
     }
@@ -1028,8 +1020,10 @@ cudaError_t launch_gemm_mt(const Q4Args &a, uint8_t *ws, int sm_count, cudaStrea
 
 template <uint32_t TYPE, bool XB, int NB>
 cudaError_t launch_gemm(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s) {
-    return a.rows >= 4096 ? launch_gemm_mt<TYPE, XB, NB, 2>(a, ws, sm_count, s)
-                          : launch_gemm_mt<TYPE, XB, NB, 1>(a, ws, sm_count, s);
+    if constexpr (NB <= 8) {  // two row tiles by more columns do not fit the registers
+        if (a.rows >= 4096) return launch_gemm_mt<TYPE, XB, NB, 2>(a, ws, sm_count, s);
+    }
+    return launch_gemm_mt<TYPE, XB, NB, 1>(a, ws, sm_count, s);
 }
 
 template <uint32_t TYPE, bool XB>

@@ -287,6 +287,7 @@ class Context:
         h = ctypes.c_void_p()
         _check(self.lib.gx_create(ctypes.byref(opts), ctypes.byref(h)), "gx_create")
         self.handle = h
+        self.device = device
         self._ticket = ctypes.c_uint64()                 # of the operator calls (one thread uses a context)
         self._ticket_ref = ctypes.byref(self._ticket)
         self.max_tokens = max_tokens
@@ -478,6 +479,13 @@ class Context:
     # --- operators around the layer ----------------------------------------------------------
     # Device tensors of this context's device, rows in the last dimension; the work is enqueued on the
     # context's stream. Each returns the ticket, or 0 with ticket=False (calls captured into a graph).
+    def _here(self, *tensors) -> None:
+        """The tensors have to lie on this context's device: a kernel would fault on any other address."""
+        dev = self.device
+        for a in tensors:
+            if a is not None and a.get_device() != dev:
+                raise ValueError(f"a tensor does not lie on device {dev}")
+
     def _done(self, rc: int, call: str, ticket: bool) -> int:
         if rc != GX_OK:
             raise GxError(rc, call)
@@ -489,6 +497,7 @@ class Context:
         m, rows, yp, ys, yd = _rows(y)
         if n != m or (rows, cols) != self.matrices[handle]:
             raise ValueError("gx_linear: x [n, cols] and y [n, rows] are needed")
+        self._here(x, y)
         return self._done(self.lib.gx_linear(self.handle, handle, xp, xd, xs, n, yp, yd, ys,
                                              self._ticket_ref if ticket else None), "gx_linear", ticket)
 
@@ -500,6 +509,7 @@ class Context:
             raise ValueError("gx_norm: x and y of one shape are needed")
         d = _PACK_NORM(xp, yp, _words(weight, w, "weight"), _words(gate_weight, w, "gate_weight"), _words(gate, n, "gate"),
                        xs, ys, xd, yd, w, eps)
+        self._here(x, y, weight, gate_weight, gate)
         return self._done(self.lib.gx_norm(self.handle, d, n, self._ticket_ref if ticket else None), "gx_norm", ticket)
 
     def norm_residual(self, y, res, res_out=None, post=None, post_norm: bool = True, eps: float = 1e-6,
@@ -523,6 +533,7 @@ class Context:
                            _words(next_gate_weight, w, "next_gate_weight"), _words(next_gate, n, "next_gate"),
                            ys, rs, os_, gs, hs, yd, rd, gd, hd, w, GX_RES_POST_NORM if post_norm else 0, kind,
                            eps, res_scale, block_scale)
+        self._here(y, res, res_out, post, gate, out, next_weight, next_gate_weight, next_gate)
         return self._done(self.lib.gx_norm_residual(self.handle, d, n, self._ticket_ref if ticket else None),
                           "gx_norm_residual", ticket)
 
@@ -537,6 +548,7 @@ class Context:
                            _words(rank, n, "rank", False), _words(entropy, n, "entropy"),
                            _words(top_ids, n * n_top, "top_ids", False), _words(top_logprobs, n * n_top, "top_logprobs"),
                            s, dt, v, n_top, scale)
+        self._here(logits, tokens, logprob, rank, entropy, top_ids, top_logprobs)
         return self._done(self.lib.gx_logprobs(self.handle, d, n, self._ticket_ref if ticket else None), "gx_logprobs",
                           ticket)
 
@@ -558,7 +570,11 @@ class Context:
 
     def norm_block(self, first: int, n_layers: int, res) -> int:
         """gx_norm_block on a device f32 tensor res [n, n_embd], updated in place. Returns the ticket."""
+        n, w, p, s, code = _rows(res)
+        if s != w or code != GX_F32 or first not in self.layers or w != self.layers[first]["n_embd"]:
+            raise ValueError("gx_norm_block: contiguous f32 rows of the layers' width are needed")
+        self._here(res)
         t = ctypes.c_uint64()
-        _check(self.lib.gx_norm_block(self.handle, first, n_layers, _ptr(res), res.shape[0], ctypes.byref(t)),
+        _check(self.lib.gx_norm_block(self.handle, first, n_layers, p, n, ctypes.byref(t)),
                "gx_norm_block")
         return t.value

@@ -333,7 +333,9 @@ GX_API gx_result gx_matvec(gx_context *context, uint32_t handle, const float *x,
  * pointers are device pointers, all work is enqueued on the context's stream and completes with the
  * ticket (out_ticket may be NULL). gx_linear, gx_norm, gx_norm_residual and gx_logprobs allocate no
  * memory and do not wait, so they can be captured into a graph from that stream (with a NULL ticket:
- * a captured call has none, and one that asks for it gets GX_E_STATE). Row strides are in elements, at least
+ * a captured call has none, and one that asks for it gets GX_E_STATE). A captured gx_linear of more than
+ * 8 tokens packs its activations in a workspace that all calls of the context share: replay such a
+ * graph on the context's stream, or ordered against it and against other such graphs. Row strides are in elements, at least
  * the row's width, and pointers need only the alignment of their element type. An output may not
  * overlap an input or another output except where that is said; such calls are refused. Sums,
  * norms and softmax statistics are f32 or wider, each output is rounded once. */
@@ -413,7 +415,7 @@ typedef struct gx_logprobs_desc {
     uint32_t dtype;               /* GX_F32 or GX_BF16 */
     uint32_t n_vocab;             /* 1..524288 */
     uint32_t n_top;               /* 0..GX_MAX_TOP, at most n_vocab */
-    float scale;                  /* > 0, finite: 1 / temperature */
+    float scale;                  /* > 0, at most 1e30: 1 / temperature */
 } gx_logprobs_desc;               /* 80 bytes */
 GX_API gx_result gx_logprobs(gx_context *context, const gx_logprobs_desc *desc, uint32_t n_rows,
                              uint64_t *out_ticket);

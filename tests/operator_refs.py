@@ -146,7 +146,8 @@ def logprobs(x, tokens, n_top, scale):
     xt = x[rows, tok][:, None]
     above = np.where(np.isnan(xt), ~np.isnan(x), x > xt).sum(1)
     # an f32 result past the largest f32 by more than half its step is an infinity (round to nearest)
-    lp = np.where(np.isfinite(lp) & (np.abs(lp) >= 2.0 ** 128 - 2.0 ** 103), np.sign(lp) * np.inf, lp)
+    far = np.isfinite(lp) & (np.abs(lp) >= 2.0 ** 128 - 2.0 ** 103)
+    lp = np.where(far, np.where(lp < 0, -np.inf, np.inf), lp)
     logprob = np.where(given, lp[rows, tok], np.where(tokens == 0xFFFFFFFF, 0.0, np.nan))
     top_lp = np.take_along_axis(lp, top, 1)
     values = {"logprob": logprob, "entropy": ent, "rank": np.where(given, above + 1, 0), "top_ids": top,

@@ -326,8 +326,13 @@ def test_norm_long_batches(ctx, width, n):
         x = refs.to_kind(rng.standard_normal((n, width), np.float32), xk)
         y, buf = out_rows(n, width, yk, width + 8)
         ctx.wait(ctx.norm(dev(x, xk), y, None if weight is None else dev(weight)))
-        near(y, *refs.norm(x, weight, 1e-6, yk)[0])
+        want = refs.norm(x, weight, 1e-6, yk)[0]
+        near(y, *want)
         untouched(buf, n, width)
+        if xk == yk:
+            t = dev(x, xk)
+            ctx.wait(ctx.norm(t, t, None if weight is None else dev(weight)))
+            near(t, *want)
 
 
 @pytest.mark.parametrize("width,n", [(512, 7200), (2560, 1300), (4096, 700)])
@@ -505,6 +510,57 @@ def test_logprobs_refusals(ctx):
         with pytest.raises(abi.GxError) as e:
             ctx.logprobs(x, **bad)
         assert e.value.code == -1
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-3, 30.0, 1e20, 1e30])
+def test_logprobs_extreme_scales(ctx, scale):
+    """Temperatures from flat to a single token; ties of the largest share it."""
+    x, tok = logits(3, 5, 4001, "f32")
+    x[2, [9, 90, 900]] = 40.0
+    tok[:] = x.argmax(1)
+    assert check_logprobs(ctx, x, "f32", tok, 4, scale) is None
+
+
+def test_rows_far_apart(ctx):
+    """Rows whose byte offsets pass 32 bits."""
+    far = 1_200_000_000
+    buf = torch.empty(far + 8192, dtype=torch.float32, device="cuda")
+    rng = np.random.default_rng(0)
+
+    def rows(width, values=None):
+        v = buf.as_strided((2, width), (far, 1))
+        if values is not None:
+            v.copy_(torch.from_numpy(values))
+        return v
+
+    x = rng.normal(0, 1, (2, 2048)).astype(np.float32)
+    y = torch.empty(2, 2048, device="cuda")
+    src = rows(2048, x)
+    torch.cuda.synchronize()
+    ctx.wait(ctx.norm(src, y))
+    near(y, *refs.norm(x, None, 1e-6, "f32")[0])
+    ctx.wait(ctx.norm(src, src))
+    near(rows(2048), *refs.norm(x, None, 1e-6, "f32")[0])
+    z, tok = logits(1, 2, 8000, "f32")
+    src = rows(8000, z)
+    torch.cuda.synchronize()
+    lp = torch.empty(2, device="cuda")
+    ctx.wait(ctx.logprobs(src, torch.from_numpy(tok.view(np.int32)).cuda(), logprob=lp))
+    want, bounds = refs.logprobs(z, tok, 0, 1.0)
+    near(lp, want["logprob"], bounds["logprob"])
+    packed, w, mag = refs.q4_matrix(7, refs.Q4_0, 40, 2048)
+    h = ctx.upload_matrix(refs.Q4_0, 40, 2048, packed)
+    src = rows(2048, x)
+    y = torch.empty(2, 40, device="cuda")
+    torch.cuda.synchronize()
+    ctx.wait(ctx.linear(h, src, y))
+    near(y, *refs.linear(x, w, mag, "f32"))
+    out = buf[4096:].as_strided((2, 40), (far, 1))
+    ctx.wait(ctx.linear(h, dev(x), out))
+    near(out, *refs.linear(x, w, mag, "f32"))
+    check = buf.as_strided((2, 2048), (far, 1))
+    ctx.wait(ctx.norm_residual(dev(x), check, post_norm=False))
+    near(check, 2.0 * x.astype(np.float64), np.abs(x) * 2.0 ** -21)
 
 
 # ---- together ---------------------------------------------------------------------------------

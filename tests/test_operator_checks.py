@@ -116,6 +116,7 @@ def test_logprobs_rules(chk):
     assert not call(tokens=None) and not call(n_top=0) and not call(n_top=33) and not call(n_vocab=4)
     assert not call(n_vocab=0) and not call(n_vocab=524289, stride=524289) and not call(stride=999)
     assert not call(scale=0.0) and not call(scale=-1.0) and not call(scale=math.inf) and not call(scale=math.nan)
+    assert call(scale=1e-40) and call(scale=1e29) and not call(scale=1e31)
     assert not call(dtype=8) and not call(logits=A + 2) and not call(logprob=C + 2)
     assert not call(logprob=A + 40) and not call(top_ids=E) and not call(entropy=C)
 
@@ -141,6 +142,7 @@ def test_binding_checks_shapes():
     """What the binding refuses before any call reaches the library."""
     ctx = abi.Context.__new__(abi.Context)
     ctx.handle, ctx.lib, ctx.matrices, ctx.layers = None, None, {0: (8, 64)}, {0: {"n_embd": 32}}
+    ctx.device = -1                     # where the host's tensors are, so that the shapes are what is refused
     f = torch.zeros
     bad = [lambda: ctx.linear(0, f(2, 64), f(3, 8)), lambda: ctx.linear(0, f(2, 32), f(2, 8)),
            lambda: ctx.linear(0, f(64, 2).T, f(2, 8)), lambda: ctx.linear(0, f(2, 64).half(), f(2, 8)),
@@ -152,11 +154,23 @@ def test_binding_checks_shapes():
            lambda: ctx.logprobs(f(2, 32), torch.zeros(3, dtype=torch.int32)),
            lambda: ctx.logprobs(f(2, 32), torch.zeros(2, dtype=torch.int64)),
            lambda: ctx.logprobs(f(2, 32), n_top=3, top_ids=torch.zeros(2, 2, dtype=torch.int32)),
-           lambda: ctx.upload_norms(0, {"pre": np.ones(31)})]
+           lambda: ctx.upload_norms(0, {"pre": np.ones(31)}), lambda: ctx.norm_block(0, 1, f(2, 31)),
+           lambda: ctx.norm_block(0, 1, f(2, 40)[:, :32]), lambda: ctx.norm_block(1, 1, f(2, 32))]
     for i, call in enumerate(bad):
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was taken")
+
+
+def test_binding_refuses_tensors_of_another_device():
+    ctx = abi.Context.__new__(abi.Context)
+    ctx.handle, ctx.lib, ctx.matrices, ctx.layers, ctx.device = None, None, {0: (8, 64)}, {0: {"n_embd": 32}}, 0
+    f = torch.zeros
+    for call in [lambda: ctx.linear(0, f(2, 64), f(2, 8)), lambda: ctx.norm(f(2, 32), f(2, 32)),
+                 lambda: ctx.norm_residual(f(2, 32), f(2, 32)), lambda: ctx.logprobs(f(2, 32)),
+                 lambda: ctx.norm_block(0, 1, f(2, 32))]:
+        with pytest.raises(ValueError, match="device"):
+            call()
 
 
 def test_references_agree_with_plain_loops():
