@@ -5,17 +5,15 @@
 //
 // with fp16 d and m per group and 4-bit q.
 //
-// The sums over a group run on the tensor cores (mma.sync m16n8k16, f32 accumulation) on the integers
-// q - 8 (Q4_1: q), which f16 holds exactly, and d meets the group's sum in f32, so no weight is ever
-// rounded. A code in the low bits of an f16 under the exponent of 1024 is 1024 + q, four bits higher
-// 1024 + 16 q: one shift, four and-ors and four half2 operations turn a word of 8 codes into its four
-// A registers. (Codes as f16 subnormals need no arithmetic at all, but the product then aligns its
-// terms by the subnormals' exponent and loses their leading zeros: 2e-6 to 4e-6 relative error
-// measured, against 1e-7.)
-//
-// Activations become f16 fragments in shared memory once per CTA: each unit of 128 columns of a token
-// is scaled by a power of two that brings its largest value to 2^14..2^15; an f32 value is split into
-// two f16 (22 bits, two columns of the product), a bf16 value fits one.
+// Up to 16 product columns are a GEMV, more a product on tcgen05 (each below). In the GEMV the sums over a
+// group run on mma.sync on the integers q - 8 (Q4_1: q), which f16 and 8-bit integers hold exactly, and d meets
+// the group's sum in f32, so no weight is ever rounded. A code in the low bits of an f16 under the exponent of
+// 1024 is 1024 + q, four bits higher 1024 + 16 q: one shift, four and-ors and four half2 operations turn a word
+// of 8 codes into its four A registers. (Codes as f16 subnormals need no arithmetic at all, but the product then
+// aligns its terms by the subnormals' exponent and loses their leading zeros: 2e-6 to 4e-6 relative error
+// measured, against 1e-7.) Its activations become fragments in shared memory once per CTA: each unit of 128
+// columns of a token is scaled by a power of two that brings its largest value to 2^14..2^15; an f32 value is
+// split into two f16 (22 bits, two columns of the product), a bf16 value fits one.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -26,6 +24,7 @@
 #include "gx_dense.cuh"
 #include "gx_device.cuh"
 #include "gx_internal.h"
+#include "gx_umma.cuh"
 
 namespace gx {
 
@@ -34,15 +33,19 @@ using namespace dense;
 namespace {
 
 // ---- device layout ---------------------------------------------------------------------------
-// Units of 16 rows x 128 columns (4 groups), ordered [row tile][unit]; rows and columns past the
-// matrix have zero scales. Lane l = 4 g + q of a warp owns rows g and g + 8 and, in each group, the
+// Units of 16 rows x 128 columns (4 groups), ordered [block of 8 row tiles][unit][row tile], so that one
+// bulk copy brings the codes of up to 128 rows; rows and columns past the matrix have zero scales. Lane l = 4 g + q of a warp owns rows g and g + 8 and, in each group, the
 // columns 8 q .. 8 q + 7, the k-slices its A registers hold:
 //   [32 lanes][4 groups] words of row g     code of column 8 q + i in bits 4 i .. 4 i + 3
 //   [32 lanes][4 groups] words of row g + 8
 //   [8 g][4 groups][row g, row g + 8] fp16 d
 //   [8 g][4 groups][row g, row g + 8] fp16 m   (Q4_1)
-constexpr int kUnitCols = 128, kTileRows = 16;
+constexpr int kUnitCols = 128, kTileRows = 16, kBlockTiles = 8;
 __host__ __device__ constexpr int unit_bytes(uint32_t type) { return type == GX_Q4_0 ? 1152 : 1280; }
+// Number of the unit u of the row tile rt, of KT units in a row.
+__host__ __device__ constexpr long long unit_index(long long rt, int u, int KT) {
+    return (rt / kBlockTiles * KT + u) * kBlockTiles + rt % kBlockTiles;
+}
 
 __device__ __forceinline__ void store_act(void *p, int bf16, size_t i, float v) {
     if (bf16) reinterpret_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
@@ -57,7 +60,7 @@ __global__ void __launch_bounds__(256) q4_repack_kernel(uint32_t type, const uin
     const int NG = (cols + kUnitCols - 1) / kUnitCols * 4;
     const long long row = i / NG;
     const int grp = (int)(i % NG), g = (int)(row & 7), hi = (int)(row >> 3) & 1, j = grp & 3;
-    uint8_t *u = w + ((row / kTileRows) * (NG / 4) + grp / 4) * unit_bytes(type);
+    uint8_t *u = w + unit_index(row / kTileRows, grp / 4, NG / 4) * unit_bytes(type);
     uint32_t words[4] = {0u, 0u, 0u, 0u};
     uint16_t d = 0, m = 0;
     if (row < rows && grp < cols / 32) {
@@ -137,17 +140,6 @@ __device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-}
-
-// The product of a group: both halves of its 32 columns, on nothing.
-__device__ __forceinline__ void mma_group(float (&d)[4], const uint32_t (&a0)[4], const uint32_t (&a1)[4], const uint4 &b) {
-    asm("{\n"
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%12,%13}, {%16,%16,%16,%16};\n"
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%8,%9,%10,%11}, {%14,%15}, {%0,%1,%2,%3};\n"
-        "}\n"
-        : "=&f"(d[0]), "=&f"(d[1]), "=&f"(d[2]), "=&f"(d[3])
-        : "r"(a0[0]), "r"(a0[1]), "r"(a0[2]), "r"(a0[3]), "r"(a1[0]), "r"(a1[1]), "r"(a1[2]), "r"(a1[3]), "r"(b.x), "r"(b.y),
-          "r"(b.z), "r"(b.w), "f"(0.f));
 }
 
 // The A registers of 8 codes of row g (r0) and of row g + 8 (r1): columns (0,4) (2,6) of each in a0,
@@ -246,14 +238,14 @@ struct Ints {
     static __device__ __forceinline__ int scale_offset(int lane) {
         return T == 1 ? (lane >> 1) * 4 + (lane >> 2) * 8 : (lane >> 2) * 16;
     }
-    static __device__ void stage(const Q4Args &a, int t0, int nt, int u0, int nu, uint8_t *smem, bool vec, int tid, int nthreads) {
-        const int cells = nu * 16, total = nt * cells;
+    static __device__ void stage(const Q4Args &a, int u0, int nu, uint8_t *smem, bool vec, int tid, int nthreads) {
+        const int cells = nu * 16, total = a.n_tok * cells;
         for (int base = 0; base < total; base += nthreads) {
             const int i = base + tid;
             const bool on = i < total;
             const int t = on ? i / cells : 0, cell = on ? i % cells : 0, q = cell & 3, j = (cell >> 2) & 3;
             float v[8];
-            const uint32_t big = load_cell<XB>(a, t0 + t, u0 * kUnitCols + cell * 8, on, vec, v), e = big >> 23;
+            const uint32_t big = load_cell<XB>(a, t, u0 * kUnitCols + cell * 8, on, vec, v), e = big >> 23;
             // 2^k with the unit's largest value below 2^30, as two factors: it may pass the f32 range
             const int k = 29 + 127 - (int)max(min(e, 254u), 1u), k1 = k / 2, k2 = k - k1;
             const float s1 = __uint_as_float((uint32_t)(127 + k1) << 23), s2 = __uint_as_float((uint32_t)(127 + k2) << 23);
@@ -387,14 +379,14 @@ struct Halves {
     static __device__ __forceinline__ int scale_offset(int lane) {
         return P == 4 ? (lane >> 1) * 4 + (lane >> 2) * 8 : (lane >> 2) * 16;
     }
-    static __device__ void stage(const Q4Args &a, int t0, int nt, int u0, int nu, uint8_t *smem, bool vec, int tid, int nthreads) {
-        const int cells = nu * 16, total = nt * cells;
+    static __device__ void stage(const Q4Args &a, int u0, int nu, uint8_t *smem, bool vec, int tid, int nthreads) {
+        const int cells = nu * 16, total = a.n_tok * cells;
         for (int base = 0; base < total; base += nthreads) {
             const int i = base + tid;
             const bool on = i < total;
             const int t = on ? i / cells : 0, cell = on ? i % cells : 0, q = cell & 3, j = (cell >> 2) & 3;
             float v[8];
-            const uint32_t e = load_cell<XB>(a, t0 + t, u0 * kUnitCols + cell * 8, on, vec, v) >> 23, se = min(268u - e, 247u);
+            const uint32_t e = load_cell<XB>(a, t, u0 * kUnitCols + cell * 8, on, vec, v) >> 23, se = min(268u - e, 247u);
             const float s = __uint_as_float(se << 23);
             float ss = 0.f;
 #pragma unroll
@@ -525,10 +517,14 @@ struct GemvPlan {
     int RT, KT;      // row tiles, units in a row
     int S;           // CTAs of a cluster that split the columns
     int WK;          // warps of a CTA that split its columns; W / WK row tiles at a time
-    int t0, nt;      // tokens of this launch
     int vec;         // activations can be read 16 bytes at a time
     int red_off;
 };
+
+__device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -570,22 +566,22 @@ __global__ void __launch_bounds__(W * 32, M::CTAS(W)) q4_gemv_kernel(Q4Args a, G
     const int step = (int)(gridDim.x / p.S) * groups;
     const int rt0 = (int)(blockIdx.x / p.S) * groups + wg;
 
-    // cursor of the loads: the next unit of this warp, units left of its row tile, row tiles left
+    // cursor of the loads: the next unit of this warp, units left of its row tile, the row tile
     constexpr int UB = unit_bytes(TYPE);
     const bool idle = wk >= nu;  // more warps than units: this one only takes part in the sums
     const int per = idle ? 0 : (nu - wk + p.WK - 1) / p.WK, scale = 1024 + M::scale_offset(lane) - lane * 16;
-    const uint8_t *lp = a.w + ((size_t)rt0 * p.KT + u0 + wk) * UB + lane * 16;
-    int lleft = per, ltiles = rt0 < p.RT && !idle ? (p.RT - rt0 + step - 1) / step : 0;
-    const int unit_step = p.WK * UB;
-    const long long tile_step = (long long)step * p.KT * UB - (long long)(per - 1) * unit_step;
+    auto tile_at = [&](int rt) { return a.w + unit_index(rt, u0 + wk, p.KT) * UB + lane * 16; };
+    const uint8_t *lp = tile_at(rt0);
+    int lleft = per, lrt = idle ? p.RT : rt0;
+    const int unit_step = p.WK * kBlockTiles * UB;
     Unit<TYPE, M::SETS> buf[kDepth];
     auto fetch = [&](Unit<TYPE, M::SETS> &u) {
-        if (ltiles > 0) {
+        if (lrt < p.RT) {
             load_unit(u, lp, scale);
             if (--lleft == 0) {
                 lleft = per;
-                --ltiles;
-                lp += tile_step;
+                lrt += step;
+                lp = tile_at(lrt);
             } else {
                 lp += unit_step;
             }
@@ -595,11 +591,11 @@ __global__ void __launch_bounds__(W * 32, M::CTAS(W)) q4_gemv_kernel(Q4Args a, G
     for (int k = 0; k < kDepth; ++k) fetch(buf[k]);
     pdl_launch_dependents();
     pdl_wait();  // the weights never change; the activations may come from the kernel before
-    M::stage(a, p.t0, p.nt, u0, nu, smem, p.vec != 0, tid, W * 32);
+    M::stage(a, u0, nu, smem, p.vec != 0, tid, W * 32);
     __syncthreads();
 
     M m;
-    m.init(lane, p.nt);
+    m.init(lane, a.n_tok);
     m.clear();
     int rt = rt0, left = per, parity = 0;
     const uint8_t *x = smem + wk * M::BYTES;  // the activations of the next unit
@@ -613,12 +609,12 @@ __global__ void __launch_bounds__(W * 32, M::CTAS(W)) q4_gemv_kernel(Q4Args a, G
         }
         const float *all = red + (size_t)(parity * W + wg * p.WK) * RED;
         float *keep = red + (size_t)(parity * W + wg * p.WK) * RED;
-        for (int i = wk * 32 + lane; i < 16 * p.nt; i += 32 * p.WK) {
+        for (int i = wk * 32 + lane; i < 16 * a.n_tok; i += 32 * p.WK) {
             float s = all[i];
             for (int k = 1; k < p.WK; ++k) s += all[(size_t)k * RED + i];
             if (p.S > 1) keep[i] = s;
             else if (rt * 16 + (i & 15) < a.rows)
-                store_act(a.y, a.y_bf16, (size_t)(p.t0 + (i >> 4)) * a.ldy + rt * 16 + (i & 15), s);
+                store_act(a.y, a.y_bf16, (size_t)(i >> 4) * a.ldy + rt * 16 + (i & 15), s);
         }
         if (p.WK == 1) __syncwarp();
         parity ^= 1;
@@ -646,11 +642,11 @@ __global__ void __launch_bounds__(W * 32, M::CTAS(W)) q4_gemv_kernel(Q4Args a, G
         cluster_sync_all();
         if (rank == 0 && rt0 < p.RT) {
             const float *all = red + (size_t)(wg * p.WK) * RED;
-            for (int i = wk * 32 + lane; i < 16 * p.nt; i += 32 * p.WK) {
+            for (int i = wk * 32 + lane; i < 16 * a.n_tok; i += 32 * p.WK) {
                 float s = all[i];
                 for (int r = 1; r < p.S; ++r) s += ld_cluster(all + i, (uint32_t)r);
                 if (rt0 * 16 + (i & 15) < a.rows)
-                    store_act(a.y, a.y_bf16, (size_t)(p.t0 + (i >> 4)) * a.ldy + rt0 * 16 + (i & 15), s);
+                    store_act(a.y, a.y_bf16, (size_t)(i >> 4) * a.ldy + rt0 * 16 + (i & 15), s);
             }
         }
         cluster_sync_all();  // no CTA leaves while its part is read
@@ -680,12 +676,10 @@ cudaError_t launch_gemv_w(const Q4Args &a, GemvPlan p, int smem, int grid, cudaS
 }
 
 template <uint32_t TYPE, bool XB, class M>
-cudaError_t launch_gemv(const Q4Args &a, int t0, int nt, int sm_count, cudaStream_t s) {
+cudaError_t launch_gemv(const Q4Args &a, int sm_count, cudaStream_t s) {
     GemvPlan p{};
     p.RT = (a.rows + kTileRows - 1) / kTileRows;
     p.KT = (a.cols + kUnitCols - 1) / kUnitCols;
-    p.t0 = t0;
-    p.nt = nt;
     const size_t esz = XB ? 2 : 4;
     p.vec = ((uintptr_t)a.x & 15) == 0 && (a.ldx * esz) % 16 == 0;
     // Enough warps for 16 on every SM: first the warps of a CTA split a row's units (down to two
@@ -709,29 +703,56 @@ cudaError_t launch_gemv(const Q4Args &a, int t0, int nt, int sm_count, cudaStrea
     return wide ? launch_gemv_w<TYPE, M, 16>(a, p, smem, grid, s) : launch_gemv_w<TYPE, M, 8>(a, p, smem, grid, s);
 }
 
-// ---- more tokens: a tiled product on mma.sync ---------------------------------------------------
-// The activations are packed once per call (q4_pack_kernel) into the same fragments, at one scale per
-// token, in a workspace of the context: [unit][4 groups][COLS columns][4 q] 16 B, then the group sums
-// [4 groups][TOK tokens] of the unit; the tokens' inverse scales stand before the first unit. (A scale and
-// a CTA per token and range of units packs no faster, and the product then waits 2 us longer for it.)
-constexpr int kQ4InvBytes = 64 * 4;
-
-struct GemmPlan {
-    int RT, KT;
-    int WM, WK;      // warps: row tiles of a CTA, and splits of its units
-    int S;           // CTAs of a cluster that split the units
-    int vec;
-};
-
+// ---- more tokens: a product on tcgen05 ----------------------------------------------------------
+// D[128 rows][N] = sum over all columns of w x, in one accumulator in tensor memory. That asks for weights
+// that the tensor core can take as they are: d (q - 8) has up to 15 significant bits, and two bf16 hold it
+// exactly (Split). Decoder warps write both parts into tensor memory, a lane a row, as A; the packed
+// activations are B in shared memory, one column a token in bf16 and three in f32 (8 bits each, all 24).
+// No weight and no activation is rounded; a sum of 8192 columns is 1024 steps in f32 over the cluster.
+//
+// (With d applied to each group's sum afterwards, as in the GEMV, the product needs one accumulator a
+// group, and warps that read each of them back: 46 us for 64 f32 tokens by 8192 x 8192 against 42, and 42 us
+// against 26 in bf16. On mma.sync the same products took 71 and 48 us.)
+//
+// What bounds it: the chain of one unit (128 columns) in the issuing thread, two waits, 16 MMAs and two
+// commits, 0.5 us; the MMAs themselves would take a third of that, the codes' bytes a tenth. So a unit has
+// one full and one empty barrier for its weights, its codes come by one bulk copy (a copy for each of its 8
+// row tiles kept the copying thread 0.9 us a unit), and one thread runs the issue loop by itself (a whole
+// warp with an elected lane: 32 us against 28).
+//
+// Warps: 0 copies, 1 tensor memory and MMA issue, then sets of four decoders that take units in turn, and four
+// that read the sums. Three sets: 25.4 us, two: 25.7 (8192 x 8192, 64 bf16 tokens).
+constexpr int kTcRows = kTileRows * kBlockTiles;
+constexpr int kQ4InvBytes = 64 * 4;  // of a workspace: the tokens' inverse scales, before the first unit
 constexpr int kPackThreads = 512;
 
-// One CTA per token.
-template <uint32_t TYPE, bool XB>
-__global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(Q4Args a, uint8_t *ws, int KT, int cols_padded, int vec) {
+// Activations of a unit: two tiles of 64 columns (two groups), [N rows][128 B] in the 128-byte swizzle, row
+// t + TP p part p of token t, a group's 8 columns of q as the 16-byte chunk 4 (group & 1) + q in the order
+// (0,4) (1,5) (2,6) (3,7), as a word of codes is unpacked; Q4_1: a third tile, chunk j the group sums of group
+// j in three parts, as m multiplies them.
+template <uint32_t TYPE, bool XB, int TP>
+struct Tc {
+    static constexpr int N = XB ? TP : 3 * TP;
+    static constexpr int BU = N * 128 * (TYPE == GX_Q4_1 ? 3 : 2);         // a unit's activations
+    static constexpr int STAGE = BU + 8 * unit_bytes(TYPE);                 // and the codes of 8 row tiles
+    static constexpr int XS = (kMaxSmem - 4096) / STAGE < 6 ? (kMaxSmem - 4096) / STAGE : 6;
+    static constexpr int SLOTS = N <= 64 ? 2 : 1, SLOT = (N + 31) / 32 * 32;  // accumulators, their TMEM columns
+    static constexpr int AC = TYPE == GX_Q4_1 ? 144 : 128;                  // TMEM columns of a unit's weights
+    static constexpr int AS = (512 - SLOTS * SLOT) / AC;                    // stages of those
+    // A set that is ahead of a ring by more than one turn would take the parity of the turn before for its own.
+    static constexpr int RING = XS < AS ? XS : AS, SETS = RING < 3 ? RING : 3;
+    static constexpr int THREADS = (6 + 4 * SETS) * 32;
+    static constexpr int BARS = XS * STAGE;
+    static constexpr int BYTES = BARS + 512 + 1024;                         // and the alignment
+};
+
+// One CTA per token: its values at the power of two that brings the largest to 2^14..2^15 (a token with an
+// Inf or NaN is all NaN), in bf16 parts.
+template <uint32_t TYPE, bool XB, int TP>
+__global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(Q4Args a, uint8_t *ws, int KT, int vec) {
+    using C = Tc<TYPE, XB, TP>;
     __shared__ uint32_t red[kPackThreads / 32];
     const int t = blockIdx.x, tid = threadIdx.x, cells = KT * 16;
-    const int tok_padded = XB ? cols_padded : cols_padded / 2;
-    const size_t unit = (size_t)cols_padded * 256 + (size_t)tok_padded * 16;
     pdl_launch_dependents();
     pdl_wait();
     auto load = [&](int cell, float (&v)[8]) {
@@ -776,236 +797,357 @@ __global__ void __launch_bounds__(kPackThreads) q4_pack_kernel(Q4Args a, uint8_t
         } else {
             load(cell, v);
         }
-        float ss = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            v[k] = e == 255u ? __uint_as_float(0x7fffffffu) : v[k] * s;
-            ss += v[k];
-        }
-        if constexpr (TYPE == GX_Q4_1) ss = quad_sum(ss);
-        if (cell >= cells) continue;
+        for (int k = 0; k < 8; ++k) v[k] = e == 255u ? __uint_as_float(0x7fffffffu) : v[k] * s;
         const int q = cell & 3, j = (cell >> 2) & 3;
-        uint8_t *u = units + (size_t)(cell >> 4) * unit;
-        put_fragment<XB>(u + (size_t)j * cols_padded * 64, t, q, v);
-        if (TYPE == GX_Q4_1 && q == 0) reinterpret_cast<float *>(u + (size_t)cols_padded * 256)[j * tok_padded + t] = ss;
-    }
-}
-
-constexpr int kGemmWarps = 8;
-constexpr int gemm_stages(int MT) { return MT == 2 ? 3 : 2; }
-
-// acc += d * c, both halves in one instruction.
-__device__ __forceinline__ void fma2(float2 &acc, float d, float2 c) {
-    asm("{\n.reg .b64 a, b, d;\n"
-        "mov.b64 a, {%0, %1};\nmov.b64 d, {%2, %2};\nmov.b64 b, {%3, %4};\n"
-        "fma.rn.f32x2 a, d, b, a;\nmov.b64 {%0, %1}, a;\n}"
-        : "+f"(acc.x), "+f"(acc.y)
-        : "f"(d), "f"(c.x), "f"(c.y));
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
-// A CTA takes WM row tiles by all tokens over its range of units: warp (wk, wm) one row tile of every
-// WK-th unit, NB product tiles wide, so that a code is unpacked once. Codes and fragments come by bulk
-// copies through a ring of shared-memory stages of WK units; the parts are added over wk and the
-// cluster's CTAs at the end.
-template <uint32_t TYPE, bool XB, int NB, int MT>
-__global__ void __launch_bounds__(kGemmWarps * 32, 2) q4_gemm_kernel(Q4Args a, const uint8_t *ws, GemmPlan p) {
-    constexpr int UB = unit_bytes(TYPE), COLS = 8 * NB, TOK = XB ? COLS : COLS / 2;
-    constexpr int BU = COLS * 256 + TOK * 16;  // a unit's fragments and sums
-    constexpr int kGemmStages = gemm_stages(MT);
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ __align__(8) uint64_t bars[kGemmStages], empty[kGemmStages];  // a stage has come; all warps have read it
-    __shared__ float inv[64];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-    const int wm = warp % p.WM, wk = warp / p.WM;
-    const int unit_stage = BU + MT * p.WM * UB, stage_bytes = p.WK * unit_stage;
-    const int rank = p.S > 1 ? (int)cluster_rank() : 0;
-    const int u0 = (int)((long long)p.KT * rank / p.S), u1 = (int)((long long)p.KT * (rank + 1) / p.S), nu = u1 - u0;
-    const int rt0 = (int)(blockIdx.x / p.S) * p.WM * MT, iters = (nu + p.WK - 1) / p.WK;
-    const int tiles = min(p.WM * MT, p.RT - rt0);
-    const uint8_t *units = ws + kQ4InvBytes;
-
-    auto copy_codes = [&](int it) {  // and the bytes that the stage waits for
-        const int n = min(p.WK, nu - it * p.WK);
-        mbar_expect_tx(&bars[it % kGemmStages], (uint32_t)(n * (BU + tiles * UB)));
-        for (int k = 0; k < n; ++k)
-            for (int t = 0; t < tiles; ++t)
-                bulk_g2s(smem + (it % kGemmStages) * stage_bytes + k * unit_stage + BU + t * UB,
-                         a.w + ((size_t)(rt0 + t) * p.KT + u0 + it * p.WK + k) * UB, UB, &bars[it % kGemmStages]);
-    };
-    auto copy_frags = [&](int it) {
-        const int n = min(p.WK, nu - it * p.WK);
-        for (int k = 0; k < n; ++k)
-            bulk_g2s(smem + (it % kGemmStages) * stage_bytes + k * unit_stage, units + (size_t)(u0 + it * p.WK + k) * BU, BU,
-                     &bars[it % kGemmStages]);
-    };
-    if (tid == 0) {
-        for (int i = 0; i < kGemmStages; ++i) {
-            mbar_init(&bars[i], 1);
-            mbar_init(&empty[i], kGemmWarps);
-        }
-        fence_barrier_init();
-        // the weights never change: they may be fetched before the activations are packed
-        for (int i = 0; i < kGemmStages && i < iters; ++i) copy_codes(i);
-    }
-    __syncthreads();
-    pdl_launch_dependents();
-    pdl_wait();
-    if (tid == 0)
-        for (int i = 0; i < kGemmStages && i < iters; ++i) copy_frags(i);
-    if (tid < 64) inv[tid] = tid < a.n_tok ? reinterpret_cast<const float *>(ws)[tid] : 0.f;
-
-    // sums of (row g; row g + 8) of columns 2 q and 2 q + 1: two tokens in bf16, the parts of one in f32
-    float2 acc[MT][NB][2];
+        uint8_t *u = units + (size_t)(cell >> 4) * C::BU;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+        for (int piece = 0; piece < (XB ? 1 : 3); ++piece) {
+            const int row = piece * TP + t;
+            uint8_t *at = u + (row >> 3) * 1024 + (row & 7) * 128;
+            float x[8], ss = 0.f;
 #pragma unroll
-        for (int n = 0; n < NB; ++n) acc[m][n][0] = acc[m][n][1] = make_float2(0.f, 0.f);
-    bool ok = true;  // an expired wait is reported and ends the warp's loop
-    int copied = min(iters, kGemmStages);
-    for (int it = 0; it < iters; ++it) {
-        ok = mbar_wait(&bars[it % kGemmStages], (uint32_t)(it / kGemmStages & 1), a.err);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        if (it * p.WK + wk < nu && wm * MT < tiles) {
-            const uint8_t *st = smem + (it % kGemmStages) * stage_bytes + wk * unit_stage;
-            const float *sums = reinterpret_cast<const float *>(st + COLS * 256);
-            const uint8_t *t = st + BU + wm * MT * UB;  // a tile past the matrix holds what was there: nothing of it is stored
-            const uint32_t *codes = reinterpret_cast<const uint32_t *>(t) + lane * 4;
-            const uint32_t *scales = reinterpret_cast<const uint32_t *>(t + 1024) + g * 4;
-#pragma unroll 1
-            for (int j = 0; j < 4; ++j) {
-                uint32_t a0[MT][4], a1[MT][4], mw[MT];
-                float d0[MT], d1[MT];
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    code_fragments<TYPE>(codes[m * (UB / 4) + j], codes[m * (UB / 4) + j + 128], a0[m], a1[m]);
-                    d0[m] = half_value(scales[m * (UB / 4) + j], 0);
-                    d1[m] = half_value(scales[m * (UB / 4) + j], 1);
-                    if constexpr (TYPE == GX_Q4_1) mw[m] = scales[m * (UB / 4) + j + 32];
-                }
-#pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                    const uint4 b = *reinterpret_cast<const uint4 *>(st + ((j * COLS + 8 * n) * 4 + lane) * 16);
-                    float2 sx = make_float2(0.f, 0.f);
-                    if constexpr (TYPE == GX_Q4_1) {
-                        if constexpr (XB) sx = *reinterpret_cast<const float2 *>(sums + j * TOK + 8 * n + 2 * q);
-                        else sx.x = sums[j * TOK + 4 * n + q];
-                    }
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        float c[4];
-                        mma_group(c, a0[m], a1[m], b);
-                        fma2(acc[m][n][0], d0[m], make_float2(c[0], c[1]));
-                        fma2(acc[m][n][1], d1[m], make_float2(c[2], c[3]));
-                        if constexpr (TYPE == GX_Q4_1) {
-                            fma2(acc[m][n][0], half_value(mw[m], 0), sx);
-                            fma2(acc[m][n][1], half_value(mw[m], 1), sx);
-                        }
-                    }
-                }
+            for (int k = 0; k < 8; ++k) {
+                x[k] = __bfloat162float(__float2bfloat16_rn(v[k]));
+                v[k] -= x[k];
+                ss += x[k];
             }
+            if constexpr (TYPE == GX_Q4_1) ss = quad_sum(ss);
+            if (cell >= cells) continue;
+            *reinterpret_cast<uint4 *>(at + (j >> 1) * C::N * 128 + (((4 * (j & 1) + q) ^ (row & 7)) << 4)) =
+                make_uint4(pack_bf2(x[0], x[4]), pack_bf2(x[1], x[5]), pack_bf2(x[2], x[6]), pack_bf2(x[3], x[7]));
+            if (TYPE == GX_Q4_1 && q == 0) {
+                const float s1 = __bfloat162float(__float2bfloat16_rn(ss)), s2 = __bfloat162float(__float2bfloat16_rn(ss - s1));
+                const float s3 = ss - s1 - s2;
+                *reinterpret_cast<uint4 *>(at + 2 * C::N * 128 + ((j ^ (row & 7)) << 4)) =
+                    make_uint4(pack_bf2(s1, s2), pack_bf2(s3, s1), pack_bf2(s2, s3), 0u);
+            }
+        }
+    }
+}
+
+// The weights of a group as two bf16 each, exactly.
+//
+// Q4_0: d = d1 + d2, d1 of 5 significant bits (nearest), so d2 has 5 too, and (q - 8) d1, (q - 8) d2 have 8. A
+// code in bits 3 .. 6 under the exponent of 128 is 8 (16 + q), and (q - 8) d1 = 8 (16 + q) d1 / 8 - 24 d1 with
+// all of it in bf16: one instruction for two weights and each part.
+//
+// Q4_1: q has 4 bits, which leaves none. d1 of 8 bits, d2 the last 3; hi = bf16(q d1), and lo = q d - hi has 7
+// bits at most. Its negative comes out of two multiply-adds, and the product subtracts it.
+template <uint32_t TYPE>
+struct Split {
+    __nv_bfloat162 a, b, c, d;
+    __device__ __forceinline__ explicit Split(float scale) {
+        if constexpr (TYPE == GX_Q4_0) {
+            const float d1 = __uint_as_float((__float_as_uint(scale) + 0x40000u) & 0xfff80000u), d2 = scale - d1;
+            a = __float2bfloat162_rn(d1 * 0.125f);
+            b = __float2bfloat162_rn(d1 * -24.f);
+            c = __float2bfloat162_rn(d2 * 0.125f);
+            d = __float2bfloat162_rn(d2 * -24.f);
+        } else {
+            a = __float2bfloat162_rn(scale);
+            const float d1 = __low2float(a);
+            b = __float2bfloat162_rn(-d1);
+            c = __float2bfloat162_rn(d1 - scale);
+        }
+    }
+    // Codes k and k + 4 of a word.
+    __device__ __forceinline__ void pair(uint32_t word, int k, uint32_t &hi, uint32_t &lo) const {
+        constexpr int at = TYPE == GX_Q4_0 ? 3 : 0;  // bit of the code
+        const int right = 4 * k - at;
+        uint32_t v;
+        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(right < 0 ? word << -right : word >> right), "r"(0x000f000fu << at), "r"(0x43004300u));
+        const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162 *>(&v);
+        __nv_bfloat162 h, l;
+        if constexpr (TYPE == GX_Q4_0) {
+            h = __hfma2(x, a, b);
+            l = __hfma2(x, c, d);
+        } else {
+            const __nv_bfloat162 q = __hadd2(x, __float2bfloat162_rn(-128.f));
+            h = __hmul2(q, a);
+            l = __hfma2(q, c, __hfma2(q, b, h));
+        }
+        hi = *reinterpret_cast<const uint32_t *>(&h);
+        lo = *reinterpret_cast<const uint32_t *>(&l);
+    }
+};
+
+struct TcPlan {
+    int RT, KT, blocks, S;
+};
+
+template <uint32_t TYPE, bool XB, int TP>
+__global__ void __launch_bounds__((Tc<TYPE, XB, TP>::THREADS), 1) q4_tc_kernel(Q4Args a, const uint8_t *ws, TcPlan p) {
+    using C = Tc<TYPE, XB, TP>;
+    constexpr int UB = unit_bytes(TYPE), XS = C::XS, AS = C::AS;
+    extern __shared__ __align__(1024) uint8_t tc_raw[];
+    __shared__ float inv[64];
+    uint8_t *sm = reinterpret_cast<uint8_t *>(((uintptr_t)tc_raw + 1023) & ~(uintptr_t)1023);
+    float *red = reinterpret_cast<float *>(sm);  // [TP][128] f32: a cluster's parts, when the stages are done
+    uint64_t *full_x = reinterpret_cast<uint64_t *>(sm + C::BARS), *empty_x = full_x + XS;
+    uint64_t *full_a = empty_x + XS, *empty_a = full_a + AS;
+    uint64_t *full_d = empty_a + AS, *empty_d = full_d + 2, *done = empty_d + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = p.S > 1 ? (int)cluster_rank() : 0;
+    const int u0 = (int)((long long)p.KT * rank / p.S), nu = (int)((long long)p.KT * (rank + 1) / p.S) - u0;
+    // row blocks of this CTA: with S > 1 one, else every gridDim.x-th
+    const int first = (int)blockIdx.x / p.S, step = (int)gridDim.x / p.S, items = first < p.blocks ? (p.blocks - first + step - 1) / step : 0;
+    if (tid == 0) {
+        for (int i = 0; i < XS; ++i) {
+            mbar_init(&full_x[i], 1);
+            mbar_init(&empty_x[i], 1);
+        }
+        for (int i = 0; i < AS; ++i) {
+            mbar_init(&full_a[i], 4);
+            mbar_init(&empty_a[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&full_d[i], 1);
+            mbar_init(&empty_d[i], 4);
+        }
+        mbar_init(done, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    pdl_launch_dependents();
+    if (warp == 1) tmem_alloc(tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t a_cols = tmem + (uint32_t)(C::SLOTS * C::SLOT);
+    // An expired wait is reported and ends every role of the CTA.
+    auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+        if (mbar_wait(bar, parity, a.err)) return true;
+        *abort_flag = 1;
+        return false;
+    };
+    auto wait_all = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
+    const int total = items * nu;  // units, item by item
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int block = first, u = 0;  // of the next codes
+            auto codes = [&](int st) {
+                mbar_expect_tx(&full_x[st], (uint32_t)C::STAGE);
+                bulk_g2s(sm + st * C::STAGE + C::BU, a.w + unit_index(block * kBlockTiles, u0 + u, p.KT) * UB, kBlockTiles * UB,
+                         &full_x[st]);
+                if (++u == nu) {
+                    u = 0;
+                    block += step;
+                }
+            };
+            // the weights never change: they are fetched before the activations are packed
+            for (int n = 0; n < XS && n < total; ++n) codes(n);
+            pdl_wait();
+            for (int n = 0, v = 0; n < total; ++n) {
+                const int st = n % XS;
+                if (n >= XS) {
+                    if (!wait(&empty_x[st], (uint32_t)(n / XS & 1) ^ 1u)) break;
+                    codes(st);
+                }
+                bulk_g2s(sm + st * C::STAGE, ws + kQ4InvBytes + (size_t)(u0 + v) * C::BU, C::BU, &full_x[st]);
+                v = v + 1 == nu ? 0 : v + 1;
+            }
+        }
+    } else if (warp == 1) {
+        if (elect_one()) {
+        constexpr uint32_t idesc = f16_idesc(kTcRows, C::N) | (1u << 7) | (1u << 10);  // A and B are bf16
+        constexpr uint32_t idesc_lo = TYPE == GX_Q4_1 ? idesc | (1u << 13) : idesc;     // A negated
+        bool ok = true;
+        for (int item = 0, n = 0; ok && item < items; ++item) {
+            const int slot = item % C::SLOTS;
+            const uint32_t dst = tmem + (uint32_t)(slot * C::SLOT);
+            ok = wait(&empty_d[slot], (uint32_t)(item / C::SLOTS & 1) ^ 1u);
+            for (int u = 0; ok && u < nu; ++u, ++n) {
+                const int sx = n % XS;
+                const int sa = n % AS;
+                ok = wait(&full_x[sx], (uint32_t)(n / XS & 1)) && wait(&full_a[sa], (uint32_t)(n / AS & 1));
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t xd = sw128_desc(smem_u32(sm + sx * C::STAGE));
+                const uint32_t at = a_cols + (uint32_t)(C::AC * sa);
+                // k-step k: half k / 4 of the unit, 32 bytes further in every 128-byte row
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    umma_f16_ts(dst, at + 8u * k, xd + (uint64_t)((k >> 2) * (C::N * 128 >> 4) + 2 * (k & 3)), idesc, (u | k) != 0);
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    umma_f16_ts(dst, at + 64u + 8u * k, xd + (uint64_t)((k >> 2) * (C::N * 128 >> 4) + 2 * (k & 3)), idesc_lo, 1u);
+                if constexpr (TYPE == GX_Q4_1) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) umma_f16_ts(dst, at + 128u + 8u * h, xd + (uint64_t)(2 * (C::N * 128 >> 4) + 2 * h), idesc, 1u);
+                }
+                umma_commit(&empty_a[sa]);
+                umma_commit(&empty_x[sx]);
+            }
+            if (ok) umma_commit(&full_d[slot]);
+            
+        }
+        // all issued MMAs complete before TMEM is released
+        umma_commit(done);
+        mbar_wait(done, 0, nullptr);
+        
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[it % kGemmStages]);
-        // the first warp refills the stage of the step before, which the others have likely left by now
-        if (tid == 0 && it > 0 && copied < iters && ok) {
-            ok = mbar_wait(&empty[(it - 1) % kGemmStages], (uint32_t)((it - 1) / kGemmStages & 1), a.err);
-            if (ok) {
-                copy_codes(copied);
-                copy_frags(copied);
-                ++copied;
+    } else if (warp < 2 + 4 * C::SETS) {
+        // decoders: row i of the block
+        const int set = (warp - 2) >> 2, lg = warp & 3, i = 32 * lg + lane, r = i & 15, rot = (r >> 1) & 3, sh = r & 8 ? 16 : 0;
+        for (int n = set; n < total; n += C::SETS) {
+            const int sx = n % XS;
+            if (!wait_all(&full_x[sx], (uint32_t)(n / XS & 1))) break;
+            // 64 bytes of the row's codes: word j of 16-byte part q are columns 8 q .. of group j. The lanes
+            // start at different parts, so that 8 of them read all banks.
+            const uint8_t *tile = sm + sx * C::STAGE + C::BU + (i >> 4) * UB;
+            const uint4 *w = reinterpret_cast<const uint4 *>(tile + (r >> 3) * 512 + (r & 7) * 64);
+            uint4 c[4] = {w[rot], w[(rot + 1) & 3], w[(rot + 2) & 3], w[(rot + 3) & 3]};  // parts rot, rot + 1, ..
+            const uint4 d4 = reinterpret_cast<const uint4 *>(tile + 1024)[r & 7];
+            uint4 m4 = make_uint4(0u, 0u, 0u, 0u);
+            if constexpr (TYPE == GX_Q4_1) m4 = reinterpret_cast<const uint4 *>(tile + 1152)[r & 7];
+            auto sel = [](bool p, uint4 x, uint4 y) { return make_uint4(p ? x.x : y.x, p ? x.y : y.y, p ? x.z : y.z, p ? x.w : y.w); };
+            {
+                const bool odd = rot & 1, two = rot & 2;
+                const uint4 e[4] = {sel(odd, c[3], c[0]), sel(odd, c[0], c[1]), sel(odd, c[1], c[2]), sel(odd, c[2], c[3])};
+                c[0] = sel(two, e[2], e[0]);
+                c[1] = sel(two, e[3], e[1]);
+                c[2] = sel(two, e[0], e[2]);
+                c[3] = sel(two, e[1], e[3]);
             }
+            const int sa = n % AS;
+            if (!wait_all(&empty_a[sa], (uint32_t)(n / AS & 1) ^ 1u)) break;
+            tc_fence_after();
+            const uint32_t at = a_cols + ((uint32_t)(32 * lg) << 16) + (uint32_t)(C::AC * sa);
+            uint32_t mv[16];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                auto group = [g](const uint4 &v) { return g == 0 ? v.x : g == 1 ? v.y : g == 2 ? v.z : v.w; };
+                const Split<TYPE> split(half_value(group(d4) >> sh, 0));
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) split.pair(group(c[q]), k, hi[4 * q + k], lo[4 * q + k]);
+                tmem_st16(at + 16u * g, hi);
+                tmem_st16(at + 64u + 16u * g, lo);
+                if constexpr (TYPE == GX_Q4_1) {
+                    const float f = half_value(group(m4) >> sh, 0), m1 = __bfloat162float(__float2bfloat16_rn(f)), m2 = f - m1;
+                    mv[4 * g] = pack_bf2(m1, m1);
+                    mv[4 * g + 1] = pack_bf2(m1, m2);
+                    mv[4 * g + 2] = pack_bf2(m2, m2);
+                    mv[4 * g + 3] = 0u;
+                }
+            }
+            if constexpr (TYPE == GX_Q4_1) tmem_st16(at + 128u, mv);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full_a[sa]);
+        }
+    } else {
+        const int lg = warp & 3, i = 32 * lg + lane;
+        pdl_wait();
+        for (int t = i; t < TP; t += kTcRows) inv[t] = t < a.n_tok ? __ldcg(reinterpret_cast<const float *>(ws) + t) : 0.f;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        for (int item = 0; item < items; ++item) {
+            const int slot = item % C::SLOTS, row = (first + item * step) * kTcRows + i;
+            if (!wait_all(&full_d[slot], (uint32_t)(item / C::SLOTS & 1))) break;
+            tc_fence_after();
+            const uint32_t at = tmem + ((uint32_t)(32 * lg) << 16) + (uint32_t)(slot * C::SLOT);
+#pragma unroll
+            for (int t0 = 0; t0 < TP; t0 += 16) {
+                uint32_t v[16];
+                tmem_ld16(at + (uint32_t)t0, v);
+                tmem_wait_ld();
+                if constexpr (!XB) {
+#pragma unroll
+                    for (int piece = 1; piece < 3; ++piece) {
+                        uint32_t x[16];
+                        tmem_ld16(at + (uint32_t)(piece * TP + t0), x);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) + __uint_as_float(x[k]));
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const int tok = t0 + k;
+                    if (tok >= a.n_tok) break;
+                    const float y = __uint_as_float(v[k]) * inv[tok];
+                    if (p.S > 1) red[tok * kTcRows + i] = y;
+                    else if (row < a.rows) store_act(a.y, a.y_bf16, (size_t)tok * a.ldy + row, y);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty_d[slot]);
         }
     }
-    if (!__syncthreads_and(ok) && tid == 0)  // no copy may outlive the CTA
-        for (int it = copied > kGemmStages ? copied - kGemmStages : 0; it < copied; ++it)
-            mbar_wait(&bars[it % kGemmStages], (uint32_t)(it / kGemmStages & 1), nullptr);
+    tc_fence_before();
     __syncthreads();
-    // parts [WK][TOK][rows + 8] over the stages
-    const int rows = MT * p.WM * 16, ld = rows + 8, part = TOK * ld;
-    float *mine = reinterpret_cast<float *>(smem) + wk * part;
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const int t = XB ? 8 * n + 2 * q : 4 * n + q;
-        const float i0 = inv[t], i1 = XB ? inv[t + 1] : 0.f;
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            const int r = (wm * MT + m) * 16 + g;
-            if constexpr (XB) {
-                mine[t * ld + r] = acc[m][n][0].x * i0;
-                mine[(t + 1) * ld + r] = acc[m][n][0].y * i1;
-                mine[t * ld + r + 8] = acc[m][n][1].x * i0;
-                mine[(t + 1) * ld + r + 8] = acc[m][n][1].y * i1;
-            } else {
-                mine[t * ld + r] = (acc[m][n][0].x + acc[m][n][0].y) * i0;
-                mine[t * ld + r + 8] = (acc[m][n][1].x + acc[m][n][1].y) * i0;
-            }
-        }
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
     }
-    if (p.S > 1) cluster_sync_all();
-    else __syncthreads();
-    // the CTAs of a cluster share the sums out, four rows of a token to a thread
-    const float *all = reinterpret_cast<const float *>(smem);
-    for (int i = rank * kGemmWarps * 32 + tid; i < a.n_tok * rows / 4; i += p.S * kGemmWarps * 32) {
-        const int t = i / (rows / 4), r = (i - t * (rows / 4)) * 4, row = rt0 * 16 + r;
-        if (row >= a.rows) continue;
-        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < p.WK; ++k) {
-            const float *at = all + k * part + t * ld + r;
+    if (warp == 0 && lane == 0 && *abort_flag) {  // no copy may outlive the CTA: at most one a stage is under way
+        for (int i = 0; i < XS; ++i)
+            for (uint32_t parity = 0; parity < 2; ++parity) mbar_wait(&full_x[i], parity, nullptr);
+    }
+    if (p.S > 1) {
+        cluster_sync_all();
+        // the CTAs of a cluster divide the sums among them, four rows of a token to a thread
+        for (int j = rank * C::THREADS + tid; j < a.n_tok * (kTcRows / 4); j += p.S * C::THREADS) {
+            const int t = j / (kTcRows / 4), r = j % (kTcRows / 4) * 4, row = first * kTcRows + r;
+            if (row >= a.rows) continue;
+            const float *at = red + t * kTcRows + r;
             float4 v[8];  // all parts on their way before the first is added
 #pragma unroll
             for (int c = 0; c < 8; ++c)
-                if (c < p.S) v[c] = p.S > 1 ? ld_cluster4(at, (uint32_t)c) : *reinterpret_cast<const float4 *>(at);
+                if (c < p.S) v[c] = ld_cluster4(at, (uint32_t)c);
+            float4 s = v[0];
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
+            for (int c = 1; c < 8; ++c)
                 if (c < p.S) {
                     s.x += v[c].x;
                     s.y += v[c].y;
                     s.z += v[c].z;
                     s.w += v[c].w;
                 }
+            const float out[4] = {s.x, s.y, s.z, s.w};
+            for (int k = 0; k < 4 && row + k < a.rows; ++k) store_act(a.y, a.y_bf16, (size_t)t * a.ldy + row + k, out[k]);
         }
-        const size_t o = (size_t)t * a.ldy + row;
-        const float out[4] = {s.x, s.y, s.z, s.w};
-        for (int k = 0; k < 4 && row + k < a.rows; ++k) store_act(a.y, a.y_bf16, o + k, out[k]);
+        cluster_sync_all();  // no CTA leaves while its part is read
     }
-    if (p.S > 1) cluster_sync_all();  // no CTA leaves while its parts are read
 }
 
-template <uint32_t TYPE, bool XB, int NB, int MT>
-cudaError_t launch_gemm_mt(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s) {
-    constexpr int COLS = 8 * NB, TOK = XB ? COLS : COLS / 2, BU = COLS * 256 + TOK * 16;
-    GemmPlan p{};
+template <uint32_t TYPE, bool XB, int TP>
+cudaError_t launch_tc(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s) {
+    using C = Tc<TYPE, XB, TP>;
+    TcPlan p{};
     p.RT = (a.rows + kTileRows - 1) / kTileRows;
     p.KT = (a.cols + kUnitCols - 1) / kUnitCols;
-    p.WM = kGemmWarps;
-    p.WK = p.S = 1;
-    // CTAs for one and a half on every SM: first the CTAs of a cluster split the units (down to two units
-    // a CTA), then fewer row tiles and more splits in a CTA.
-    auto ctas = [&] { return (p.RT + MT * p.WM - 1) / (MT * p.WM) * p.S; };
-    auto ring = [&](int wm, int wk) { return gemm_stages(MT) * wk * (BU + MT * wm * unit_bytes(TYPE)); };
-    while (p.S < 8 && ctas() < sm_count * 3 / 2 && p.KT >= 4 * p.S) p.S *= 2;
-    while (p.WM > 1 && ctas() < sm_count * 3 / 2 && p.KT >= 4 * p.S * p.WK && ring(p.WM / 2, p.WK * 2) <= kMaxSmem / 2) {
-        p.WM /= 2;
-        p.WK *= 2;
-    }
-    const int parts = p.WK * TOK * (MT * p.WM * 16 + 8) * 4;
-    const int smem = ring(p.WM, p.WK) > parts ? ring(p.WM, p.WK) : parts;
-    if (smem > kMaxSmem - kStaticSmem) return cudaErrorInvalidValue;
-    p.vec = ((uintptr_t)a.x & 15) == 0 && a.ldx * (XB ? 2 : 4) % 16 == 0;
-    cudaError_t e = launch_chain_pdl(true, q4_pack_kernel<TYPE, XB>, dim3((unsigned)a.n_tok), dim3(kPackThreads), 0, s, a, ws,
-                                     p.KT, COLS, p.vec);
+    p.blocks = (p.RT + 7) / 8;
+    // One CTA an SM. Where row blocks leave SMs idle, the CTAs of a cluster split the units (down to two a
+    // CTA). 148 SMs take 130 to 135 CTAs at once in clusters of 3 to 6, but 120 in clusters of 8: 16 row blocks
+    // of 8192 columns by 64 tokens took 24 us with 8 (two waves), 15.2 with 6.
+    p.S = 1;
+    for (int c = 2; c <= 6; ++c)
+        if (p.blocks * c <= (c == 2 ? sm_count : sm_count * 7 / 8) && p.KT >= 2 * c) p.S = c;
+    const int vec = ((uintptr_t)a.x & 15) == 0 && a.ldx * (XB ? 2 : 4) % 16 == 0;
+    cudaError_t e = launch_chain_pdl(true, q4_pack_kernel<TYPE, XB, TP>, dim3((unsigned)a.n_tok), dim3(kPackThreads), 0, s, a, ws,
+                                     p.KT, vec);
     if (e != cudaSuccess) return e;
-    auto *k = q4_gemm_kernel<TYPE, XB, NB, MT>;
+    auto *k = q4_tc_kernel<TYPE, XB, TP>;
     static SmemLimit limit;
     e = limit.raise(k);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas());
-    cfg.blockDim = dim3(kGemmWarps * 32);
-    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.gridDim = dim3((unsigned)(p.S > 1 ? p.blocks * p.S : p.blocks < sm_count ? p.blocks : sm_count));
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = C::BYTES;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1018,44 +1160,30 @@ cudaError_t launch_gemm_mt(const Q4Args &a, uint8_t *ws, int sm_count, cudaStrea
     return cudaLaunchKernelEx(&cfg, k, a, (const uint8_t *)ws, p);
 }
 
-template <uint32_t TYPE, bool XB, int NB>
-cudaError_t launch_gemm(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s) {
-    if constexpr (NB <= 8) {  // two row tiles by more columns do not fit the registers
-        if (a.rows >= 4096) return launch_gemm_mt<TYPE, XB, NB, 2>(a, ws, sm_count, s);
-    }
-    return launch_gemm_mt<TYPE, XB, NB, 1>(a, ws, sm_count, s);
-}
-
+// The GEMV takes up to 16 product columns (a token is one in bf16, two in f32), but every CTA stages the
+// activations for itself, which from 48 K of them costs more than the product's two launches: 8192 x 8192 by 3, 5,
+// 8 tokens of f32 take 26.7, 50, 56 us there and 20.5, 20.7, 21.1 here; 8192 x 2048 takes 6.6, 6.5, 7.2 there and
+// 9.5, 9.8, 9.9 here. One and two tokens (Ints) are always the GEMV's: 8192 x 8192 11.4 and 12.8 us.
 template <uint32_t TYPE, bool XB>
 cudaError_t launch_tokens(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s) {
-    constexpr int T1 = XB ? 8 : 4;
-    if (a.n_tok > 2 * T1) {  // up to 64 tokens: 8 product tiles in bf16, 16 in f32
-        const int tiles = (a.n_tok + T1 - 1) / T1;
-        if (tiles <= 4) return launch_gemm<TYPE, XB, 4>(a, ws, sm_count, s);
-        if (tiles <= 6) return launch_gemm<TYPE, XB, 6>(a, ws, sm_count, s);
-        if (tiles <= 8) return launch_gemm<TYPE, XB, 8>(a, ws, sm_count, s);
-        if constexpr (!XB) {
-            if (tiles <= 12) return launch_gemm<TYPE, XB, 12>(a, ws, sm_count, s);
-            return launch_gemm<TYPE, XB, 16>(a, ws, sm_count, s);
+    const int n = a.n_tok, columns = XB ? n : 2 * n;
+    if (n == 1) return launch_gemv<TYPE, XB, Ints<TYPE, XB, 1>>(a, sm_count, s);
+    if (n == 2) return launch_gemv<TYPE, XB, Ints<TYPE, XB, 2>>(a, sm_count, s);
+    if (columns <= 16 && (long long)columns * a.cols < 48 * 1024) {
+        if constexpr (XB) {
+            if (columns <= 4) return launch_gemv<TYPE, XB, Halves<TYPE, XB, 4>>(a, sm_count, s);
         }
+        if (columns <= 8) return launch_gemv<TYPE, XB, Halves<TYPE, XB, 8>>(a, sm_count, s);
+        return launch_gemv<TYPE, XB, Halves<TYPE, XB, 16>>(a, sm_count, s);
     }
-    // 16 columns where their activations fit the cluster's shared memory, else 8 at a time
-    const int KT = (a.cols + kUnitCols - 1) / kUnitCols;
-    const int most = ((KT + 7) / 8) * Halves<TYPE, XB, 16>::BYTES <= 160 * 1024 ? 2 * T1 : T1;
-    for (int t0 = 0; t0 < a.n_tok; t0 += most) {
-        const int nt = a.n_tok - t0 < most ? a.n_tok - t0 : most, cols = XB ? nt : 2 * nt;
-        const cudaError_t e = nt == 1     ? launch_gemv<TYPE, XB, Ints<TYPE, XB, 1>>(a, t0, nt, sm_count, s)
-                              : nt == 2   ? launch_gemv<TYPE, XB, Ints<TYPE, XB, 2>>(a, t0, nt, sm_count, s)
-                              : cols <= 4 ? launch_gemv<TYPE, XB, Halves<TYPE, XB, 4>>(a, t0, nt, sm_count, s)
-                              : cols <= 8 ? launch_gemv<TYPE, XB, Halves<TYPE, XB, 8>>(a, t0, nt, sm_count, s)
-                                          : launch_gemv<TYPE, XB, Halves<TYPE, XB, 16>>(a, t0, nt, sm_count, s);
-        if (e != cudaSuccess) return e;
-    }
-    return cudaSuccess;
+    if (n <= 16) return launch_tc<TYPE, XB, 16>(a, ws, sm_count, s);
+    if (n <= 32) return launch_tc<TYPE, XB, 32>(a, ws, sm_count, s);
+    return launch_tc<TYPE, XB, 64>(a, ws, sm_count, s);
 }
 
 uint64_t padded_units(uint64_t rows, uint64_t cols) {
-    return (rows + kTileRows - 1) / kTileRows * ((cols + kUnitCols - 1) / kUnitCols);
+    constexpr uint64_t block = kTileRows * kBlockTiles;
+    return (rows + block - 1) / block * kBlockTiles * ((cols + kUnitCols - 1) / kUnitCols);
 }
 
 }  // namespace
@@ -1077,8 +1205,7 @@ cudaError_t launch_q4_repack(uint32_t type, const uint8_t *raw, uint32_t rows, u
 }
 
 uint64_t q4_workspace_bytes(uint64_t cols) {
-    // 64 tokens in f32: 128 product columns of 64 B in each of a unit's groups, and 64 sums
-    return kQ4InvBytes + (cols + kUnitCols - 1) / kUnitCols * (4 * (128 * 64 + 64 * 4));
+    return kQ4InvBytes + (cols + kUnitCols - 1) / kUnitCols * Tc<GX_Q4_1, false, 64>::BU;
 }
 
 cudaError_t launch_q4_linear(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s) {

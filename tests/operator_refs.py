@@ -43,7 +43,9 @@ def q4_weights(packed, kind, cols):
 def linear(x, w, mag, y_kind):
     """y and its bound. A group of 32 columns is summed in at most two matrix products of 17 terms with
     f32 accumulators that may truncate (34 * 2 u), the groups in a chain of up to cols / 32 additions,
-    and an activation keeps 22 bits of its token's largest value or better (2^-23 of it)."""
+    and an activation keeps 22 bits of its token's largest value or better (2^-23 of it). More tokens are
+    summed in steps of 16 terms whose truncations may point alike, cols / 8 * 2 u at worst; they are held to
+    the same bound."""
     x = x.astype(np.float64)
     y = x @ w.T
     s = np.abs(x) @ mag.T

@@ -90,6 +90,32 @@ def test_linear_long(ctx, rows, cols, n):
         check_linear(ctx, refs.Q4_0 if n != 3 else refs.Q4_1, rows, cols, n, xk, "f32", seed=cols)
 
 
+@pytest.mark.parametrize("kind", [refs.Q4_0, refs.Q4_1])
+@pytest.mark.parametrize("n,xk", [(12, "f32"), (30, "f32"), (64, "f32"), (20, "bf16"), (64, "bf16")])
+def test_linear_more_row_blocks_than_multiprocessors(ctx, kind, n, xk):
+    check_linear(ctx, kind, 40009, 160, n, xk, "f32", seed=n)
+
+
+@pytest.mark.parametrize("n,xk", [(2, "f32"), (4, "f32"), (16, "f32"), (40, "bf16")])
+@pytest.mark.parametrize("kind", [refs.Q4_0, refs.Q4_1])
+def test_linear_scales_at_the_ends_of_fp16(ctx, kind, n, xk):
+    """Group scales from the smallest subnormal to the largest fp16, and offsets of Q4_1 alike."""
+    rng = np.random.default_rng(n)
+    rows, cols = 150, 608
+    packed, _, _ = refs.q4_matrix(3, kind, rows, cols)
+    blocks = packed.reshape(rows, cols // 32, refs.BLOCK[kind]).copy()
+    ends = np.array([2.0 ** -24, 3 * 2.0 ** -24, 1023 * 2.0 ** -24, 2.0 ** -14, 1.0, 2047.0, 65504.0, -65504.0, -2.0 ** -24, 0.0], np.float16)
+    for at in range(0, refs.BLOCK[kind] - 16, 2):
+        blocks[:, :, at:at + 2] = ends[rng.integers(0, len(ends), blocks.shape[:2] + (1,))].view(np.uint8)
+    packed = blocks.reshape(rows, -1)
+    w, mag = refs.q4_weights(packed, kind, cols)
+    x = refs.to_kind(rng.standard_normal((n, cols)), xk)
+    h = ctx.upload_matrix(kind, rows, cols, packed)
+    y = torch.empty(n, rows, device="cuda")
+    ctx.wait(ctx.linear(h, dev(x, xk), y))
+    near(y, *refs.linear(x, w, mag, "f32"))
+
+
 @pytest.mark.parametrize("n", [1, 7, 40])
 def test_linear_strides_and_alignment(ctx, n):
     """Rows of wider buffers at odd strides, and buffers that start at an odd element."""
