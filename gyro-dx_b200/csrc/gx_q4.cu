@@ -715,7 +715,7 @@ cudaError_t launch_gemv(const Q4Args &a, int sm_count, cudaStream_t s) {
 // against 26 in bf16. On mma.sync the same products took 71 and 48 us.)
 //
 // What bounds it: the chain of one unit (128 columns) in the issuing thread, two waits, 16 MMAs and two
-// commits, 0.5 us; the MMAs themselves would take a third of that, the codes' bytes a tenth. So a unit has
+// commits, 0.5 us; the MMAs at their full rate would take 0.15 us, the codes' bytes 0.18. So a unit has
 // one full and one empty barrier for its weights, its codes come by one bulk copy (a copy for each of its 8
 // row tiles kept the copying thread 0.9 us a unit), and one thread runs the issue loop by itself (a whole
 // warp with an elected lane: 32 us against 28).
@@ -928,6 +928,8 @@ __global__ void __launch_bounds__((Tc<TYPE, XB, TP>::THREADS), 1) q4_tc_kernel(Q
     };
     auto wait_all = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
     const int total = items * nu;  // units, item by item
+    // No bounded wait starts before the activations can be packed, however long the kernel before takes.
+    if (warp != 0) pdl_wait();
 
     if (warp == 0) {
         if (lane == 0) {
@@ -1049,7 +1051,6 @@ __global__ void __launch_bounds__((Tc<TYPE, XB, TP>::THREADS), 1) q4_tc_kernel(Q
         }
     } else {
         const int lg = warp & 3, i = 32 * lg + lane;
-        pdl_wait();
         for (int t = i; t < TP; t += kTcRows) inv[t] = t < a.n_tok ? __ldcg(reinterpret_cast<const float *>(ws) + t) : 0.f;
         asm volatile("bar.sync 1, 128;" ::: "memory");
         for (int item = 0; item < items; ++item) {

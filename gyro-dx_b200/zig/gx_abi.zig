@@ -21,6 +21,15 @@ pub const e_range: gx_result = -10;
 pub const dtype_f32: u32 = 0;
 pub const dtype_q8_0: u32 = 8;
 pub const dtype_bf16: u32 = 30;
+/// 4-bit matrices of gx_upload_matrix (GGUF type ids).
+pub const type_q4_0: u32 = 2;
+pub const type_q4_1: u32 = 3;
+pub const res_post_norm: u32 = 1;
+pub const gate_none: u32 = 0;
+pub const gate_token: u32 = 1;
+pub const gate_element: u32 = 2;
+pub const no_token: u32 = 0xffffffff;
+pub const max_top: u32 = 32;
 pub const flag_profile: u32 = 1;
 pub const ep_none: u32 = 0;
 pub const ep_nccl: u32 = 1;
@@ -126,6 +135,72 @@ pub const gx_timings = extern struct {
     layers: u64,
 };
 
+pub const gx_norm_desc = extern struct {
+    x: ?*const anyopaque,
+    y: ?*anyopaque,
+    weight: ?[*]const f32,
+    gate_weight: ?[*]const f32,
+    gate: ?[*]f32,
+    x_stride: u64,
+    y_stride: u64,
+    x_dtype: u32,
+    y_dtype: u32,
+    n_embd: u32,
+    eps: f32,
+};
+
+pub const gx_residual_desc = extern struct {
+    y: ?*const anyopaque,
+    res: ?*const anyopaque,
+    res_out: ?*anyopaque,
+    gate: ?*const anyopaque,
+    post: ?[*]const f32,
+    out: ?*anyopaque,
+    next: ?[*]const f32,
+    next_gate_weight: ?[*]const f32,
+    next_gate: ?[*]f32,
+    y_stride: u64,
+    res_stride: u64,
+    res_out_stride: u64,
+    gate_stride: u64,
+    out_stride: u64,
+    y_dtype: u32,
+    res_dtype: u32,
+    gate_dtype: u32,
+    out_dtype: u32,
+    n_embd: u32,
+    flags: u32,
+    gate_kind: u32,
+    eps: f32,
+    res_scale: f32,
+    block_scale: f32,
+};
+
+pub const gx_logprobs_desc = extern struct {
+    logits: ?*const anyopaque,
+    tokens: ?[*]const u32,
+    logprob: ?[*]f32,
+    rank: ?[*]u32,
+    entropy: ?[*]f32,
+    top_ids: ?[*]u32,
+    top_logprobs: ?[*]f32,
+    stride: u64,
+    dtype: u32,
+    n_vocab: u32,
+    n_top: u32,
+    scale: f32,
+};
+
+pub const gx_norms_desc = extern struct {
+    pre: ?[*]const f32,
+    post: ?[*]const f32,
+    gate: ?[*]const f32,
+    post_norm: u32,
+    eps: f32,
+    res_scale: f32,
+    block_scale: f32,
+};
+
 pub extern fn gx_create(options: *const gx_options, context: *?*gx_context) gx_result;
 pub extern fn gx_get_caps(context: *gx_context, caps: *gx_caps) gx_result;
 pub extern fn gx_upload_layer(context: *gx_context, layer: u32, desc: *const gx_layer_desc, timeout_ms: u32) gx_result;
@@ -153,6 +228,14 @@ pub extern fn gx_upload_matrix(context: *gx_context, type_id: u32, rows: u32, co
     packed_bytes: u64, handle: *u32, timeout_ms: u32) gx_result;
 pub extern fn gx_matvec(context: *gx_context, handle: u32, x: [*]const f32, n_tok: u32, y: [*]f32,
     ticket: ?*u64) gx_result;
+pub extern fn gx_linear(context: *gx_context, handle: u32, x: ?*const anyopaque, x_dtype: u32, x_stride: u64,
+    n_tok: u32, y: ?*anyopaque, y_dtype: u32, y_stride: u64, ticket: ?*u64) gx_result;
+pub extern fn gx_norm(context: *gx_context, desc: *const gx_norm_desc, n_tok: u32, ticket: ?*u64) gx_result;
+pub extern fn gx_norm_residual(context: *gx_context, desc: *const gx_residual_desc, n_tok: u32, ticket: ?*u64) gx_result;
+pub extern fn gx_logprobs(context: *gx_context, desc: *const gx_logprobs_desc, n_rows: u32, ticket: ?*u64) gx_result;
+pub extern fn gx_upload_norms(context: *gx_context, layer: u32, desc: ?*const gx_norms_desc, timeout_ms: u32) gx_result;
+pub extern fn gx_norm_block(context: *gx_context, first_layer: u32, n_layers: u32, res: ?[*]f32, n_tok: u32,
+    ticket: ?*u64) gx_result;
 pub extern fn gx_read_timings(context: *gx_context, timings: *gx_timings) gx_result;
 pub extern fn gx_comm_unique_id(out_id: [*]u8, bytes: u64) gx_result;
 pub extern fn gx_read_expert_counts(context: *gx_context, layer: u32, counts: [*]u32, reset: u32,
@@ -179,4 +262,11 @@ comptime {
     assert(@sizeOf(gx_gguf_layer_info) == 40);
     assert(@sizeOf(gx_hc_desc) == 72);
     assert(@offsetOf(gx_hc_desc, "down_bytes") == 48);
+    assert(@sizeOf(gx_norm_desc) == 72);
+    assert(@offsetOf(gx_norm_desc, "x_dtype") == 56);
+    assert(@sizeOf(gx_residual_desc) == 152);
+    assert(@offsetOf(gx_residual_desc, "y_dtype") == 112);
+    assert(@sizeOf(gx_logprobs_desc) == 80);
+    assert(@offsetOf(gx_logprobs_desc, "dtype") == 64);
+    assert(@sizeOf(gx_norms_desc) == 40);
 }

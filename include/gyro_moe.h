@@ -334,9 +334,9 @@ GX_API gx_result gx_matvec(gx_context *context, uint32_t handle, const float *x,
  * ticket (out_ticket may be NULL). gx_linear, gx_norm, gx_norm_residual and gx_logprobs allocate no
  * memory and do not wait, so they can be captured into a graph from that stream (with a NULL ticket:
  * a captured call has none, and one that asks for it gets GX_E_STATE). A captured gx_linear of more than
- * 8 tokens packs its activations in a workspace that all calls of the context share: replay such a
- * graph on the context's stream, or ordered against it and against other such graphs. Row strides are in elements, at least
- * the row's width, and pointers need only the alignment of their element type. An output may not
+ * 2 tokens may pack its activations in a workspace that all calls of the context share: replay such a
+ * graph on the context's stream, or ordered against it and against other such graphs. Row strides are in
+ * elements, at least the row's width, and pointers need only the alignment of their element type. An output may not
  * overlap an input or another output except where that is said; such calls are refused. Sums,
  * norms and softmax statistics are f32 or wider, each output is rounded once. */
 

@@ -649,6 +649,51 @@ def test_scoring_run(ctx):
     check(x)
 
 
+def test_batches_in_flight_share_a_workspace(ctx):
+    """Batch products of different sizes one after another without a wait between them, each packing its
+    activations where the one before did, eagerly and as a graph that is replayed on new ones."""
+    work = []
+    for i, (kind, rows, cols, n, xk) in enumerate([(refs.Q4_0, 700, 2048, 40, "f32"), (refs.Q4_1, 130, 4096, 12, "f32"),
+                                                   (refs.Q4_0, 40, 8192, 64, "bf16"), (refs.Q4_1, 1000, 256, 20, "bf16"),
+                                                   (refs.Q4_0, 129, 6144, 5, "f32"), (refs.Q4_0, 2100, 1024, 33, "bf16")]):
+        packed, w, mag = refs.q4_matrix(70 + i, kind, rows, cols)
+        work.append(dict(h=ctx.upload_matrix(kind, rows, cols, packed), w=w, mag=mag, n=n, cols=cols, xk=xk,
+                         xd=dev(refs.to_kind(np.zeros((n, cols)), xk), xk), y=torch.empty(n, rows, device="cuda")))
+
+    def load(seed):
+        for i, s in enumerate(work):
+            s["x"] = refs.to_kind(np.random.default_rng(seed + i).normal(0, 1, (s["n"], s["cols"])), s["xk"])
+            s["xd"].copy_(dev(s["x"], s["xk"]))
+            s["y"].fill_(float("nan"))
+        torch.cuda.synchronize()
+
+    def steps():
+        for _ in range(3):
+            for s in work:
+                ctx.linear(s["h"], s["xd"], s["y"], ticket=False)
+
+    def check():
+        torch.cuda.synchronize()
+        for s in work:
+            near(s["y"], *refs.linear(s["x"], s["w"], s["mag"], "f32"))
+
+    load(1)
+    steps()
+    check()
+    stream = torch.cuda.ExternalStream(ctx.stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+        steps()
+    for seed in (20, 40):
+        load(seed)
+        with torch.cuda.stream(stream):
+            graph.replay()
+        check()
+    load(60)
+    steps()
+    check()
+
+
 def test_two_contexts_at_once():
     """Two contexts' streams with calls in flight together share no workspace."""
     V, n, cols = 30011, 9, 4096
