@@ -704,15 +704,15 @@ cudaError_t launch_gemv(const Q4Args &a, int sm_count, cudaStream_t s) {
 }
 
 // ---- more tokens: a product on tcgen05 ----------------------------------------------------------
-// D[128 rows][N] = sum over all columns of w x, in one accumulator in tensor memory. That asks for weights
+// D[128 rows][N] = sum over the columns of w x, in an accumulator in tensor memory. That asks for weights
 // that the tensor core can take as they are: d (q - 8) has up to 15 significant bits, and two bf16 hold it
 // exactly (Split). Decoder warps write both parts into tensor memory, a lane a row, as A; the packed
 // activations are B in shared memory, one column a token in bf16 and three in f32 (8 bits each, all 24).
-// No weight and no activation is rounded; a sum of 8192 columns is 1024 steps in f32 over the cluster.
+// No weight and no activation is rounded.
 //
-// (With d applied to each group's sum afterwards, as in the GEMV, the product needs one accumulator a
-// group, and warps that read each of them back: 46 us for 64 f32 tokens by 8192 x 8192 against 42, and 42 us
-// against 26 in bf16. On mma.sync the same products took 71 and 48 us.)
+// (With d applied to each group's sum afterwards, as in the GEMV, the product needs an accumulator a group,
+// read back by warps that multiply: 42 us alone on a stream against 26, 64 bf16 tokens by 8192 x 8192, and
+// 48 to 62 on mma.sync.)
 //
 // What bounds it: the chain of one unit (128 columns) in the issuing thread, two waits, 16 MMAs and two
 // commits, 0.5 us; the MMAs at their full rate would take 0.15 us, the codes' bytes 0.18. So a unit has
@@ -723,6 +723,12 @@ cudaError_t launch_gemv(const Q4Args &a, int sm_count, cudaStream_t s) {
 // Warps: 0 copies, 1 tensor memory and MMA issue, then sets of four decoders that take units in turn, and four
 // that read the sums. Three sets: 25.4 us, two: 25.7 (8192 x 8192, 64 bf16 tokens).
 constexpr int kTcRows = kTileRows * kBlockTiles;
+// Units that one accumulator takes before it is read and added in registers. The tensor core cuts its sum off
+// after each of a unit's 16 MMAs, always towards zero: 14 units in one accumulator (13 tokens by 2560 x 10240) gave
+// 2.6e-6 relative error; one, its small parts first, 1.5e-7 (two 2.7e-7), where a product of the unpacked weights in
+// f32 has 3.7e-7. It costs 64 f32 tokens 58 us in place of 49 (two units) or 42 (all). bf16 results, which their
+// rounding moves by 2^-9, take 16: 8192 x 8192 by 64 tokens 23.7 us, and 24.9 with one.
+constexpr int tc_run(bool y_bf16) { return y_bf16 ? 16 : 1; }  // powers of two
 constexpr int kQ4InvBytes = 64 * 4;  // of a workspace: the tokens' inverse scales, before the first unit
 constexpr int kPackThreads = 512;
 
@@ -736,7 +742,7 @@ struct Tc {
     static constexpr int BU = N * 128 * (TYPE == GX_Q4_1 ? 3 : 2);         // a unit's activations
     static constexpr int STAGE = BU + 8 * unit_bytes(TYPE);                 // and the codes of 8 row tiles
     static constexpr int XS = (kMaxSmem - 4096) / STAGE < 6 ? (kMaxSmem - 4096) / STAGE : 6;
-    static constexpr int SLOTS = N <= 64 ? 2 : 1, SLOT = (N + 31) / 32 * 32;  // accumulators, their TMEM columns
+    static constexpr int SLOTS = N <= 96 ? 2 : 1, SLOT = (N + 31) / 32 * 32;  // accumulators, their TMEM columns
     static constexpr int AC = TYPE == GX_Q4_1 ? 144 : 128;                  // TMEM columns of a unit's weights
     static constexpr int AS = (512 - SLOTS * SLOT) / AC;                    // stages of those
     // A set that is ahead of a ring by more than one turn would take the parity of the turn before for its own.
@@ -874,6 +880,7 @@ struct Split {
 
 struct TcPlan {
     int RT, KT, blocks, S;
+    int run;  // units of an accumulator
 };
 
 template <uint32_t TYPE, bool XB, int TP>
@@ -961,34 +968,32 @@ __global__ void __launch_bounds__((Tc<TYPE, XB, TP>::THREADS), 1) q4_tc_kernel(Q
         constexpr uint32_t idesc = f16_idesc(kTcRows, C::N) | (1u << 7) | (1u << 10);  // A and B are bf16
         constexpr uint32_t idesc_lo = TYPE == GX_Q4_1 ? idesc | (1u << 13) : idesc;     // A negated
         bool ok = true;
-        for (int item = 0, n = 0; ok && item < items; ++item) {
-            const int slot = item % C::SLOTS;
+        for (int n = 0, u = 0, run = 0; ok && n < total; ++n) {
+            const int sx = n % XS, sa = n % AS, slot = run % C::SLOTS, first_unit = (u & (p.run - 1)) == 0;
             const uint32_t dst = tmem + (uint32_t)(slot * C::SLOT);
-            ok = wait(&empty_d[slot], (uint32_t)(item / C::SLOTS & 1) ^ 1u);
-            for (int u = 0; ok && u < nu; ++u, ++n) {
-                const int sx = n % XS;
-                const int sa = n % AS;
-                ok = wait(&full_x[sx], (uint32_t)(n / XS & 1)) && wait(&full_a[sa], (uint32_t)(n / AS & 1));
-                if (!ok) break;
-                tc_fence_after();
-                const uint64_t xd = sw128_desc(smem_u32(sm + sx * C::STAGE));
-                const uint32_t at = a_cols + (uint32_t)(C::AC * sa);
-                // k-step k: half k / 4 of the unit, 32 bytes further in every 128-byte row
+            if (first_unit) ok = wait(&empty_d[slot], (uint32_t)(run / C::SLOTS & 1) ^ 1u);
+            ok = ok && wait(&full_x[sx], (uint32_t)(n / XS & 1)) && wait(&full_a[sa], (uint32_t)(n / AS & 1));
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t xd = sw128_desc(smem_u32(sm + sx * C::STAGE));
+            const uint32_t at = a_cols + (uint32_t)(C::AC * sa);
+            // k-step k: half k / 4 of the unit, 32 bytes further in every 128-byte row. The small parts come first,
+            // and m before the codes that it offsets: what an MMA cuts off goes by the sum so far.
+            auto step_b = [&](int k) { return xd + (uint64_t)((k >> 2) * (C::N * 128 >> 4) + 2 * (k & 3)); };
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    umma_f16_ts(dst, at + 8u * k, xd + (uint64_t)((k >> 2) * (C::N * 128 >> 4) + 2 * (k & 3)), idesc, (u | k) != 0);
+            for (int k = 0; k < 8; ++k) umma_f16_ts(dst, at + 64u + 8u * k, step_b(k), idesc_lo, !(first_unit && k == 0));
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    umma_f16_ts(dst, at + 64u + 8u * k, xd + (uint64_t)((k >> 2) * (C::N * 128 >> 4) + 2 * (k & 3)), idesc_lo, 1u);
-                if constexpr (TYPE == GX_Q4_1) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) umma_f16_ts(dst, at + 128u + 8u * h, xd + (uint64_t)(2 * (C::N * 128 >> 4) + 2 * h), idesc, 1u);
-                }
-                umma_commit(&empty_a[sa]);
-                umma_commit(&empty_x[sx]);
+            for (int k = 0; k < 8; ++k) {
+                if (TYPE == GX_Q4_1 && k % 4 == 0) umma_f16_ts(dst, at + 128u + 2u * k, step_b(8 + k / 4), idesc, 1u);
+                umma_f16_ts(dst, at + 8u * k, step_b(k), idesc, 1u);
             }
-            if (ok) umma_commit(&full_d[slot]);
-            
+            umma_commit(&empty_a[sa]);
+            umma_commit(&empty_x[sx]);
+            u = u + 1 == nu ? 0 : u + 1;
+            if (u == 0 || (u & (p.run - 1)) == 0) {
+                umma_commit(&full_d[slot]);
+                ++run;
+            }
         }
         // all issued MMAs complete before TMEM is released
         umma_commit(done);
@@ -1053,38 +1058,38 @@ __global__ void __launch_bounds__((Tc<TYPE, XB, TP>::THREADS), 1) q4_tc_kernel(Q
         const int lg = warp & 3, i = 32 * lg + lane;
         for (int t = i; t < TP; t += kTcRows) inv[t] = t < a.n_tok ? __ldcg(reinterpret_cast<const float *>(ws) + t) : 0.f;
         asm volatile("bar.sync 1, 128;" ::: "memory");
-        for (int item = 0; item < items; ++item) {
-            const int slot = item % C::SLOTS, row = (first + item * step) * kTcRows + i;
-            if (!wait_all(&full_d[slot], (uint32_t)(item / C::SLOTS & 1))) break;
-            tc_fence_after();
-            const uint32_t at = tmem + ((uint32_t)(32 * lg) << 16) + (uint32_t)(slot * C::SLOT);
+        bool ok = true;
+        for (int item = 0, run = 0; ok && item < items; ++item) {
+            const int row = (first + item * step) * kTcRows + i;
+            float acc[TP];
 #pragma unroll
-            for (int t0 = 0; t0 < TP; t0 += 16) {
-                uint32_t v[16];
-                tmem_ld16(at + (uint32_t)t0, v);
-                tmem_wait_ld();
-                if constexpr (!XB) {
+            for (int t = 0; t < TP; ++t) acc[t] = 0.f;
+            for (int u = 0; u < nu; u += p.run, ++run) {
+                const int slot = run % C::SLOTS;
+                ok = wait_all(&full_d[slot], (uint32_t)(run / C::SLOTS & 1));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t at = tmem + ((uint32_t)(32 * lg) << 16) + (uint32_t)(slot * C::SLOT);
 #pragma unroll
-                    for (int piece = 1; piece < 3; ++piece) {
-                        uint32_t x[16];
-                        tmem_ld16(at + (uint32_t)(piece * TP + t0), x);
-                        tmem_wait_ld();
+                for (int t0 = 0; t0 < C::N; t0 += 16) {  // in f32 the parts of a token lie TP apart
+                    uint32_t v[16];
+                    tmem_ld16(at + (uint32_t)t0, v);
+                    tmem_wait_ld();
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) + __uint_as_float(x[k]));
-                    }
+                    for (int k = 0; k < 16; ++k) acc[(t0 + k) % TP] += __uint_as_float(v[k]);
                 }
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const int tok = t0 + k;
-                    if (tok >= a.n_tok) break;
-                    const float y = __uint_as_float(v[k]) * inv[tok];
-                    if (p.S > 1) red[tok * kTcRows + i] = y;
-                    else if (row < a.rows) store_act(a.y, a.y_bf16, (size_t)tok * a.ldy + row, y);
-                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty_d[slot]);
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&empty_d[slot]);
+            if (!ok) break;
+#pragma unroll
+            for (int t = 0; t < TP; ++t) {
+                if (t >= a.n_tok) break;
+                const float y = acc[t] * inv[t];
+                if (p.S > 1) red[t * kTcRows + i] = y;
+                else if (row < a.rows) store_act(a.y, a.y_bf16, (size_t)t * a.ldy + row, y);
+            }
         }
     }
     tc_fence_before();
@@ -1131,9 +1136,10 @@ cudaError_t launch_tc(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s
     p.RT = (a.rows + kTileRows - 1) / kTileRows;
     p.KT = (a.cols + kUnitCols - 1) / kUnitCols;
     p.blocks = (p.RT + 7) / 8;
+    p.run = tc_run(a.y_bf16 != 0);
     // One CTA an SM. Where row blocks leave SMs idle, the CTAs of a cluster split the units (down to two a
     // CTA). 148 SMs take 130 to 135 CTAs at once in clusters of 3 to 6, but 120 in clusters of 8: 16 row blocks
-    // of 8192 columns by 64 tokens took 24 us with 8 (two waves), 15.2 with 6.
+    // of 8192 columns by 64 tokens took 24 us with 8 (two waves), 15.8 with 6.
     p.S = 1;
     for (int c = 2; c <= 6; ++c)
         if (p.blocks * c <= (c == 2 ? sm_count : sm_count * 7 / 8) && p.KT >= 2 * c) p.S = c;
