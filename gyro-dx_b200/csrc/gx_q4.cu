@@ -24,6 +24,7 @@
 #include "gx_dense.cuh"
 #include "gx_device.cuh"
 #include "gx_internal.h"
+#include "gx_q4_tc.h"
 #include "gx_umma.cuh"
 
 namespace gx {
@@ -41,7 +42,6 @@ namespace {
 //   [8 g][4 groups][row g, row g + 8] fp16 d
 //   [8 g][4 groups][row g, row g + 8] fp16 m   (Q4_1)
 constexpr int kUnitCols = 128, kTileRows = 16, kBlockTiles = 8;
-__host__ __device__ constexpr int unit_bytes(uint32_t type) { return type == GX_Q4_0 ? 1152 : 1280; }
 // Number of the unit u of the row tile rt, of KT units in a row.
 __host__ __device__ constexpr long long unit_index(long long rt, int u, int KT) {
     return (rt / kBlockTiles * KT + u) * kBlockTiles + rt % kBlockTiles;
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(256) q4_repack_kernel(uint32_t type, const uin
     const int NG = (cols + kUnitCols - 1) / kUnitCols * 4;
     const long long row = i / NG;
     const int grp = (int)(i % NG), g = (int)(row & 7), hi = (int)(row >> 3) & 1, j = grp & 3;
-    uint8_t *u = w + unit_index(row / kTileRows, grp / 4, NG / 4) * unit_bytes(type);
+    uint8_t *u = w + unit_index(row / kTileRows, grp / 4, NG / 4) * q4_unit_bytes(type);
     uint32_t words[4] = {0u, 0u, 0u, 0u};
     uint16_t d = 0, m = 0;
     if (row < rows && grp < cols / 32) {
@@ -497,7 +497,7 @@ struct Halves {
     }
 };
 
-constexpr int kMaxSmem = 227 * 1024, kStaticSmem = 1024;  // of a CTA; what of it is not dynamic, at most
+constexpr int kStaticSmem = 1024;  // of a CTA, what is not dynamic, at most
 
 // Lets a kernel use all of it, once per device (a call for every launch costs 0.5 us).
 struct SmemLimit {
@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(W * 32, M::CTAS(W)) q4_gemv_kernel(Q4Args a, G
     const int rt0 = (int)(blockIdx.x / p.S) * groups + wg;
 
     // cursor of the loads: the next unit of this warp, units left of its row tile, the row tile
-    constexpr int UB = unit_bytes(TYPE);
+    constexpr int UB = q4_unit_bytes(TYPE);
     const bool idle = wk >= nu;  // more warps than units: this one only takes part in the sums
     const int per = idle ? 0 : (nu - wk + p.WK - 1) / p.WK, scale = 1024 + M::scale_offset(lane) - lane * 16;
     auto tile_at = [&](int rt) { return a.w + unit_index(rt, u0 + wk, p.KT) * UB + lane * 16; };
@@ -732,26 +732,6 @@ constexpr int tc_run(bool y_bf16) { return y_bf16 ? 16 : 1; }  // powers of two
 constexpr int kQ4InvBytes = 64 * 4;  // of a workspace: the tokens' inverse scales, before the first unit
 constexpr int kPackThreads = 512;
 
-// Activations of a unit: two tiles of 64 columns (two groups), [N rows][128 B] in the 128-byte swizzle, row
-// t + TP p part p of token t, a group's 8 columns of q as the 16-byte chunk 4 (group & 1) + q in the order
-// (0,4) (1,5) (2,6) (3,7), as a word of codes is unpacked; Q4_1: a third tile, chunk j the group sums of group
-// j in three parts, as m multiplies them.
-template <uint32_t TYPE, bool XB, int TP>
-struct Tc {
-    static constexpr int N = XB ? TP : 3 * TP;
-    static constexpr int BU = N * 128 * (TYPE == GX_Q4_1 ? 3 : 2);         // a unit's activations
-    static constexpr int STAGE = BU + 8 * unit_bytes(TYPE);                 // and the codes of 8 row tiles
-    static constexpr int XS = (kMaxSmem - 4096) / STAGE < 6 ? (kMaxSmem - 4096) / STAGE : 6;
-    static constexpr int SLOTS = N <= 96 ? 2 : 1, SLOT = (N + 31) / 32 * 32;  // accumulators, their TMEM columns
-    static constexpr int AC = TYPE == GX_Q4_1 ? 144 : 128;                  // TMEM columns of a unit's weights
-    static constexpr int AS = (512 - SLOTS * SLOT) / AC;                    // stages of those
-    // A set that is ahead of a ring by more than one turn would take the parity of the turn before for its own.
-    static constexpr int RING = XS < AS ? XS : AS, SETS = RING < 3 ? RING : 3;
-    static constexpr int THREADS = (6 + 4 * SETS) * 32;
-    static constexpr int BARS = XS * STAGE;
-    static constexpr int BYTES = BARS + 512 + 1024;                         // and the alignment
-};
-
 // One CTA per token: its values at the power of two that brings the largest to 2^14..2^15 (a token with an
 // Inf or NaN is all NaN), in bf16 parts.
 template <uint32_t TYPE, bool XB, int TP>
@@ -886,7 +866,7 @@ struct TcPlan {
 template <uint32_t TYPE, bool XB, int TP>
 __global__ void __launch_bounds__((Tc<TYPE, XB, TP>::THREADS), 1) q4_tc_kernel(Q4Args a, const uint8_t *ws, TcPlan p) {
     using C = Tc<TYPE, XB, TP>;
-    constexpr int UB = unit_bytes(TYPE), XS = C::XS, AS = C::AS;
+    constexpr int UB = q4_unit_bytes(TYPE), XS = C::XS, AS = C::AS;
     extern __shared__ __align__(1024) uint8_t tc_raw[];
     __shared__ float inv[64];
     uint8_t *sm = reinterpret_cast<uint8_t *>(((uintptr_t)tc_raw + 1023) & ~(uintptr_t)1023);
@@ -1200,7 +1180,7 @@ uint64_t q4_row_bytes(uint32_t type, uint64_t cols) {
     return cols / 32 * (type == GX_Q4_0 ? 18 : 20);
 }
 
-uint64_t q4_bytes(uint32_t type, uint64_t rows, uint64_t cols) { return padded_units(rows, cols) * unit_bytes(type); }
+uint64_t q4_bytes(uint32_t type, uint64_t rows, uint64_t cols) { return padded_units(rows, cols) * q4_unit_bytes(type); }
 
 cudaError_t launch_q4_repack(uint32_t type, const uint8_t *raw, uint32_t rows, uint32_t cols, uint8_t *w,
                              cudaStream_t s) {
