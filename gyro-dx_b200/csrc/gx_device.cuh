@@ -147,6 +147,31 @@ __device__ __forceinline__ void fwht128_warp(float (&v)[4], int lane) {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Barriers that whole warps enter together (.aligned): the lanes of a warp meet first, since a loop or branch
+// before may have sent them apart.
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive_relaxed() {  // this CTA has started; nothing is released
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// The n threads (whole warps) of barrier id.
+__device__ __forceinline__ void named_sync(int id, int n) {
+    __syncwarp();
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
+}
+
 // Launch of a kernel of the many-token chain (router .. combine, and the expert-parallel
 // exchange kernels) with programmatic dependent launch: the kernel may be scheduled while its
 // predecessor on the stream still runs, and every such kernel calls pdl_launch_dependents() first

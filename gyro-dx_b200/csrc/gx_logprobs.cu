@@ -107,11 +107,6 @@ struct Vec<__nv_bfloat16> {
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-__device__ __forceinline__ uint32_t lp_cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
 __device__ __forceinline__ uint32_t peer_addr(const void *p, uint32_t rank) {
     uint32_t at;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
@@ -123,11 +118,6 @@ __device__ __forceinline__ void st_peer(uint32_t at, uint32_t v) {
 __device__ __forceinline__ void st_peer(uint32_t at, u64 v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
 }
-__device__ __forceinline__ void lp_cluster_sync() {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
-}
-
 // The best 32 keys of two falling lists, a key in a lane, as a falling list: one against the other
 // reversed leaves the best 32 in a bitonic order, which five exchanges sort.
 __device__ __forceinline__ u64 merge_lists(u64 a, u64 b, int lane) {
@@ -204,7 +194,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(LogprobsArgs a,
     __shared__ Part parts[kLpMaxCluster];
     static_assert(kLpMaxCluster >= kLpWarps && kMaxTop == 32, "a list is a warp wide");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rank = C > 1 ? (int)lp_cluster_rank() : 0;
+    const int rank = C > 1 ? (int)cluster_rank() : 0;
     const size_t r = blockIdx.x / C;
     const int V = a.n_vocab;
     // this CTA's logits [i0, i1) of the row: 16-byte words in the middle, single logits at the ends
@@ -214,7 +204,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(LogprobsArgs a,
     const int head = min(n, (int)((16 - ((uintptr_t)src & 15)) & 15) / SZ);
     const int words = (n - head) / N, tail0 = head + words * N;
     const uint4 *word = reinterpret_cast<const uint4 *>(src + head);
-    if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA has started
+    if (C > 1) cluster_arrive_relaxed();
     pdl_launch_dependents();
     pdl_wait();
     uint4 next[kLpAhead];
@@ -385,7 +375,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(LogprobsArgs a,
     __syncthreads();
     u64 best = TOP ? merge_all(lists, kLpWarps, warp, lane) : 0;
     // into the first CTA's parts
-    if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (C > 1) cluster_wait();
     if (warp == 0) {
         // the warps' sums, one in a lane
         float m = lane < kLpWarps ? redf[0][lane] : -CUDART_INF_F, ss = lane < kLpWarps ? redf[2][lane] : 0.f;
@@ -417,7 +407,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(LogprobsArgs a,
             parts[0].above = ab;
         }
     }
-    if (C > 1) lp_cluster_sync();
+    if (C > 1) cluster_sync_all();
     else __syncthreads();
     if (rank != 0) return;
     // the row: every thread computes the same totals

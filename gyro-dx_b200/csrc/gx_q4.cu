@@ -526,14 +526,6 @@ __device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
-}
 __device__ __forceinline__ float ld_cluster(const float *p, uint32_t rank) {
     uint32_t at;
     float v;
@@ -602,11 +594,8 @@ __global__ void __launch_bounds__(W * 32, M::CTAS(W)) q4_gemv_kernel(Q4Args a, G
     auto finish = [&]() {  // the row tile rt is complete in this warp
         float *mine = red + (size_t)(parity * W + warp) * RED;
         m.put(mine, lane);
-        if (p.WK > 1) {
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + wg), "r"(32 * p.WK) : "memory");
-        } else {
-            __syncwarp();
-        }
+        if (p.WK > 1) named_sync(1 + wg, 32 * p.WK);
+        else __syncwarp();
         const float *all = red + (size_t)(parity * W + wg * p.WK) * RED;
         float *keep = red + (size_t)(parity * W + wg * p.WK) * RED;
         for (int i = wk * 32 + lane; i < 16 * a.n_tok; i += 32 * p.WK) {
@@ -616,7 +605,7 @@ __global__ void __launch_bounds__(W * 32, M::CTAS(W)) q4_gemv_kernel(Q4Args a, G
             else if (rt * 16 + (i & 15) < a.rows)
                 store_act(a.y, a.y_bf16, (size_t)(i >> 4) * a.ldy + rt * 16 + (i & 15), s);
         }
-        if (p.WK == 1) __syncwarp();
+        __syncwarp();  // the product of the next unit takes a whole warp
         parity ^= 1;
         rt += step;
         m.clear();
@@ -1037,7 +1026,7 @@ __global__ void __launch_bounds__((Tc<TYPE, XB, TP>::THREADS), 1) q4_tc_kernel(Q
     } else {
         const int lg = warp & 3, i = 32 * lg + lane;
         for (int t = i; t < TP; t += kTcRows) inv[t] = t < a.n_tok ? __ldcg(reinterpret_cast<const float *>(ws) + t) : 0.f;
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        named_sync(1, 128);
         bool ok = true;
         for (int item = 0, run = 0; ok && item < items; ++item) {
             const int row = (first + item * step) * kTcRows + i;
