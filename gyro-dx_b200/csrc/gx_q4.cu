@@ -974,7 +974,8 @@ __global__ void __launch_bounds__((Tc<TYPE, XB, TP>::THREADS), 1) q4_tc_kernel(Q
         // decoders: row i of the block
         const int set = (warp - 2) >> 2, lg = warp & 3, i = 32 * lg + lane, r = i & 15, rot = (r >> 1) & 3, sh = r & 8 ? 16 : 0;
         for (int n = set; n < total; n += C::SETS) {
-            const int sx = n % XS;
+            const int sx = n % XS, sa = n % AS;
+            if (C::FREE_FIRST && !wait_all(&empty_a[sa], (uint32_t)(n / AS & 1) ^ 1u)) break;
             if (!wait_all(&full_x[sx], (uint32_t)(n / XS & 1))) break;
             // 64 bytes of the row's codes: word j of 16-byte part q are columns 8 q .. of group j. The lanes
             // start at different parts, so that 8 of them read all banks.
@@ -993,8 +994,7 @@ __global__ void __launch_bounds__((Tc<TYPE, XB, TP>::THREADS), 1) q4_tc_kernel(Q
                 c[2] = sel(two, e[0], e[2]);
                 c[3] = sel(two, e[1], e[3]);
             }
-            const int sa = n % AS;
-            if (!wait_all(&empty_a[sa], (uint32_t)(n / AS & 1) ^ 1u)) break;
+            if (!C::FREE_FIRST && !wait_all(&empty_a[sa], (uint32_t)(n / AS & 1) ^ 1u)) break;
             tc_fence_after();
             const uint32_t at = a_cols + ((uint32_t)(32 * lg) << 16) + (uint32_t)(C::AC * sa);
             uint32_t mv[16];

@@ -98,13 +98,16 @@ int walk(int total, uint64_t slow, uint64_t seed) {
         }
         const int d = who - 4, w = d % W, n = dn[d];
         if (n >= total) return false;
-        if (dstep[d] == 0) {
+        // a decoder waits for its codes and for its stage of weights, in the order of the header
+        const bool free_turn = (dstep[d] == 0) == C::FREE_FIRST;
+        if (free_turn) {
+            if (!empty_a[n % AS].passed((n / AS & 1) ^ 1)) return false;
+            if (done < n - AS + 1) bad = 3;
+        } else {
             if (!full_x[n % XS].passed(n / XS & 1)) return false;
             if (codes[n % XS] != n) bad = 1;
-            return dstep[d] = 1, true;
         }
-        if (!empty_a[n % AS].passed((n / AS & 1) ^ 1)) return false;
-        if (done < n - AS + 1) bad = 3;
+        if (dstep[d] == 0) return dstep[d] = 1, true;
         a[n % AS][w] = n;
         full_a[n % AS].arrive();
         dn[d] += SETS;
