@@ -712,12 +712,12 @@ cudaError_t launch_gemv(const Q4Args &a, int sm_count, cudaStream_t s) {
 // Warps: 0 copies, 1 tensor memory and MMA issue, then sets of four decoders that take units in turn, and four
 // that read the sums. Three sets: 25.4 us, two: 25.7 (8192 x 8192, 64 bf16 tokens).
 constexpr int kTcRows = kTileRows * kBlockTiles;
-// Units that one accumulator takes before it is read and added in registers. The tensor core cuts its sum off
-// after each of a unit's 16 MMAs, always towards zero: 14 units in one accumulator (13 tokens by 2560 x 10240) gave
-// 2.6e-6 relative error; one, its small parts first, 1.5e-7 (two 2.7e-7), where a product of the unpacked weights in
-// f32 has 3.7e-7. It costs 64 f32 tokens 58 us in place of 49 (two units) or 42 (all). bf16 results, which their
-// rounding moves by 2^-9, take 16: 8192 x 8192 by 64 tokens 23.7 us, and 24.9 with one.
-constexpr int tc_run(bool y_bf16) { return y_bf16 ? 16 : 1; }  // powers of two
+// An accumulator takes one unit and is then read and added in registers. The tensor core cuts its sum off after each
+// of a unit's 16 MMAs, always towards zero. Relative error in the 2-norm before the results are rounded (64 bf16 tokens
+// by 8192 x 8192, Q4_0 and Q4_1; a product of the unpacked weights in f32 has 1.5e-6), and time with bf16 results:
+//   one unit 1.3e-7, 2.4e-7, 29.3 us;  four 6.2e-7, 8.6e-7, 28.0;  sixteen 2.7e-6, 3.6e-6, 27.7
+// (64 f32 tokens: 56.9, 45.9, 43.2 us). Sixteen would do for bf16 results, but put twice as many of them on the other
+// side of a rounding's border as the product in f32 does; with one, a bf16 result is the f32 result rounded.
 constexpr int kQ4InvBytes = 64 * 4;  // of a workspace: the tokens' inverse scales, before the first unit
 constexpr int kPackThreads = 512;
 
@@ -849,7 +849,6 @@ struct Split {
 
 struct TcPlan {
     int RT, KT, blocks, S;
-    int run;  // units of an accumulator
 };
 
 template <uint32_t TYPE, bool XB, int TP>
@@ -937,10 +936,10 @@ __global__ void __launch_bounds__((Tc<TYPE, XB, TP>::THREADS), 1) q4_tc_kernel(Q
         constexpr uint32_t idesc = f16_idesc(kTcRows, C::N) | (1u << 7) | (1u << 10);  // A and B are bf16
         constexpr uint32_t idesc_lo = TYPE == GX_Q4_1 ? idesc | (1u << 13) : idesc;     // A negated
         bool ok = true;
-        for (int n = 0, u = 0, run = 0; ok && n < total; ++n) {
-            const int sx = n % XS, sa = n % AS, slot = run % C::SLOTS, first_unit = (u & (p.run - 1)) == 0;
+        for (int n = 0; ok && n < total; ++n) {
+            const int sx = n % XS, sa = n % AS, slot = n % C::SLOTS;
             const uint32_t dst = tmem + (uint32_t)(slot * C::SLOT);
-            if (first_unit) ok = wait(&empty_d[slot], (uint32_t)(run / C::SLOTS & 1) ^ 1u);
+            ok = wait(&empty_d[slot], (uint32_t)(n / C::SLOTS & 1) ^ 1u);
             ok = ok && wait(&full_x[sx], (uint32_t)(n / XS & 1)) && wait(&full_a[sa], (uint32_t)(n / AS & 1));
             if (!ok) break;
             tc_fence_after();
@@ -950,7 +949,7 @@ __global__ void __launch_bounds__((Tc<TYPE, XB, TP>::THREADS), 1) q4_tc_kernel(Q
             // and m before the codes that it offsets: what an MMA cuts off goes by the sum so far.
             auto step_b = [&](int k) { return xd + (uint64_t)((k >> 2) * (C::N * 128 >> 4) + 2 * (k & 3)); };
 #pragma unroll
-            for (int k = 0; k < 8; ++k) umma_f16_ts(dst, at + 64u + 8u * k, step_b(k), idesc_lo, !(first_unit && k == 0));
+            for (int k = 0; k < 8; ++k) umma_f16_ts(dst, at + 64u + 8u * k, step_b(k), idesc_lo, k > 0);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 if (TYPE == GX_Q4_1 && k % 4 == 0) umma_f16_ts(dst, at + 128u + 2u * k, step_b(8 + k / 4), idesc, 1u);
@@ -958,16 +957,11 @@ __global__ void __launch_bounds__((Tc<TYPE, XB, TP>::THREADS), 1) q4_tc_kernel(Q
             }
             umma_commit(&empty_a[sa]);
             umma_commit(&empty_x[sx]);
-            u = u + 1 == nu ? 0 : u + 1;
-            if (u == 0 || (u & (p.run - 1)) == 0) {
-                umma_commit(&full_d[slot]);
-                ++run;
-            }
+            umma_commit(&full_d[slot]);
         }
         // all issued MMAs complete before TMEM is released
         umma_commit(done);
         mbar_wait(done, 0, nullptr);
-        
         }
         __syncwarp();
     } else if (warp < 2 + 4 * C::SETS) {
@@ -1028,14 +1022,14 @@ __global__ void __launch_bounds__((Tc<TYPE, XB, TP>::THREADS), 1) q4_tc_kernel(Q
         for (int t = i; t < TP; t += kTcRows) inv[t] = t < a.n_tok ? __ldcg(reinterpret_cast<const float *>(ws) + t) : 0.f;
         named_sync(1, 128);
         bool ok = true;
-        for (int item = 0, run = 0; ok && item < items; ++item) {
+        for (int item = 0, n = 0; ok && item < items; ++item) {
             const int row = (first + item * step) * kTcRows + i;
             float acc[TP];
 #pragma unroll
             for (int t = 0; t < TP; ++t) acc[t] = 0.f;
-            for (int u = 0; u < nu; u += p.run, ++run) {
-                const int slot = run % C::SLOTS;
-                ok = wait_all(&full_d[slot], (uint32_t)(run / C::SLOTS & 1));
+            for (int u = 0; u < nu; ++u, ++n) {
+                const int slot = n % C::SLOTS;
+                ok = wait_all(&full_d[slot], (uint32_t)(n / C::SLOTS & 1));
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t at = tmem + ((uint32_t)(32 * lg) << 16) + (uint32_t)(slot * C::SLOT);
@@ -1105,7 +1099,6 @@ cudaError_t launch_tc(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s
     p.RT = (a.rows + kTileRows - 1) / kTileRows;
     p.KT = (a.cols + kUnitCols - 1) / kUnitCols;
     p.blocks = (p.RT + 7) / 8;
-    p.run = tc_run(a.y_bf16 != 0);
     // One CTA an SM. Where row blocks leave SMs idle, the CTAs of a cluster split the units (down to two a
     // CTA). 148 SMs take 130 to 135 CTAs at once in clusters of 3 to 6, but 120 in clusters of 8: 16 row blocks
     // of 8192 columns by 64 tokens took 24 us with 8 (two waves), 15.8 with 6.
