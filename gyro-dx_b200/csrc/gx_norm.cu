@@ -36,11 +36,14 @@ __device__ __forceinline__ void store_act(void *p, int bf16, size_t i, float v) 
     else reinterpret_cast<float *>(p)[i] = v;
 }
 
-// 1 / (1 + e^-x) to about 4 units of 2^-24, in 10 instructions (expf and a division take four times as
-// many, which bounds the kernel that gates every element): 2^t with the rounding of t = -x log2 e put back.
+// 1 / (1 + e^-x) in 10 instructions (expf and a division take four times as many, which bounds the kernel that
+// gates every element): 2^t with the rounding of t = -x log2 e put back, off by at most 8 units of 2^-24 (4 of the
+// power of two, 2 of the reciprocal, 1 of each sum). From -88 down, where 2^t would pass the f32 range and its
+// correction with it, x counts as -88: the reciprocal of 2^126.96 is below the smallest normal number, and 0. From
+// 10^4 up (and at Inf, whose remainder would be a NaN) it is 1. A NaN stays one.
 __device__ __forceinline__ float sigmoid(float x) {
     constexpr float l2e = 1.44269504088896341f, l2e_rest = (float)(1.44269504088896341 - (double)1.44269504088896341f);
-    asm("min.NaN.f32 %0, %0, 0f461c4000;\n max.NaN.f32 %0, %0, 0fc61c4000;" : "+f"(x));  // +-10^4: 0 or 1 beyond
+    asm("min.NaN.f32 %0, %0, 0f461c4000;\n max.NaN.f32 %0, %0, 0fc2b00000;" : "+f"(x));  // 10^4, -88
     const float t = -x * l2e, rest = fmaf(-x, l2e_rest, fmaf(-x, l2e, -t));
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
