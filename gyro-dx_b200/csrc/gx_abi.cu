@@ -18,6 +18,7 @@
 #include "gx_comm.h"
 #include "gx_internal.h"
 #include "gx_tile.h"
+#include "gx_upload.h"
 
 namespace {
 
@@ -2583,6 +2584,26 @@ GX_API gx_result gx_logprobs(gx_context *c, const gx_logprobs_desc *d, uint32_t 
     return finish_call(c, capturing, out_ticket);
 }
 
+namespace {
+
+// Device calls of gx::replace_buffer on the context's stream.
+struct StreamUpload {
+    gx_context *c;
+    uint32_t timeout_ms;
+    gx_result alloc(uint64_t bytes, void **p) {
+        GX_CUDA(cudaMalloc(p, bytes));
+        return GX_OK;
+    }
+    gx_result copy(void *dst, const void *src, uint64_t bytes) {
+        GX_CUDA(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyHostToDevice, c->stream));
+        return GX_OK;
+    }
+    gx_result wait() { return sync_all(c, timeout_ms); }
+    void release(void *p) { cudaFree(p); }
+};
+
+}  // namespace
+
 GX_API gx_result gx_upload_norms(gx_context *c, uint32_t layer, const gx_norms_desc *d, uint32_t timeout_ms) {
     if (!c) return GX_E_INVALIDARG;
     if (c->broken) return GX_E_DEVICE;
@@ -2591,28 +2612,21 @@ GX_API gx_result gx_upload_norms(gx_context *c, uint32_t layer, const gx_norms_d
     const uint64_t E = L.E;
     if (d && !gx::norms_args_ok(*d)) return GX_E_INVALIDARG;
     GX_CUDA(cudaSetDevice(c->device));
-    if (L.nm_arena) {
-        gx_result r = sync_all(c, timeout_ms);  // queued blocks may still read the old weights
-        if (r != GX_OK) return r;
-        cudaFree(L.nm_arena);
+    if (d && !c->norm_gate) GX_CUDA(cudaMalloc(&c->norm_gate, (size_t)c->max_tokens * sizeof(float)));
+    if (!d && !L.nm_arena) return GX_OK;
+    StreamUpload up{c, timeout_ms};
+    const uint64_t row = E * sizeof(float);
+    const gx::HostPiece pieces[3] = {{d ? d->pre : nullptr, 0, row}, {d ? d->post : nullptr, row, row}, {d ? d->gate : nullptr, 2 * row, row}};
+    void *held = L.nm_arena;
+    const gx_result r = gx::replace_buffer(up, held, d ? 3 * row : 0, pieces, 3);
+    if (r != GX_OK) return r;
+    float *arena = L.nm_arena = static_cast<float *>(held);
+    if (!d) {
+        L.nm_bytes = 0;
+        L.nm_pre = L.nm_post = L.nm_gate = nullptr;
+        return GX_OK;
     }
-    L.nm_arena = nullptr;
-    L.nm_bytes = 0;
-    L.nm_pre = L.nm_post = L.nm_gate = nullptr;
-    if (!d) return GX_OK;
-    if (!c->norm_gate) GX_CUDA(cudaMalloc(&c->norm_gate, (size_t)c->max_tokens * sizeof(float)));
-    float *arena = nullptr;
-    GX_CUDA(cudaMalloc(&arena, 3 * E * sizeof(float)));
-    const float *src[3] = {d->pre, d->post, d->gate};
-    cudaError_t e = cudaSuccess;
-    for (int i = 0; i < 3 && e == cudaSuccess; ++i)
-        if (src[i]) e = cudaMemcpy(arena + i * E, src[i], E * sizeof(float), cudaMemcpyHostToDevice);
-    if (e != cudaSuccess) {
-        cudaFree(arena);
-        return fail_cuda(c, e);
-    }
-    L.nm_arena = arena;
-    L.nm_bytes = 3 * E * sizeof(float);
+    L.nm_bytes = 3 * row;
     L.nm_pre = d->pre ? arena : nullptr;
     L.nm_post = d->post ? arena + E : nullptr;
     L.nm_gate = d->gate ? arena + 2 * E : nullptr;

@@ -20,7 +20,7 @@ SOURCES = ["gx_kernels.cu", "gx_decode_stack.cu", "gx_prefill.cu", "gx_gemm_ts.c
            "gx_q4.cu", "gx_norm.cu", "gx_logprobs.cu",
            "gx_comm.cu", "gx_abi.cu", "gx_gguf.cpp"]
 HEADERS = ["gx_tile.h", "gx_device.cuh", "gx_gemv.cuh", "gx_internal.h", "gx_umma.cuh", "gx_comm.h", "gx_dense.cuh",
-           "gx_checks.h", "gx_q4_tc.h"]
+           "gx_checks.h", "gx_q4_tc.h", "gx_upload.h"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden", "--expt-relaxed-constexpr",

@@ -421,7 +421,8 @@ GX_API gx_result gx_logprobs(gx_context *context, const gx_logprobs_desc *desc, 
                              uint64_t *out_ticket);
 
 /* The norms, gate and residual scale of an uploaded layer used as the FFN block of a plain residual
- * stream (desc NULL removes them; gx_upload_layer of the same index does too). Blocking. */
+ * stream (desc NULL removes them; gx_upload_layer of the same index does too). Blocking: the weights are in place when
+ * it returns, and after an error the layer has the norms that it had before. */
 typedef struct gx_norms_desc {
     const float *pre;             /* [n_embd] weights of the norm before the layer, host memory, NULL for 1 */
     const float *post;            /* [n_embd] weights of the norm after it, with post_norm (NULL for 1) */
