@@ -1877,7 +1877,7 @@ GX_API gx_result gx_upload_layer(gx_context *c, uint32_t layer, const gx_layer_d
         sl.gate_expert_bytes = L.gate_expert_bytes;
         sl.down_expert_bytes = L.down_expert_bytes;
         sl.scale = L.scale;
-        GX_CUDA(cudaMemcpy(c->stack_table + layer, &sl, sizeof(sl), cudaMemcpyHostToDevice));
+        GX_CUDA(cudaMemcpyAsync(c->stack_table + layer, &sl, sizeof(sl), cudaMemcpyHostToDevice, c->stream));
     }
     // A re-uploaded layer invalidates captured stacks.
     for (auto &kv : c->graphs) {
@@ -2005,7 +2005,8 @@ GX_API gx_result gx_upload_shared(gx_context *c, uint32_t layer, const gx_shared
     if (r != GX_OK) return r;
     uint8_t *arena = nullptr;
     GX_CUDA(cudaMalloc(&arena, off));
-    cudaError_t e = cudaMemcpy(arena, host.data(), off, cudaMemcpyHostToDevice);
+    // on the stream that reads it: a plain copy of pageable memory may return before it has arrived
+    cudaError_t e = cudaMemcpyAsync(arena, host.data(), off, cudaMemcpyHostToDevice, c->stream);
     if (e != cudaSuccess) {
         cudaFree(arena);
         return fail_cuda(c, e);
@@ -2077,7 +2078,8 @@ GX_API gx_result gx_upload_hc(gx_context *c, uint32_t layer, const gx_hc_desc *d
     if (r != GX_OK) return r;
     uint8_t *arena = nullptr;
     GX_CUDA(cudaMalloc(&arena, off));
-    cudaError_t e = cudaMemcpy(arena, host.data(), off, cudaMemcpyHostToDevice);
+    // on the stream that reads it: a plain copy of pageable memory may return before it has arrived
+    cudaError_t e = cudaMemcpyAsync(arena, host.data(), off, cudaMemcpyHostToDevice, c->stream);
     if (e != cudaSuccess) {
         cudaFree(arena);
         return fail_cuda(c, e);
