@@ -2445,6 +2445,7 @@ GX_API gx_result gx_matvec(gx_context *c, uint32_t handle, const float *x, uint3
     if (n_tok) {
         const Matrix &m = c->mats[handle];
         if (m.type == GX_Q4_0 || m.type == GX_Q4_1) {
+            if (!gx::linear_args_ok(m.rows, m.cols, x, GX_F32, m.cols, n_tok, y, GX_F32, m.rows)) return GX_E_INVALIDARG;
             gx_result r = enqueue_q4(c, m, x, GX_F32, m.cols, n_tok, y, GX_F32, m.rows);
             if (r != GX_OK) return r;
             return record_ticket(c, out_ticket);

@@ -320,7 +320,7 @@ GX_API gx_result gx_decode_blocks(gx_context *context, uint32_t type_id, const v
  * x [n_tok][cols] f32 device, y [n_tok][rows] f32 device, n_tok <= 64. gx_upload_matrix returns
  * a handle (index) owned by the context. Gyro types (144..151): rows a multiple of 8, cols a
  * multiple of 128 up to 2048. GX_Q4_0 and GX_Q4_1: any rows from 1 to 2^24, cols a multiple of
- * 32 up to 65536. */
+ * 32 up to 65536; gx_matvec takes them by the argument rules of gx_linear. */
 GX_API gx_result gx_upload_matrix(gx_context *context, uint32_t type_id, uint32_t rows, uint32_t cols,
                                   const void *packed, uint64_t packed_bytes, uint32_t *out_handle,
                                   uint32_t timeout_ms);
