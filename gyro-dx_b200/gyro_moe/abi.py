@@ -472,9 +472,19 @@ class Context:
         return h.value
 
     def matvec(self, handle: int, x, y) -> int:
+        """gx_matvec: y = W x on contiguous f32 rows, x [n, cols] and y [n, rows], n <= 64."""
+        n, cols, xp, xs, xd = _rows(x)
+        m, rows, yp, ys, yd = _rows(y)
+        if n != m or self._other_shape(handle, rows, cols) or not (xd == yd == GX_F32 and xs == cols and ys == rows):
+            raise ValueError("gx_matvec: contiguous f32 x [n, cols] and y [n, rows] are needed")
+        self._here(x, y)
         t = ctypes.c_uint64()
-        _check(self.lib.gx_matvec(self.handle, handle, _ptr(x), x.shape[0], _ptr(y), ctypes.byref(t)), "gx_matvec")
+        _check(self.lib.gx_matvec(self.handle, handle, xp, n, yp, ctypes.byref(t)), "gx_matvec")
         return t.value
+
+    def _other_shape(self, handle: int, rows: int, cols: int) -> bool:
+        """Whether the matrix has another shape (an unknown handle is the library's to refuse)."""
+        return self.matrices.get(handle, (rows, cols)) != (rows, cols)
 
     # --- operators around the layer ----------------------------------------------------------
     # Device tensors of this context's device, rows in the last dimension; the work is enqueued on the
@@ -495,7 +505,7 @@ class Context:
         """gx_linear: y = W x for a 4-bit matrix, x [n, cols] and y [n, rows] in f32 or bf16, n <= 64."""
         n, cols, xp, xs, xd = _rows(x)
         m, rows, yp, ys, yd = _rows(y)
-        if n != m or (rows, cols) != self.matrices[handle]:
+        if n != m or self._other_shape(handle, rows, cols):
             raise ValueError("gx_linear: x [n, cols] and y [n, rows] are needed")
         self._here(x, y)
         return self._done(self.lib.gx_linear(self.handle, handle, xp, xd, xs, n, yp, yd, ys,
@@ -562,7 +572,7 @@ class Context:
         for k in ("pre", "post", "gate"):
             a = norms.get(k)
             w[k] = None if a is None else np.ascontiguousarray(a, dtype=np.float32)
-            if a is not None and w[k].shape != (self.layers[index]["n_embd"],):
+            if a is not None and index in self.layers and w[k].shape != (self.layers[index]["n_embd"],):
                 raise ValueError(f"{k}: one weight per hidden channel is needed")
         d = NormsDesc(_ptr(w["pre"]), _ptr(w["post"]), _ptr(w["gate"]), int(norms.get("post_norm", True)),
                       norms.get("eps", 1e-6), norms.get("res_scale", 1.0), norms.get("block_scale", 1.0))
