@@ -7,7 +7,9 @@
 // Bound by reading the logits once, 10 instructions a logit. A cluster of CTAs takes a row, each CTA a
 // slice that its threads stream through registers, four 16-byte words ahead. The reference ref need not be
 // the maximum, only near it: it is that of the slice's first words, and a thread that meets a logit more
-// than 2^8 times as likely moves on to a new one. Each lane's maximum in the first words also gives a
+// than 2^8 times as likely moves on to a new one. (It is always a logit of the row: either the largest, and s >= 1
+// and all t <= 0 exactly, or one that weighs 2^-8 of it, and no probability is within roundings of 1. So no log
+// probability comes out above 0 and no entropy below.) Each lane's maximum in the first words also gives a
 // floor for the top, so that few logits are candidates; those enter the warp's sorted list, a key in a
 // lane. The lists and sums meet in shared memory, then in that of the cluster's first CTA. Nothing
 // depends on the order in which threads run.
