@@ -217,14 +217,15 @@ struct Ints {
     // [4 groups][T tokens][4 digits][4 q] 8 B: the digit of columns (0 2 4 6) and (1 3 5 7) of 8 q ..
     static constexpr int GROUP = T * 128, ZERO = 4 * GROUP;       // T == 1: 32 B of zeros
     static constexpr int INIT = ZERO + (T == 1 ? 32 : 0);         // Q4_0: [group][token][digit pair] int4 accumulators
-    static constexpr int SUM = INIT;                              // Q4_1: [group][token][digit pair] float: sum x, 0
+    static constexpr int SUM = INIT;                              // Q4_1: [group][token][digit pair] float: sum x in kUnit, 0
     static constexpr int INV = TYPE == GX_Q4_0 ? INIT + T * 128 : SUM + T * 32;  // [token] float: 2^24 units of the numbers
     static constexpr int BYTES = (INV + T * 4 + 15) / 16 * 16;
     static constexpr uint32_t kOffset = 0x4b400000u;              // 2^23 + 2^22 as a float
+    // Of the lane's sums: with Q4_1 in 32nds, since sum x of a group may pass the f32 range where m sum x does not.
+    static constexpr float kUnit = TYPE == GX_Q4_1 ? 0x1p-5f : 1.f;
 
     int at[4];       // the lane's fragment in each group
-    float w0, w1;    // weights of the digits that its accumulator columns hold
-    float acc[NA];   // rows g and g + 8; T == 2: token q >> 1
+    float acc[NA];   // rows g and g + 8; T == 2: token q >> 1; odd lanes hold the lower two digits, 2^16 times
 
     __device__ __forceinline__ void init(int lane, int nt) {
         const int g = lane >> 2, q = lane & 3;
@@ -232,8 +233,6 @@ struct Ints {
         for (int j = 0; j < 4; ++j)
             at[j] = T == 2 ? j * GROUP + ((g >> 2) < nt ? g : (g & 3)) * 32 + q * 8
                            : (g >> 2 == (j & 1) ? j * GROUP + (g & 3) * 32 : ZERO) + q * 8;
-        w0 = (q & 1) ? 0x1p-16f : 1.f;
-        w1 = (q & 1) ? 0x1p-24f : 0x1p-8f;
     }
     static __device__ __forceinline__ int scale_offset(int lane) {
         return T == 1 ? (lane >> 1) * 4 + (lane >> 2) * 8 : (lane >> 2) * 16;
@@ -255,7 +254,7 @@ struct Ints {
             for (int c = 0; c < 8; ++c) {
                 const float x = e == 255u ? 0.f : v[c] * s1 * s2;
                 b[c] = ((uint32_t)__float2int_rn(x) + 0x00808080u) ^ 0x00808080u;  // signed digits, byte by byte
-                fs += v[c];
+                fs = fmaf(v[c], kUnit, fs);
             }
             uint32_t w[2][4];  // [half of the columns][digit, most significant first]
 #pragma unroll
@@ -293,7 +292,7 @@ struct Ints {
             if ((cell & 15) == 0) {
                 reinterpret_cast<float *>(u + INV)[t] =
                     e == 255u ? __uint_as_float(0x7fffffffu)
-                              : __uint_as_float((uint32_t)(151 - k1) << 23) * __uint_as_float((uint32_t)(127 - k2) << 23);
+                              : __uint_as_float((uint32_t)(151 - k1) << 23) * __uint_as_float((uint32_t)(127 - k2) << 23) * kUnit;
                 if constexpr (T == 1) {
                     reinterpret_cast<uint4 *>(u + ZERO)[0] = make_uint4(0u, 0u, 0u, 0u);
                     reinterpret_cast<uint4 *>(u + ZERO)[1] = make_uint4(0u, 0u, 0u, 0u);
@@ -304,7 +303,7 @@ struct Ints {
     __device__ __forceinline__ void unit(const Unit<TYPE, SETS> &u, const uint8_t *x, int lane) {
         const int q = lane & 3;
         const uint32_t c0[4] = {u.c0.x, u.c0.y, u.c0.z, u.c0.w}, c1[4] = {u.c1.x, u.c1.y, u.c1.z, u.c1.w};
-        const float inv = reinterpret_cast<const float *>(x + INV)[T == 1 ? 0 : q >> 1], v0 = inv * w0, v1 = inv * w1;
+        const float inv = reinterpret_cast<const float *>(x + INV)[T == 1 ? 0 : q >> 1];
         int4 c;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -325,8 +324,9 @@ struct Ints {
             constexpr float off = 12582912.f;
             const float f0 = __int_as_float(c.x) - off, f1 = __int_as_float(c.y) - off;
             const float f2 = __int_as_float(c.z) - off, f3 = __int_as_float(c.w) - off;
-            acc[0] = fmaf(half_value(u.d[set], 0), fmaf(f1, v1, f0 * v0), acc[0]);
-            acc[1] = fmaf(half_value(u.d[set], 1), fmaf(f3, v1, f2 * v0), acc[1]);
+            // d before the unit's power of two: the sum of x by codes alone may pass the f32 range
+            acc[0] = fmaf(half_value(u.d[set], 0) * fmaf(f1, 0x1p-8f, f0), inv, acc[0]);
+            acc[1] = fmaf(half_value(u.d[set], 1) * fmaf(f3, 0x1p-8f, f2), inv, acc[1]);
             if constexpr (TYPE == GX_Q4_1) {
                 const float sx = reinterpret_cast<const float *>(x + SUM)[row];
                 acc[0] = fmaf(half_value(u.m[set], 0), sx, acc[0]);
@@ -338,6 +338,7 @@ struct Ints {
         const int g = lane >> 2, q = lane & 3;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
+            acc[k] *= (q & 1) ? 0x1p-16f / kUnit : 1.f / kUnit;
             acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], 1);
             if (T == 1) acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], 2);
         }

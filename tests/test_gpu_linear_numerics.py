@@ -62,3 +62,50 @@ def test_batch_sums_are_kept_in_f32(ctx, kind, n, xk):
     exact = x.double() @ torch.from_numpy(w).cuda().T
     y = linear(ctx, h, x, rows, torch.float32).double()
     assert float(((y - exact).abs() / exact).max()) <= 20 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("kind", [refs.Q4_0, refs.Q4_1])
+@pytest.mark.parametrize("xk", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 2, 3, 7, 20, 40])
+def test_activations_near_the_end_of_the_range(ctx, kind, xk, n):
+    """Activations up to the largest f32 by small weights: every sum of the definition is finite, and so are the results."""
+    rows, cols = 70, 2080
+    rng = np.random.default_rng(n)
+    g = cols // 32
+    q = rng.integers(0, 16, (rows, g, 32), dtype=np.uint8)
+    half = [(rng.choice([-1, 1], (rows, g, 1)) * 2.0 ** rng.uniform(-23, -19, (rows, g, 1))).astype(np.float16) for _ in range(kind - 1)]
+    packed = np.concatenate([h.view(np.uint8) for h in half] + [q[..., :16] | (q[..., 16:] << 4)], axis=2).reshape(rows, -1)
+    w, mag = refs.q4_weights(packed, kind, cols)
+    h = ctx.upload_matrix(kind, rows, cols, packed)
+    for low, high in [(1e33, 1e35), (1e35, 3e37), (3e37, 3.38e38)]:
+        x = rng.choice([-1, 1], (n, cols)) * np.exp(rng.uniform(np.log(low), np.log(high), (n, cols)))
+        x[0] = np.abs(x[0])
+        x = refs.to_kind(x.astype(np.float32), xk)
+        assert np.isfinite(x).all()
+        xd = torch.from_numpy(x).to(torch.bfloat16 if xk == "bf16" else torch.float32).cuda()
+        want, bound = refs.linear(x, w, mag, "f32")
+        assert np.abs(want).max() < 3e38
+        y = linear(ctx, h, xd, rows, torch.float32).cpu().numpy().astype(np.float64)
+        assert np.isfinite(y).all() and (np.abs(y - want) <= bound).all(), (low, high)
+
+
+@pytest.mark.parametrize("kind", [refs.Q4_0, refs.Q4_1])
+@pytest.mark.parametrize("xk", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 2, 3, 7, 20, 40])
+def test_activations_near_the_smallest(ctx, kind, xk, n):
+    """Activations around the smallest normal f32 by large weights: results of ordinary relative error."""
+    rows, cols = 70, 2080
+    rng = np.random.default_rng(n)
+    g = cols // 32
+    q = rng.integers(0, 16, (rows, g, 32), dtype=np.uint8)
+    half = [(rng.choice([-1, 1], (rows, g, 1)) * rng.uniform(3e4, 6.5e4, (rows, g, 1))).astype(np.float16) for _ in range(kind - 1)]
+    packed = np.concatenate([h.view(np.uint8) for h in half] + [q[..., :16] | (q[..., 16:] << 4)], axis=2).reshape(rows, -1)
+    w, mag = refs.q4_weights(packed, kind, cols)
+    h = ctx.upload_matrix(kind, rows, cols, packed)
+    for size in (1e-38, 1e-36, 1e-33):
+        x = refs.to_kind((rng.standard_normal((n, cols)) * size).astype(np.float32), xk)
+        xd = torch.from_numpy(x).to(torch.bfloat16 if xk == "bf16" else torch.float32).cuda()
+        want, bound = refs.linear(x, w, mag, "f32")
+        y = linear(ctx, h, xd, rows, torch.float32).cpu().numpy().astype(np.float64)
+        # a sum is kept in steps of 2^-144 or less (32 times the smallest f32), one half a step lost for each group
+        assert (np.abs(y - want) <= bound + cols / 32 * 2.0 ** -144).all(), size
