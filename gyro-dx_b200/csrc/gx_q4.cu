@@ -701,17 +701,17 @@ cudaError_t launch_gemv(const Q4Args &a, int sm_count, cudaStream_t s) {
 // No weight and no activation is rounded.
 //
 // (With d applied to each group's sum afterwards, as in the GEMV, the product needs an accumulator a group,
-// read back by warps that multiply: 42 us alone on a stream against 26, 64 bf16 tokens by 8192 x 8192, and
-// 48 to 62 on mma.sync.)
+// read back by warps that multiply: 42 us alone on a stream, 64 bf16 tokens by 8192 x 8192, and 48 to 62 on
+// mma.sync; this one takes 28.7.)
 //
-// What bounds it: the chain of one unit (128 columns) in the issuing thread, two waits, 16 MMAs and two
-// commits, 0.5 us; the MMAs at their full rate would take 0.15 us, the codes' bytes 0.18. So a unit has
+// What bounds it: the chain of one unit (128 columns) in the issuing thread, three waits, 16 MMAs and three
+// commits, more than 0.5 us; the MMAs at their full rate would take 0.15 us, the codes' bytes 0.18. So a unit has
 // one full and one empty barrier for its weights, its codes come by one bulk copy (a copy for each of its 8
 // row tiles kept the copying thread 0.9 us a unit), and one thread runs the issue loop by itself (a whole
-// warp with an elected lane: 32 us against 28).
+// warp with an elected lane took 4 us more, measured with one accumulator over all units).
 //
 // Warps: 0 copies, 1 tensor memory and MMA issue, then sets of four decoders that take units in turn, and four
-// that read the sums. Three sets: 25.4 us, two: 25.7 (8192 x 8192, 64 bf16 tokens).
+// that read the sums. Three sets: 28.7 us, two: 29.2 (8192 x 8192, 64 bf16 tokens).
 constexpr int kTcRows = kTileRows * kBlockTiles;
 // An accumulator takes one unit and is then read and added in registers. The tensor core cuts its sum off after each
 // of a unit's 16 MMAs, always towards zero. Relative error in the 2-norm before the results are rounded (64 bf16 tokens
@@ -1102,7 +1102,7 @@ cudaError_t launch_tc(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s
     p.blocks = (p.RT + 7) / 8;
     // One CTA an SM. Where row blocks leave SMs idle, the CTAs of a cluster split the units (down to two a
     // CTA). 148 SMs take 130 to 135 CTAs at once in clusters of 3 to 6, but 120 in clusters of 8: 16 row blocks
-    // of 8192 columns by 64 tokens took 24 us with 8 (two waves), 15.8 with 6.
+    // of 8192 columns by 64 tokens took 25.5 us with 8 (two waves), 16.2 with 6.
     p.S = 1;
     for (int c = 2; c <= 6; ++c)
         if (p.blocks * c <= (c == 2 ? sm_count : sm_count * 7 / 8) && p.KT >= 2 * c) p.S = c;
@@ -1132,8 +1132,8 @@ cudaError_t launch_tc(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s
 
 // The GEMV takes up to 16 product columns (a token is one in bf16, two in f32), but every CTA stages the
 // activations for itself, which from 48 K of them costs more than the product's two launches: 8192 x 8192 by 3, 5,
-// 8 tokens of f32 take 26.7, 50, 56 us there and 20.5, 20.7, 21.1 here; 8192 x 2048 takes 6.6, 6.5, 7.2 there and
-// 9.5, 9.8, 9.9 here. One and two tokens (Ints) are always the GEMV's: 8192 x 8192 11.4 and 12.8 us.
+// 8 tokens of f32 take 28.2, 51.5, 57.3 us there and 24.0, 24.3, 24.6 here; 8192 x 2048 takes 6.8, 6.4, 7.0 there and
+// 10.4, 10.6, 10.7 here. One and two tokens (Ints) are always the GEMV's: 8192 x 8192 11.7 and 12.8 us.
 template <uint32_t TYPE, bool XB>
 cudaError_t launch_tokens(const Q4Args &a, uint8_t *ws, int sm_count, cudaStream_t s) {
     const int n = a.n_tok, columns = XB ? n : 2 * n;

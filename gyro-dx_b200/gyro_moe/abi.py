@@ -488,7 +488,9 @@ class Context:
 
     # --- operators around the layer ----------------------------------------------------------
     # Device tensors of this context's device, rows in the last dimension; the work is enqueued on the
-    # context's stream. Each returns the ticket, or 0 with ticket=False (calls captured into a graph).
+    # context's stream, which no stream of torch waits for or is waited for by: synchronise (or record and wait
+    # for an event on ctx.stream()) between what torch enqueues on the tensors and the call, and wait for the
+    # ticket before torch reads the results. Each returns the ticket, or 0 with ticket=False (calls captured into a graph).
     def _here(self, *tensors) -> None:
         """The tensors have to lie on this context's device: a kernel would fault on any other address."""
         dev = self.device

@@ -350,7 +350,8 @@ GX_API gx_result gx_linear(gx_context *context, uint32_t handle, const void *x, 
 
 /* Norm before a block: y[t] = x[t] / sqrt(mean(x[t]^2) + eps) * weight (src/kernels.zig:281-291),
  * and, with gate_weight, the block's gate logit gate[t] = sum_i gate_weight[i] * y[t][i] (from the
- * unrounded y). Rows of n_embd values, 1..65536, at any number of tokens. */
+ * unrounded y). Rows of n_embd values, 1..65536, at up to 2^24 tokens. Squares are summed in f32, here and in
+ * gx_norm_residual: a row whose sum of squares passes its range (values of about 1e19 and more) gives zeros. */
 typedef struct gx_norm_desc {
     const void *x;                /* [n_tok][n_embd] */
     void *y;                      /* [n_tok][n_embd]; may be x itself (same pointer, stride and encoding) */
@@ -368,7 +369,8 @@ GX_API gx_result gx_norm(gx_context *context, const gx_norm_desc *desc, uint32_t
  *   v = y[t], or y[t] / sqrt(mean(y[t]^2) + eps) * post          (GX_RES_POST_NORM)
  *   r = res_scale * res[t] + block_scale * gate * v,  gate = 1, sigmoid(g[t]) or sigmoid(g[t][i])
  *   res_out[t] = r;   out[t] = r / sqrt(mean(r^2) + eps) * next;  next_gate[t] = next_gate_weight . out[t]
- * The next norm sees r before it is rounded to res_out's encoding. */
+ * The next norm sees r before it is rounded to res_out's encoding. A gate logit of -88 or less, -Inf among them, is a
+ * gate of 0; one of NaN makes a NaN. */
 enum { GX_RES_POST_NORM = 1u };
 enum { GX_GATE_NONE = 0, GX_GATE_TOKEN = 1, GX_GATE_ELEMENT = 2 };
 typedef struct gx_residual_desc {
