@@ -716,8 +716,8 @@ constexpr int kTcRows = kTileRows * kBlockTiles;
 // An accumulator takes one unit and is then read and added in registers. The tensor core cuts its sum off after each
 // of a unit's 16 MMAs, always towards zero. Relative error in the 2-norm before the results are rounded (64 bf16 tokens
 // by 8192 x 8192, Q4_0 and Q4_1; a product of the unpacked weights in f32 has 1.5e-6), and time with bf16 results:
-//   one unit 1.3e-7, 2.4e-7, 29.3 us;  four 6.2e-7, 8.6e-7, 28.0;  sixteen 2.7e-6, 3.6e-6, 27.7
-// (64 f32 tokens: 56.9, 45.9, 43.2 us). Sixteen would do for bf16 results, but put twice as many of them on the other
+//   one unit 1.3e-7, 2.4e-7, 28.7 us;  four 6.2e-7, 8.6e-7, 28.0;  sixteen 2.7e-6, 3.6e-6, 27.7
+// (64 f32 tokens: 57.9, 45.9, 43.2 us). Sixteen would do for bf16 results, but put twice as many of them on the other
 // side of a rounding's border as the product in f32 does; with one, a bf16 result is the f32 result rounded.
 constexpr int kQ4InvBytes = 64 * 4;  // of a workspace: the tokens' inverse scales, before the first unit
 constexpr int kPackThreads = 512;
